@@ -73,11 +73,12 @@ def init_random(loaded: LoadedModel, seed: int) -> LoadedModel:
 
 def build_engine(loaded: LoadedModel, *, max_batch: int = 1, max_seq_len: Optional[int] = None,
                  max_tokens: Optional[int] = None, use_cuda_graph: bool = True,
-                 options: KernelOptions = DEFAULT_OPTIONS) -> Engine:
+                 options: KernelOptions = DEFAULT_OPTIONS, kv_cache: Optional[str] = None) -> Engine:
     """The counterpart of the reference's ``build_cache``: cache and step function for a loaded model.
-    ``options`` chooses kernels where there is a choice (``KernelOptions``)."""
+    ``options`` chooses kernels where there is a choice (``KernelOptions``).  ``kv_cache``: None, "int8" or
+    "int4", what keys and values are held in (None: the compute dtype)."""
     return Engine(loaded.model, max_batch=max_batch, max_seq_len=max_seq_len, max_tokens=max_tokens,
-                  use_cuda_graph=use_cuda_graph, options=options)
+                  use_cuda_graph=use_cuda_graph, options=options, kv_cache=kv_cache)
 
 
 def generate(prompt_ids: Sequence[int], engine: Engine, max_new_tokens: int = 256, temperature: float = 1.0,

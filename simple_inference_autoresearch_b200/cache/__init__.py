@@ -1,3 +1,3 @@
 """Slots, paged keys and values, fixed-size per-sequence state."""
-from .sequence_cache import (CacheError, FreeList, KVEntry, KVGroup, SequenceCache, StateEntry,  # noqa: F401
-                             StateGroup, round_up)
+from .sequence_cache import (CacheError, FreeList, KV_FORMATS, KVEntry, KVGroup, QuantizedKVEntry,  # noqa: F401
+                             SequenceCache, StateEntry, StateGroup, round_up)

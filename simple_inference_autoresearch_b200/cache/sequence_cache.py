@@ -85,6 +85,44 @@ class KVEntry:
     page_tokens: int
 
 
+#: formats a cache may hold its keys and values in besides the compute type
+KV_FORMATS = ("int8", "int4")
+#: dims of a row that share a scale in the 4-bit format
+KV_GROUP = 64
+
+
+@dataclass
+class QuantizedKVEntry:
+    """A cache entry whose keys and values are held in 8 or 4 bits; goes wherever a ``KVEntry`` goes
+    (``ops.rope_kv_write``, ``ops.attention``, ``ops.rope_and_attention``, ``ops.read_kv``).  A row is
+    one position of one kv head.
+
+    * 8 bits: ``k``, ``v`` int8 ``[n_pages, kv_heads, page_tokens, head_dim]``; ``k_scale``, ``v_scale``
+      float32 ``[n_pages, kv_heads, page_tokens]``; a value is ``code * scale``, ``scale = max|row| / 127``.
+    * 4 bits: ``k``, ``v`` uint8 ``[..., head_dim / 2]`` (dim 2i in the low half of byte i); ``k_scale``,
+      ``v_scale`` bfloat16 ``[n_pages, kv_heads, page_tokens, ceil(head_dim / 64), 2]``, for every run of
+      64 dims ``(scale, mid)``; a value is ``(code - 8) * scale + mid``.
+
+    Keys are quantised after their rotation, once; a row that holds an infinity or a NaN reads back as
+    NaN (4 bits: the run of 64 dims that holds it).  The reference's int8 cache has the same row scale
+    (model/kv_cache.py:58-67), held in 16 bits."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    block_table: torch.Tensor
+    page_tokens: int
+
+    @property
+    def bits(self) -> int:
+        return 8 if self.k.dtype == torch.int8 else 4
+
+    @property
+    def head_dim(self) -> int:
+        return self.k.shape[-1] * (1 if self.bits == 8 else 2)
+
+
 @dataclass
 class StateEntry:
     """Fixed-size per-sequence state of one cache entry: ``[n_slots, *shape]``,
@@ -95,23 +133,45 @@ class StateEntry:
 
 class KVGroup:
     def __init__(self, need: KVNeed, n_entries: int, n_slots: int, n_pages: int, max_pages_per_seq: int,
-                 page_tokens: int, dtype: torch.dtype, device):
+                 page_tokens: int, dtype: torch.dtype, device, kv_format: Optional[str] = None):
         if need.window is not None and need.window <= 0:
             raise CacheError(f"a window of keys must be positive, got {need.window}")
+        if kv_format is not None and kv_format not in KV_FORMATS:
+            raise CacheError(f"a cache holds keys and values in the compute dtype (None) or as one of "
+                             f"{', '.join(KV_FORMATS)}, got {kv_format!r}")
+        if kv_format is not None and (need.v_head_dim or need.head_dim) != need.head_dim:
+            raise CacheError(f"a cache in {kv_format} holds keys and values of one width, got {need.head_dim} and "
+                             f"{need.v_head_dim}")
+        if kv_format is not None and (need.head_dim % 16 or not 0 < need.head_dim <= 256):
+            raise CacheError(f"a cache in {kv_format} takes head_dim in steps of 16 up to 256, got {need.head_dim}")
+        self.kv_format = kv_format
         self.need = need
         self.n_entries = n_entries
         self.page_tokens = page_tokens
         self.max_pages_per_seq = max_pages_per_seq
         self.pages = FreeList(n_pages, "cache page")
         shape = (n_entries, n_pages, need.n_kv_heads, page_tokens)
-        self.k = torch.zeros(shape + (need.head_dim,), dtype=dtype, device=device)
-        self.v = torch.zeros(shape + (need.v_head_dim or need.head_dim,), dtype=dtype, device=device)
+        z = lambda width, dt: torch.zeros(shape + width, dtype=dt, device=device)  # noqa: E731
+        self.k_scale = self.v_scale = None
+        if kv_format == "int8":
+            self.k, self.v = z((need.head_dim,), torch.int8), z((need.head_dim,), torch.int8)
+            self.k_scale, self.v_scale = z((), torch.float32), z((), torch.float32)
+        elif kv_format == "int4":
+            groups = (-(-need.head_dim // KV_GROUP), 2)
+            self.k, self.v = z((need.head_dim // 2,), torch.uint8), z((need.head_dim // 2,), torch.uint8)
+            self.k_scale, self.v_scale = z(groups, torch.bfloat16), z(groups, torch.bfloat16)
+        else:
+            self.k = z((need.head_dim,), dtype)
+            self.v = z((need.v_head_dim or need.head_dim,), dtype)
         # -1 marks "no page"; the cache-write kernel flags a write through it.
         self.block_table = torch.full((n_slots, max_pages_per_seq), -1, dtype=torch.int32, device=device)
         # per slot: the page of every page index so far; None once a windowed group gave it back
         self.slot_pages: Dict[int, List[Optional[int]]] = {}
 
-    def entry(self, i: int) -> KVEntry:
+    def entry(self, i: int):
+        if self.kv_format is not None:
+            return QuantizedKVEntry(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i], self.block_table,
+                                    self.page_tokens)
         return KVEntry(self.k[i], self.v[i], self.block_table, self.page_tokens)
 
     def open_slot(self, slot: int) -> None:
@@ -165,7 +225,7 @@ class KVGroup:
         return [(slot, idx, -1) for idx, p in enumerate(pages) if p is not None]
 
     def bytes(self) -> int:
-        return (self.k.numel() + self.v.numel()) * self.k.element_size()
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
 
 class StateGroup:
@@ -195,10 +255,13 @@ class SequenceCache:
     ``needs``: one need (or None) per cache entry, in the model's entry order.
     ``max_tokens``: the most positions live sequences hold at any time, each
     sequence's count rounded up to ``page_tokens``.
+    ``kv_format``: None holds keys and values in ``dtype``, "int8" or "int4" in 8 or 4 bits (all
+    groups of keys and values; see ``QuantizedKVEntry``).
     """
 
     def __init__(self, needs: Sequence[object], max_tokens: int, max_slots: int, max_seq_len: int,
-                 dtype: torch.dtype, device, page_tokens: int = DEFAULT_PAGE_TOKENS):
+                 dtype: torch.dtype, device, page_tokens: int = DEFAULT_PAGE_TOKENS,
+                 kv_format: Optional[str] = None):
         if max_tokens <= 0 or max_slots <= 0 or max_seq_len <= 0:
             raise CacheError("max_tokens, max_slots and max_seq_len must be positive")
         self.page_tokens = page_tokens
@@ -206,7 +269,7 @@ class SequenceCache:
         self.n_slots = min(max_slots, self.n_pages)
         # the caller's limit stands as given (only the page count is rounded up)
         self.max_seq_len = min(int(max_seq_len), self.n_pages * page_tokens)
-        self.dtype, self.device = dtype, device
+        self.dtype, self.device, self.kv_format = dtype, device, kv_format
         self.slots = FreeList(self.n_slots, "cache slot")
         self.lengths: Dict[int, int] = {}
         self.groups: List[object] = []
@@ -219,7 +282,7 @@ class SequenceCache:
         for need, entries in by_need.items():
             if isinstance(need, KVNeed):
                 g = KVGroup(need, len(entries), self.n_slots, self.n_pages,
-                            -(-self.max_seq_len // page_tokens), page_tokens, dtype, device)
+                            -(-self.max_seq_len // page_tokens), page_tokens, dtype, device, kv_format)
             elif isinstance(need, StateNeed):
                 g = StateGroup(need, len(entries), self.n_slots, device)
             else:

@@ -424,6 +424,13 @@ static int launch_decode(const void* qkv, const void* k_pool, const void* v_pool
   return (int)cudaGetLastError();
 }
 
+// 1 when a block of the decode kernel holds the group's state in shared memory (many query heads of a
+// wide 32-bit head do not fit; the prompt kernel takes those sizes).
+extern "C" int siar_attn_decode_fits(int is_bf16, int Hq, int Hkv, int D) {
+  if (Hkv <= 0 || Hq % Hkv != 0) return 0;
+  return (is_bf16 ? decode_smem_bytes<__nv_bfloat16>(Hq / Hkv, D) : decode_smem_bytes<float>(Hq / Hkv, D)) <= 200 * 1024;
+}
+
 // One new token per sequence.  max_kv_len bounds base_len[b] + 1 over the batch
 // and fixes the grid and the scratch layout (so a captured launch stays valid
 // while lengths grow up to it).

@@ -41,10 +41,12 @@ class Engine:
     def __init__(self, model: DecoderModel, max_batch: int = 8, max_seq_len: Optional[int] = None,
                  max_tokens: Optional[int] = None, max_slots: Optional[int] = None, page_tokens: int = DEFAULT_PAGE_TOKENS,
                  use_cuda_graph: bool = True, options: KernelOptions = DEFAULT,
-                 beyond_trained_positions: bool = False):
+                 beyond_trained_positions: bool = False, kv_cache: Optional[str] = None):
         """``beyond_trained_positions``: let ``max_seq_len`` exceed the configuration's
         ``max_position_embeddings`` (nothing in the kernels depends on it: rotation angles are computed
-        from the position; it is the length the model was trained for, and the default refuses more)."""
+        from the position; it is the length the model was trained for, and the default refuses more).
+        ``kv_cache``: None holds keys and values in the compute dtype, "int8" or "int4" in 8 or 4 bits
+        (``cache.QuantizedKVEntry``)."""
         self.model = model
         self.options = options        # which kernel runs where there is a choice (this engine's steps only)
         self.device = model.device
@@ -57,7 +59,7 @@ class Engine:
         if max_tokens is None:
             max_tokens = self.max_batch * round_up(max_seq_len, page_tokens)
         self.cache = SequenceCache(model.cache_needs, int(max_tokens), int(max_slots or self.max_batch),
-                                   max_seq_len, model.dtype, self.device, page_tokens)
+                                   max_seq_len, model.dtype, self.device, page_tokens, kv_cache)
         self.max_seq_len = self.cache.max_seq_len
         self.use_cuda_graph = bool(use_cuda_graph)
         self._graphs: Dict[Tuple[int, int], "_DecodeGraph"] = {}      # in order of last use

@@ -17,7 +17,8 @@ added with ``config.register_preset``, of whatever registered architecture its c
 seeded random weights made on the GPU (``--seed``; ``--norm-init`` overrides the configuration's rule for norm weights); ``--prompt-len N`` feeds N seeded random
 token ids; ``--batch N`` generates for N prompts at once (``--prompt-len`` draws N different
 ones, their lengths spread between N/2 and N tokens; a given prompt is repeated) and prints the token
-lists instead of streaming; ``--stop-id ID`` (repeatable) adds stop tokens to the model's own.
+lists instead of streaming; ``--stop-id ID`` (repeatable) adds stop tokens to the model's own;
+``--kv-cache int8`` or ``int4`` holds keys and values in 8 or 4 bits.
 """
 
 from __future__ import annotations
@@ -59,6 +60,8 @@ def main(argv=None) -> int:
     ap.add_argument("--stop-id", type=int, action="append", default=[], help="a further stop token id (repeatable)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--ignore-eos", action="store_true", help="do not stop at the model's stop tokens")
+    ap.add_argument("--kv-cache", choices=["int8", "int4"],
+                    help="hold keys and values in 8 or 4 bits (default: in --dtype)")
     ap.add_argument("--no-cuda-graph", action="store_true")
     args = ap.parse_args(argv)
     if args.batch < 1:
@@ -100,7 +103,7 @@ def main(argv=None) -> int:
         ap.error("one of --prompt / --prompt-ids / --prompt-len is required")
     engine = siar.build_engine(loaded, max_batch=args.batch,
                                max_seq_len=max(len(p) for p in prompts) + args.max_new_tokens,
-                               use_cuda_graph=not args.no_cuda_graph)
+                               use_cuda_graph=not args.no_cuda_graph, kv_cache=args.kv_cache)
     if args.batch > 1:
         params = siar.SamplingParams(args.temperature, args.top_k, args.top_p, args.seed)
         outs, stats = engine.generate(prompts, params, args.max_new_tokens, stop_token_ids=args.stop_id or None,

@@ -47,6 +47,7 @@ _signatures = {
         "siar_attn_decode": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                              c_void_p, c_void_p],
+        "siar_attn_decode_fits": [c_int, c_int, c_int, c_int],
         "siar_attn_decode_chunk": [],
         "siar_attn_max_head_dim": [],
     },
@@ -69,6 +70,18 @@ _signatures = {
                                  c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
                                  c_void_p],
         "siar_attn_tc_supported": [c_int, c_int, c_int, c_int],
+    },
+    "kv_quant": {
+        # is_bf16, bits, qkv, q_out, inv_freq, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len,
+        # N, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, write_kv, status, stream, rotary_dim, interleaved
+        "siar_rope_quantize": [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                               c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int],
+        # is_bf16, bits, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, k_out, v_out, out_table,
+        # out_slots, B, Hkv, D, page_tokens, max_pages, n_pages, pages_out, max_kv_len, window, status, stream
+        "siar_read_kv": [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                         c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                         c_int, c_int, c_void_p, c_void_p],
     },
     "sampling": {
         "siar_sample": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -101,6 +114,24 @@ def _launch(unit: str, name: str, *args, kernels: int = 1) -> None:
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    """Stands for the current device where a tensor already lives on it."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_here = _Here()
+
+
+def _on_device(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one (its stream and launches are then that device's)."""
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -371,10 +402,16 @@ def _check_if_asked(options: KernelOptions, kv, meta, n_rows: int, writes: bool,
 
 
 def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads: int,
-                  head_dim: int, write_kv: bool = True, options: KernelOptions = DEFAULT) -> None:
+                  head_dim: int, write_kv: bool = True, options: KernelOptions = DEFAULT,
+                  q_out: Optional[torch.Tensor] = None) -> None:
     """Rotates the q (in place) and k heads of the fused ``qkv`` rows by their
     positions and writes k and v into the pages of ``kv`` (a cache entry).  ``rotary``: see
-    ``rotary_layout``; every layout it describes is taken."""
+    ``rotary_layout``; every layout it describes is taken.  A ``QuantizedKVEntry`` gets k and v as codes
+    and scales; there ``q_out`` (a tensor like ``qkv``) takes the rotated queries and leaves ``qkv`` as it is."""
+    if kv_quant.is_quantized(kv):
+        return kv_quant.rope_kv_write(qkv, rotary, kv, meta, n_heads, n_kv_heads, head_dim, write_kv, options, q_out)
+    if q_out is not None:
+        raise ValueError("q_out goes with a quantised cache entry; this one's queries are rotated in place")
     inv_freq, rotary_dim, interleaved = rotary_layout(rotary, head_dim)
     _need_cuda(qkv, inv_freq, kv.k)
     n = qkv.shape[0]
@@ -474,7 +511,10 @@ def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_h
     sequence on the tensor-core path this is ONE kernel (q is rotated in registers, the new k and
     v go to the cache and are used from shared memory); otherwise two.  The one kernel rotates whole
     heads in pairs (i, i + head_dim/2) only: any other rotary layout (see ``rotary_layout``) takes the
-    two-kernel way.  ``window``: see ``attention``."""
+    two-kernel way.  ``window``: see ``attention``.  ``qkv`` may be changed (its queries rotated)."""
+    if kv_quant.is_quantized(kv):
+        return kv_quant.rope_and_attention(qkv, rotary, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv,
+                                           window, options)
     inv_freq, rotary_dim, interleaved = rotary_layout(rotary, head_dim)
     plain_layout = inv_freq is None or (rotary_dim == head_dim and not interleaved)
     if window is not None or not plain_layout or not decode_fuses_rope(meta, qkv.dtype, n_heads, n_kv_heads, head_dim,
@@ -504,7 +544,10 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     """Causal attention of the new tokens' (already rotated) queries over the
     cache entry ``kv``; returns [N, n_heads * head_dim] in qkv's dtype.  bfloat16
     with head_dim 64 or 128 runs on the tensor cores, everything else on the CUDA cores.
-    ``window`` = w: a query at position p sees keys p - w + 1 .. p only (CUDA-core kernels)."""
+    ``window`` = w: a query at position p sees keys p - w + 1 .. p only (CUDA-core kernels).
+    A ``QuantizedKVEntry`` is read back as pages of qkv's dtype first (``read_kv``)."""
+    if kv_quant.is_quantized(kv):
+        return kv_quant.attention(qkv, kv, meta, n_heads, n_kv_heads, head_dim, scale, window, options)
     if window is not None and window <= 0:
         raise ValueError(f"an attention window must be positive, got {window}")
     _need_cuda(qkv, kv.k)
@@ -543,6 +586,16 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
         _launch("attention", "siar_attn_prefill", _is_bf16(qkv.dtype), _ptr(qkv), _ptr(kv.k), _ptr(kv.v), *common,
                 _ptr(out), *sizes, meta.max_q_len, win, float(scale), _stream(), _ptr(status_word(qkv.device)))
     return out
+
+
+def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options: KernelOptions = DEFAULT):
+    """The keys and values that the batch's sequences hold in a ``QuantizedKVEntry`` (the ones this step
+    brings among them: ``base_len`` plus the new tokens), as a ``KVEntry`` of ``dtype`` (bfloat16 or float32):
+    sequence b's pages stand one behind the other, in the order of the batch, and row b of the block
+    table names them (-1 beyond its last).  Rows of a page behind the last token are zeros.  With
+    ``window`` = w, pages that lie wholly in front of the first new token's window are not read and get
+    cell -1; their places in the pools are not written."""
+    return kv_quant.read_kv(kv, meta, dtype, window, options)
 
 
 def swiglu(gate_up: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
@@ -609,3 +662,6 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     _launch("sampling", "siar_sample", _ptr(logits), r, v, _ptr(temperature), _ptr(top_k), _ptr(top_p),
             _ptr(seeds), _ptr(draw_index), int(advance_index), _ptr(out), _stream())
     return out
+
+
+from . import kv_quant  # noqa: E402  (its functions call this module's)

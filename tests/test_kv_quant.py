@@ -1,0 +1,144 @@
+"""A cache held in 8 or 4 bits, without a GPU: storage and accounting, what the functions refuse, and the
+engine's logic over it with the plain restatements in place of the kernels."""
+
+import math
+
+import pytest
+import torch
+
+import simple_inference_autoresearch_b200 as siar
+from simple_inference_autoresearch_b200.cache import CacheError, QuantizedKVEntry, SequenceCache
+from simple_inference_autoresearch_b200.kernels import kv_quant, ops
+from simple_inference_autoresearch_b200.parts.base import KVNeed, StateNeed
+from tests import emulated_kv_quant as eq
+from tests import plain_llama, tiny_configs
+
+
+def cache(kv_format, need=KVNeed(2, 80), **kw):
+    return SequenceCache([need, need, StateNeed((3,))], 640, 4, 256, torch.bfloat16, "cpu", kv_format=kv_format, **kw)
+
+
+@pytest.mark.parametrize("kv_format,row", [("int8", 80 + 4), ("int4", 40 + 2 * 4)])
+def test_entries_and_bytes(kv_format, row):
+    c = cache(kv_format)
+    e = c.entry(0)
+    assert isinstance(e, QuantizedKVEntry) and e.bits == int(kv_format[3:]) and e.head_dim == 80
+    kv_quant.check_entry(e, 2, 80, e.k.device)
+    assert c.entry(1).k.data_ptr() != e.k.data_ptr() and c.entry(2).state.shape == (4, 3)
+    assert c.groups[0].bytes() == 2 * 2 * 10 * 2 * 64 * row          # entries, k and v, pages, heads, positions
+    assert not eq.values(e.k, e.k_scale).any() or kv_format == "int4"
+    s = c.alloc()
+    c.reserve([s], [130])
+    c.commit([s], [130])
+    assert c.groups[0].held_pages(s) == 3
+    c.free(s)
+    assert c.groups[0].pages.held == 0
+
+
+def test_what_a_cache_refuses():
+    with pytest.raises(CacheError, match="int8, int4"):
+        cache("fp8")
+    with pytest.raises(CacheError, match="one width"):
+        cache("int8", KVNeed(2, 64, v_head_dim=32))
+    with pytest.raises(CacheError, match="steps of 16"):
+        cache("int4", KVNeed(2, 20))
+    with pytest.raises(CacheError, match="steps of 16"):
+        cache("int8", KVNeed(2, 272))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_what_the_functions_refuse(bits):
+    b = eq.Batch(bits, 4, 2, 64, [70, 3], [1, 1])
+    run = lambda kv=b.kv, qkv=b.qkv, heads=4, **kw: ops.rope_and_attention(  # noqa: E731
+        qkv, None, kv, b.meta(), heads, 2, 64, 0.125, **kw)
+    with pytest.raises(RuntimeError, match="CUDA device only"):
+        run()
+    with pytest.raises(RuntimeError, match="CUDA device only"):
+        ops.read_kv(b.kv, b.meta(), torch.bfloat16)
+    with pytest.raises(ValueError, match="not a multiple"):
+        run(heads=5)
+    with pytest.raises(ValueError, match="qkv must be"):
+        run(qkv=b.qkv[:1])
+    with pytest.raises(ValueError, match="contiguous"):
+        run(qkv=torch.empty(512, 2, dtype=torch.bfloat16).t())
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        run(qkv=b.qkv.half())
+    with pytest.raises(ValueError, match="window"):
+        run(window=0)
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        ops.read_kv(b.kv, b.meta(), torch.float16)
+    with pytest.raises(ValueError, match="window"):
+        ops.read_kv(b.kv, b.meta(), torch.bfloat16, window=-1)
+    with pytest.raises(ValueError, match="q_out"):
+        ops.rope_kv_write(b.qkv, None, b.kv, b.meta(), 4, 2, 64, q_out=torch.empty(2, 64, dtype=torch.bfloat16))
+
+    def changed(**kw):
+        e = b.entry()
+        return QuantizedKVEntry(**{**{n: getattr(e, n) for n in ("k", "v", "k_scale", "v_scale", "block_table", "page_tokens")}, **kw})
+
+    for entry, words in ((changed(v=b.kv.v[:1]), "v of a cache entry"), (changed(k=b.kv.k.float()), "int8 .8 bits. or uint8"),
+                         (changed(k_scale=b.kv.k_scale.double()), "k_scale"), (changed(v_scale=b.kv.v_scale[:, :1]), "v_scale"),
+                         (changed(k=b.kv.k.transpose(1, 2).contiguous().transpose(1, 2)), "contiguous"),
+                         (changed(block_table=b.kv.block_table.long()), "block_table"),
+                         (changed(block_table=b.kv.block_table.t()), "block_table"), (changed(page_tokens=32), "k of a cache entry")):
+        with pytest.raises(ValueError, match=words):
+            run(kv=entry)
+
+
+def test_an_ordinary_entry_has_no_read_back_and_rotates_in_place():
+    c = SequenceCache([KVNeed(2, 16)], 64, 1, 64, torch.float32, "cpu")
+    b = eq.Batch(8, 4, 2, 16, [0], [1], dtype=torch.float32)
+    with pytest.raises(TypeError, match="quantised cache entry"):
+        ops.read_kv(c.entry(0), b.meta(), torch.float32)
+    with pytest.raises(ValueError, match="q_out"):
+        ops.rope_kv_write(b.qkv, None, c.entry(0), b.meta(), 4, 2, 16, q_out=b.qkv)
+
+
+@pytest.mark.parametrize("bits,step", [(8, 1 / 127), (4, 1 / 7.5)])
+def test_the_formats_error_is_half_a_step(bits, step):
+    """|value - x| <= half a step (8 bits: max|row| / 127; 4 bits: range / 15 of its run of 64), plus the
+    rounding of a 4-bit run's scale and mid to 16 bits: 8 steps x 2^-8 and 2^-8 of |mid|, plus float32's."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 3, 160, generator=g) * 3 + 1
+    got = eq.values(*eq.quantise(x, bits))
+    if bits == 8:
+        s = x.abs().amax(-1, keepdim=True).double() / 127
+        bound = s * (0.5 + 2 ** -16)
+    else:
+        bound = torch.empty_like(got)
+        for at in (0, 64, 128):
+            r = x[..., at:at + 64].double()
+            lo, hi = r.amin(-1, keepdim=True), r.amax(-1, keepdim=True)
+            s = (hi - lo) / 15
+            bound[..., at:at + 64] = s * (0.5 + 15 * 2 ** -8) + (lo + 8 * s).abs() * 2 ** -8
+    assert bool(((got - x.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+def test_engine_over_a_quantised_cache(tmp_path, monkeypatch, kv_format):
+    """The engine's logic with the restated kernels: unequal batches, early enders and slot reuse give what
+    a sequence alone gives, and 8 bits stay near the cache in the compute dtype."""
+    eq.install(monkeypatch)
+    folder = tiny_configs.make_folder(tmp_path, "A", seed=3)
+    loaded = siar.load_model(folder, device="cpu", dtype=torch.float32)
+    g = torch.Generator().manual_seed(1)
+    prompts = [torch.randint(0, 256, (n,), generator=g).tolist() for n in (3, 17, 66)]
+    run = lambda ps, fmt, **kw: siar.build_engine(loaded, max_batch=2, max_seq_len=96, kv_cache=fmt, **kw).generate(  # noqa: E731
+        ps, siar.SamplingParams(temperature=0.0), max_new_tokens=4, ignore_eos=True)
+    outs = run(prompts, kv_format)
+    assert outs == [run([p], kv_format)[0] for p in prompts]
+    engine, plain = (siar.build_engine(loaded, max_batch=1, max_seq_len=96, kv_cache=f) for f in (kv_format, None))
+    assert isinstance(engine.cache.entry(0), QuantizedKVEntry)
+    logits = [e.step([siar.StepEntry(e.open(), prompts[2], [65])]) for e in (engine, plain)]
+    # rounding to steps of s gives an rms error of s / sqrt(12); a row of 16 has max / rms about 2, a run's
+    # range / rms about 3.6: 2 / 127 / 3.5 = 0.5% and 3.6 / 15 / 3.5 = 7% of the keys and values, which reach
+    # the logits through scores and sums; four times that is allowed
+    off = float((logits[0] - logits[1]).norm() / logits[1].norm())
+    assert 0 < off < (0.02 if kv_format == "int8" else 0.3), off
+
+
+def test_unknown_kv_cache_is_refused(tmp_path):
+    folder = tiny_configs.make_folder(tmp_path, "A", seed=3)
+    loaded = siar.load_model(folder, device="cpu", dtype=torch.float32)
+    with pytest.raises(CacheError, match="int8, int4"):
+        siar.build_engine(loaded, max_seq_len=64, kv_cache="int2")

@@ -1,0 +1,290 @@
+"""A cache held in 8 or 4 bits on the GPU: what is stored, what is read back, and the attention over it,
+against plain restatements (``emulated_kv_quant.py``)."""
+
+import math
+
+import pytest
+import torch
+
+from simple_inference_autoresearch_b200.kernels import ops
+from simple_inference_autoresearch_b200.kernels.options import DEFAULT as OPTS
+from simple_inference_autoresearch_b200.parts.rope import RotaryParams
+from tests import emulated_kv_quant as eq
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def freqs(dim, theta=10000.0):
+    return (1.0 / theta ** (torch.arange(0, dim, 2, dtype=torch.float64) / dim)).float()
+
+
+def on_device(rotary):
+    if isinstance(rotary, RotaryParams):
+        return RotaryParams(rotary.inv_freq.to(DEV), rotary.rotary_dim, rotary.interleaved)
+    return None if rotary is None else rotary.to(DEV)
+
+
+def same(a, b):
+    """Equal, NaN where NaN."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.5), b.nan_to_num(0.5))
+
+
+SHAPES = [(4, 2, 16), (3, 1, 48), (8, 2, 64), (32, 8, 128), (6, 6, 80), (2, 1, 256)]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+def test_store_gives_the_plain_codes_and_touches_nothing_else(bits, dtype, heads, kv_heads, dim):
+    b = eq.Batch(bits, heads, kv_heads, dim, [0, 63, 130, 5, 100000 % 640], [1, 2, 70, 64, 3], seed=dim + bits, dtype=dtype)
+    kv = b.entry(DEV)
+    qkv = b.qkv.to(DEV)
+    q = torch.full_like(qkv, 7.0)
+    inv = freqs(dim)
+    ops.rope_kv_write(qkv, inv.to(DEV), kv, b.meta(DEV), *b.sizes(), q_out=q)
+    ops.check_status(DEV)
+    assert torch.equal(qkv.cpu(), b.qkv)
+    want, want_q = b.entry(), torch.full_like(b.qkv, 7.0)
+    eq.rope_kv_write(b.qkv, inv, want, b.meta(), *b.sizes(), q_out=want_q)
+    assert torch.equal(q.cpu(), want_q)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    # in place, and without storing
+    again, before = qkv.clone(), kv.k.clone()
+    ops.rope_kv_write(again, inv.to(DEV), kv, b.meta(DEV), *b.sizes(), write_kv=False)
+    n = heads * dim
+    assert torch.equal(again[:, :n].cpu(), want_q[:, :n]) and torch.equal(again[:, n:].cpu(), b.qkv[:, n:])
+    assert torch.equal(kv.k, before)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("layout", ["none", "partial", "interleaved", "partial_interleaved"])
+def test_store_takes_every_rotary_layout(bits, layout):
+    b = eq.Batch(bits, 4, 2, 64, [0, 200], [70, 3], seed=3)
+    dim = 32 if "partial" in layout else 64
+    rotary = None if layout == "none" else RotaryParams(freqs(dim), dim, "interleaved" in layout)
+    kv, qkv, q = b.entry(DEV), b.qkv.to(DEV), torch.zeros_like(b.qkv, device=DEV)
+    ops.rope_kv_write(qkv, on_device(rotary), kv, b.meta(DEV), *b.sizes(), q_out=q)
+    want, want_q = b.entry(), torch.zeros_like(b.qkv)
+    eq.rope_kv_write(b.qkv, rotary, want, b.meta(), *b.sizes(), q_out=want_q)
+    assert torch.equal(q.cpu(), want_q)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_far_positions_are_rotated_by_their_exact_angle(bits):
+    """Positions near 131,072: a float32 product of position and frequency is off by up to 2^-8 there."""
+    page = 64
+    b = eq.Batch(bits, 2, 1, 64, [3], [2], seed=9)
+    b.base_len[0] = 131061                                  # the table's row is as long as that needs
+    table = torch.full((3, 131072 // page), -1, dtype=torch.int32)
+    table[int(b.slot_ids[0]), 131061 // page] = 1
+    b.kv.block_table, b.held = table, [131061]
+    kv, qkv, q = b.entry(DEV), b.qkv.to(DEV), torch.zeros_like(b.qkv, device=DEV)
+    ops.rope_kv_write(qkv, freqs(64).to(DEV), kv, b.meta(DEV), *b.sizes(), q_out=q)
+    want, want_q = b.entry(), torch.zeros_like(b.qkv)
+    eq.rope_kv_write(b.qkv, freqs(64), want, b.meta(), *b.sizes(), q_out=want_q)
+    assert torch.equal(q.cpu(), want_q)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_rows_with_special_values(bits):
+    """Zeros, a constant, infinities, NaN, the largest and the smallest numbers: a bad row (or run of 64
+    dims) reads back as NaN, every other one as its values."""
+    b = eq.Batch(bits, 2, 2, 128, [0], [8], seed=4, dtype=torch.float32)
+    rows = b.qkv.view(8, 6, 128)
+    rows[0, 2:] = 0.0
+    rows[1, 2:] = 1.5
+    rows[2, 2, 100] = float("inf")
+    rows[2, 4, 3] = float("-inf")
+    rows[3, 3, 77] = float("nan")
+    rows[4, 2:] *= 1e38
+    rows[5, 2:] *= 1e-38
+    rows[6, 2:] *= 1e-44
+    rows[7, 2:, 0] = 1e30
+    kv = b.entry(DEV)
+    ops.rope_kv_write(b.qkv.to(DEV), None, kv, b.meta(DEV), *b.sizes(), q_out=torch.empty_like(b.qkv, device=DEV))
+    want = b.entry()
+    eq.rope_kv_write(b.qkv, None, want, b.meta(), *b.sizes(), q_out=torch.empty_like(b.qkv))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    got = ops.read_kv(kv, b.meta(DEV), torch.float32)
+    ops.check_status(DEV)
+    page = int(got.block_table[0, 0])
+    ref = eq.values(want.k, want.k_scale, torch.float32)[int(want.block_table[int(b.slot_ids[0]), 0])]
+    assert same(got.k[page, :, :8].cpu(), ref[:, :8])
+    assert not got.k[page, :, 8:].any()                      # rows behind the last token, stale NaN in the cache
+    assert bool(ref[0, 2].isnan().any()) and not bool(ref[1, 2].isnan().any()) and not bool(ref[:, 4:8].isnan().any())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+def test_read_back_gives_the_values_of_the_batch(bits, dtype, heads, kv_heads, dim):
+    held, new = [0, 63, 130, 300, 64], [1, 1, 70, 5, 64]
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=dim, dtype=dtype, stale="random")
+    for host in (True, False):
+        got = ops.read_kv(b.entry(DEV), b.meta(DEV, host_lengths=host), dtype)
+        ops.check_status(DEV)
+        assert got.block_table.shape == (5, b.kv.block_table.shape[1])
+        k_all, v_all = (eq.values(c, s, torch.float32).to(dtype) for c, s in ((b.kv.k, b.kv.k_scale), (b.kv.v, b.kv.v_scale)))
+        at = 0
+        for i, (c, n) in enumerate(zip(held, new)):
+            pages = -(-(c + n) // 64)
+            assert got.block_table[i].tolist() == list(range(at, at + pages)) + [-1] * (b.kv.block_table.shape[1] - pages)
+            rows = b.kv.block_table[int(b.slot_ids[i]), :pages].long()
+            for pool, whole in ((got.k, k_all), (got.v, v_all)):
+                want = whole[rows].transpose(1, 2).reshape(pages * 64, kv_heads, dim).clone()
+                want[c + n:] = 0
+                assert torch.equal(pool[at:at + pages].transpose(1, 2).reshape(pages * 64, kv_heads, dim).cpu(), want)
+            at += pages
+        if host:
+            assert got.k.shape[0] == at
+
+
+def check_attention(b, out, q, kv, scale, window=None):
+    want, bound, rms = eq.attention_bounds(b, q, kv, scale, window)
+    err = (out.cpu().double().view_as(want) - want).abs()
+    assert torch.isfinite(out).all()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    assert float(err.square().mean().sqrt()) <= 4 * rms + 1e-9, (float(err.square().mean().sqrt()), rms)
+
+
+ATTN = [(4, 2, 16), (3, 1, 48), (8, 2, 64), (16, 16, 64), (32, 8, 128), (6, 2, 128), (16, 1, 128), (8, 1, 64),
+        (40, 2, 64), (5, 1, 256)]
+STEPS = {
+    "first": ([0], [1]),
+    "decode": ([0, 1, 63, 64, 65, 200, 1000, 127], [1] * 8),
+    "long": ([3001, 17], [1, 1]),
+    "run": ([0, 63, 500, 130], [2, 4, 3, 1]),
+    "chunk": ([0, 100, 64], [70, 33, 130]),
+}
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("step", list(STEPS))
+@pytest.mark.parametrize("heads,kv_heads,dim", ATTN)
+def test_attention_over_the_quantised_cache(bits, dtype, heads, kv_heads, dim, step):
+    """Scale poison behind every sequence's last token (NaN in masked places must not come through)."""
+    held, new = STEPS[step]
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=heads + dim, dtype=dtype)
+    inv, scale = freqs(dim), 1.0 / math.sqrt(dim)
+    kv = b.entry(DEV)
+    out = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV), *b.sizes(), scale)
+    ops.check_status(DEV)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), inv, want, b.meta(), *b.sizes())
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    pos = [c + i for c, n in zip(held, new) for i in range(n)]
+    q = eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv)
+    check_attention(b, out, q, want, scale)
+    # the same without rotation or storing, on what is in the cache now
+    plain = ops.attention(b.qkv.to(DEV), kv, b.meta(DEV), *b.sizes(), scale)
+    check_attention(b, plain, b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), want, scale)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("step", ["decode", "run", "chunk"])
+def test_attention_with_a_window(bits, step):
+    held, new = STEPS[step]
+    b = eq.Batch(bits, 4, 2, 64, held, new, seed=2)
+    window = 70
+    for i, c in enumerate(held):                             # pages in front of the window were given back
+        b.kv.block_table[int(b.slot_ids[i]), :max(0, c - window + 1) // 64] = -1
+    kv = b.entry(DEV)
+    out = ops.rope_and_attention(b.qkv.to(DEV), None, kv, b.meta(DEV), *b.sizes(), 0.125, window=window)
+    ops.check_status(DEV)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), None, want, b.meta(), *b.sizes())
+    check_attention(b, out, b.qkv.view(b.tokens, -1, 64)[:, :4].float(), want, 0.125, window)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 5, 80])
+def test_an_absent_page_is_reported(bits, new):
+    for where in ("old", "new"):
+        b = eq.Batch(bits, 8, 2, 128, [300, 20], [new, 1], seed=1)
+        b.kv.block_table[int(b.slot_ids[0]), 1 if where == "old" else (300 + new - 1) // 64] = -1
+        kv = b.entry(DEV)
+        before = [t.clone() for t in (kv.k, kv.v)]
+        ops.rope_and_attention(b.qkv.to(DEV), None, kv, b.meta(DEV), *b.sizes(), 0.1)
+        with pytest.raises(RuntimeError, match="without a page"):
+            ops.check_status(DEV)
+        if where == "new" and new == 1:                      # the first sequence's token had no place
+            for pool, old in zip((kv.k, kv.v), before):
+                rows = b.kv.block_table[int(b.slot_ids[1])]
+                pool[rows[:1].long()] = old[rows[:1].long()]
+                assert torch.equal(pool, old)
+    ops.check_status(DEV)
+
+
+def test_argument_checks_see_the_quantised_entry():
+    b = eq.Batch(8, 8, 2, 64, [70], [1], seed=1)
+    b.kv.block_table[int(b.slot_ids[0]), 0] = 1000
+    with pytest.raises(ValueError, match="no page of the pool"):
+        ops.rope_and_attention(b.qkv.to(DEV), None, b.entry(DEV), b.meta(DEV), *b.sizes(), 0.1,
+                               options=OPTS.but(check_arguments=True))
+
+
+# ----------------------------------------------------------------------------- through the engine
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+@pytest.mark.parametrize("config,dtype", [("A", torch.float32), ("C", torch.bfloat16), ("D", torch.bfloat16), ("E", torch.bfloat16)])
+def test_engine_steps_against_the_restated_kernels(tmp_path, monkeypatch, kv_format, config, dtype):
+    """Prompts of unequal lengths, a second turn of several tokens, single tokens: every step's logits
+    against the same engine on the CPU with the restated kernels (same weights; bfloat16 rounds there as
+    here up to the order of sums, hence the tolerance the engine's own tests use)."""
+    import simple_inference_autoresearch_b200 as siar
+    from tests import tiny_configs
+    folder = tiny_configs.make_folder(tmp_path, config, seed=5)
+    raw, _ = tiny_configs.read_folder(folder)
+    g = torch.Generator().manual_seed(2)
+    tok = lambda n: torch.randint(0, raw["vocab_size"], (n,), generator=g).tolist()  # noqa: E731
+    turns = [[tok(n) for n in ns] for ns in ((5, 64, 33), (3, 1, 2), (1, 1, 1), (1, 1, 1))]
+
+    def logits(device, dt):
+        engine = siar.build_engine(siar.load_model(folder, device=device, dtype=dt), max_batch=3, max_seq_len=96, kv_cache=kv_format)
+        slots = [engine.open() for _ in range(3)]
+        return [engine.step([siar.StepEntry(s, t, range(len(t))) for s, t in zip(slots, turn)]).cpu().double() for turn in turns]
+
+    got = logits(DEV, dtype)
+    ops.check_status(DEV)
+    with monkeypatch.context() as m:
+        eq.install(m)
+        want = logits("cpu", torch.float32 if dtype == torch.float32 else dtype)
+    for a, w in zip(got, want):
+        off = float((a - w).abs().max() / w.abs().max())
+        # a key or value next to a rounding border may fall to the other side: one step of its row, in one of
+        # thousands of terms, so the 4-bit cache gets its 15 / 127 times coarser step's share on top
+        assert off <= (2e-4 if dtype == torch.float32 else 3e-2) * (1 if kv_format == "int8" else 127 / 15), off
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+@pytest.mark.parametrize("config,dtype", [("A", torch.float32), ("C", torch.bfloat16), ("D", torch.bfloat16), ("E", torch.bfloat16)])
+def test_captured_steps_draw_what_eager_steps_draw(tmp_path, kv_format, config, dtype):
+    import simple_inference_autoresearch_b200 as siar
+    from tests import tiny_configs
+    folder = tiny_configs.make_folder(tmp_path, config, seed=6)
+    raw, _ = tiny_configs.read_folder(folder)
+    loaded = siar.load_model(folder, device=DEV, dtype=dtype)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, raw["vocab_size"], (n,), generator=g).tolist() for n in (3, 40, 21, 9, 60)]
+    outs = {}
+    for graph in (False, True):
+        engine = siar.build_engine(loaded, max_batch=3, max_seq_len=96, use_cuda_graph=graph, kv_cache=kv_format)
+        outs[graph] = [engine.generate(prompts, siar.SamplingParams(temperature=0.0), max_new_tokens=n, ignore_eos=True)
+                       for n in (12, 5)]
+    assert outs[False] == outs[True]
+
+
+def test_command_line_takes_the_cache_format(capsys):
+    from simple_inference_autoresearch_b200 import inference
+    for fmt in ("int8", "int4"):
+        assert inference.main(["--model", "tiny-a", "--random-weights", "--prompt-len", "9", "--max-new-tokens", "4",
+                               "--temperature", "0", "--kv-cache", fmt]) == 0
+    assert "new_tokens" in capsys.readouterr().out
