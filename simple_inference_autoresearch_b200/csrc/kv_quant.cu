@@ -17,13 +17,9 @@
 // The rotation angle is position x frequency without rounding (a product of two 24-bit numbers fits a
 // double), its cosine and sine are rounded to 32 bits once, and the rotated value is formed by two
 // rounded products and a rounded sum, so a code depends on the token's row and position alone.
-#include "common.cuh"
-
-#include <math.h>
+#include "kv_quant.cuh"
 
 namespace siar {
-
-constexpr int kQuantGroup = 64;      // dims that share a scale in the 4-bit format
 
 // The batch description and the block table are read through plain pointers, behind pdl_wait(): the
 // kernel in front may have written them (advance_lengths, set_table_cells), and a load through a
@@ -35,12 +31,6 @@ __device__ __forceinline__ int sequence_of(const int* q_start, int B, int t) {
     if (q_start[mid] <= t) lo = mid; else hi = mid - 1;
   }
   return lo;
-}
-
-__device__ __forceinline__ float warp_min(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
 }
 
 // ------------------------------------------------------------------ rotate, quantise, store
@@ -66,10 +56,7 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
   const int half = rotary_dim >> 1;
   if (inv_freq != nullptr) {
     for (int i = threadIdx.x; i < half; i += blockDim.x) {
-      double sn, cn;
-      sincos((double)pos * (double)inv_freq[i], &sn, &cn);
-      cs[i] = (float)cn;
-      cs[half + i] = (float)sn;
+      rotation(pos, inv_freq[i], &cs[i], &cs[half + i]);
     }
   }
   int page = -1;
@@ -92,8 +79,8 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
       for (int i = lane; i < half; i += 32) {
         const int i0 = interleaved ? 2 * i : i, i1 = interleaved ? 2 * i + 1 : i + half;
         const float a = to_f32(src[i0]), c = to_f32(src[i1]);
-        row[i0] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(c, cs[half + i]));
-        row[i1] = __fadd_rn(__fmul_rn(c, cs[i]), __fmul_rn(a, cs[half + i]));
+        row[i0] = rotate_lo(a, c, cs[i], cs[half + i]);
+        row[i1] = rotate_hi(a, c, cs[i], cs[half + i]);
       }
     }
     for (int d = (rotates ? rotary_dim : 0) + lane; d < D; d += 32) row[d] = to_f32(src[d]);
@@ -107,49 +94,18 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
     const int kvh = is_k ? head - Hq : head - Hq - Hkv;
     const size_t at = ((size_t)page * Hkv + kvh) * page_tokens + pos % page_tokens;     // row of the pools
     uint8_t* codes = (is_k ? k_pool : v_pool) + at * (BITS == 8 ? D : D / 2);
-    const float nan = __int_as_float(0x7fc00000);
-    if (BITS == 8) {
-      float amax = 0.f;
-      bool bad = false;
-      for (int d = lane; d < D; d += 32) {
-        amax = fmaxf(amax, fabsf(row[d]));
-        bad |= !isfinite(row[d]);
-      }
-      amax = warp_max(amax);
-      bad = __any_sync(0xffffffffu, bad);
-      const float s = __fdiv_rn(amax, 127.f);
-      for (int d = 2 * lane; d < D; d += 64) {
-        int c[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          c[e] = bad || !(s > 0.f) ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(row[d + e], s))));
-        *reinterpret_cast<uint16_t*>(codes + d) = (uint16_t)((c[0] & 0xff) | ((c[1] & 0xff) << 8));
-      }
-      if (lane == 0) reinterpret_cast<float*>(is_k ? k_scale : v_scale)[at] = bad ? nan : s;
-    } else {
-      const int groups = (D + kQuantGroup - 1) / kQuantGroup;
-      __nv_bfloat162* sc = reinterpret_cast<__nv_bfloat162*>(is_k ? k_scale : v_scale) + at * groups;
-      for (int g = 0; g < groups; ++g) {
-        const int d = g * kQuantGroup + 2 * lane;
-        const bool in = d < D;
-        const float x0 = in ? row[d] : 0.f, x1 = in ? row[d + 1] : 0.f;
-        const bool bad = __any_sync(0xffffffffu, !isfinite(x0) || !isfinite(x1));
-        const float lo = warp_min(in ? fminf(x0, x1) : INFINITY), hi = warp_max(in ? fmaxf(x0, x1) : -INFINITY);
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)));
-        const float s = __bfloat162float(sb);
-        const __nv_bfloat16 mb = __float2bfloat16_rn(__fadd_rn(lo, 8.f * s));
-        const float m = __bfloat162float(mb);
-        if (in) {
-          int c[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            c[e] = bad || !(s > 0.f) ? 8
-                                     : max(0, min(15, __float2int_rn(__fdiv_rn(__fsub_rn(e ? x1 : x0, m), s)) + 8));
-          codes[d / 2] = (uint8_t)(c[0] | (c[1] << 4));
-        }
-        if (lane == 0) sc[g] = bad ? __floats2bfloat162_rn(nan, nan) : __halves2bfloat162(sb, mb);
-      }
-    }
+    float* s8 = reinterpret_cast<float*>(is_k ? k_scale : v_scale) + at;
+    __nv_bfloat162* s4 = reinterpret_cast<__nv_bfloat162*>(is_k ? k_scale : v_scale) + at * ((D + kQuantGroup - 1) / kQuantGroup);
+    quantize_row<BITS>(
+        row, D, lane,
+        [&](int d, uint32_t c) {
+          if (BITS == 8) *reinterpret_cast<uint16_t*>(codes + d) = (uint16_t)c;
+          else codes[d / 2] = (uint8_t)c;
+        },
+        [&](int g, float s, __nv_bfloat162 sm) {
+          if (BITS == 8) *s8 = s;
+          else s4[g] = sm;
+        });
   }
 }
 

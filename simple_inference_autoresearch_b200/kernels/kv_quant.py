@@ -126,6 +126,64 @@ def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options:
     return _read(kv, meta, dtype, window)[0]
 
 
+#: query rows (new tokens x heads of a group) a sequence may bring to the kernel that works on the codes; a
+#: longer run reads the cache back once for the prompt kernel instead of walking the codes for every 16 rows
+MOST_ROWS = 64
+
+
+def works_on_codes(kv, meta, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int,
+                   window: Optional[int] = None, options: KernelOptions = DEFAULT) -> bool:
+    """True when attention over this entry runs on the codes themselves (bfloat16, head_dim 64 or 128, pages of
+    a multiple of 64, no window, single tokens or short runs); else the cache is read back first."""
+    if dtype != torch.bfloat16 or window is not None or head_dim not in (64, 128) or not options.use_mma_attention:
+        return False
+    if not meta.is_decode and meta.max_q_len * (n_heads // n_kv_heads) > MOST_ROWS:
+        return False
+    return bool(ops._fn("attention_quant", "siar_attn_quant_supported")(n_heads, n_kv_heads, head_dim, kv.page_tokens,
+                                                                        kv.k.shape[0]))
+
+
+_eager_counters, _captured_counters = {}, {}
+
+
+def _zeroed_counters(n: int, device, stream: int) -> torch.Tensor:
+    """``n`` int32 zeros that a launch uses and leaves zero.  Launches of one stream follow one another and
+    share them; a captured graph may be replayed beside anything, so every capture has its own, zeroed by
+    the graph itself, shared by the launches that it holds on one stream."""
+    fn = ops._fn("attention_quant", "siar_capture_id")
+    fn.restype = ops.c_ulonglong
+    capture = fn(stream)
+    key = (device.index, stream)
+    if capture:
+        held = _captured_counters.get(key)
+        if held is None or held[0] != capture or held[1].numel() < n:
+            held = _captured_counters[key] = (capture, torch.zeros(n, dtype=torch.int32, device=device))
+        return held[1]
+    t = _eager_counters.get(key)
+    if t is None or t.numel() < n:
+        t = _eager_counters[key] = torch.zeros(n, dtype=torch.int32, device=device)
+    return t
+
+
+def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
+    device = qkv.device
+    out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
+    with ops._on_device(qkv):
+        blocks = ops._fn("attention_quant", "siar_attn_quant_blocks")(
+            meta.n_seqs, n_heads, n_kv_heads, head_dim, meta.max_q_len, meta.max_kv_len, ops._sm_count(device))
+        fn = ops._fn("attention_quant", "siar_attn_quant_scratch_floats")
+        fn.restype = ops.c_longlong
+        scratch = torch.empty(fn(n_heads, n_kv_heads, head_dim, meta.max_q_len, blocks), dtype=torch.float32, device=device)
+        stream = ops._stream()
+        counters = _zeroed_counters(blocks, device, stream)
+        ops._launch("attention_quant", "siar_attn_quant", kv.bits, ops._ptr(qkv), ops._ptr(kv.k), ops._ptr(kv.v),
+                    ops._ptr(kv.k_scale), ops._ptr(kv.v_scale), ops._ptr(kv.block_table), *_batch(meta), ops._ptr(inv_freq),
+                    ops._ptr(out), ops._ptr(scratch), ops._ptr(counters), blocks, meta.n_seqs, n_heads, n_kv_heads, head_dim,
+                    kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], meta.max_q_len, int(fused), int(write_kv),
+                    float(scale), ops._ptr(ops.status_word(device)), stream)
+    return out
+
+
 def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
               window: Optional[int] = None, options: KernelOptions = DEFAULT) -> torch.Tensor:
     check_window(window)
@@ -133,6 +191,8 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     check_entry(kv, n_kv_heads, head_dim, qkv.device)
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], False, window)
+    if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
+        return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, False)
     pages, slots = _read(kv, meta, qkv.dtype, window)
     of_batch = copy.copy(meta)
     of_batch.slot_ids = slots
@@ -147,6 +207,15 @@ def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_h
                        write_kv: bool = True, window: Optional[int] = None,
                        options: KernelOptions = DEFAULT) -> torch.Tensor:
     check_window(window)
+    inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
+    plain_layout = inv_freq is None or (rotary_dim == head_dim and not interleaved)
+    if meta.is_decode and plain_layout and options.fuse_decode_rope and works_on_codes(
+            kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
+        check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
+        check_entry(kv, n_kv_heads, head_dim, qkv.device)
+        ops._need_cuda(qkv, inv_freq)
+        ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
+        return _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, True, write_kv)
     q = torch.empty_like(qkv)               # the rotated queries; qkv stays as it is
     rope_kv_write(qkv, rotary, kv, meta, n_heads, n_kv_heads, head_dim, write_kv=write_kv, options=options, q_out=q)
     return attention(q, kv, meta, n_heads, n_kv_heads, head_dim, scale, window=window, options=options)

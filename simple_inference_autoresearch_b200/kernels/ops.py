@@ -20,6 +20,7 @@ from . import build
 from .options import DEFAULT, KernelOptions
 
 c_int, c_float, c_void_p, c_longlong = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
+c_ulonglong = ctypes.c_ulonglong
 
 # ------------------------------------------------------------------ plumbing
 #: kernels launched through this module since import (graph replays add what the graph holds)
@@ -82,6 +83,17 @@ _signatures = {
         "siar_read_kv": [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                          c_int, c_int, c_void_p, c_void_p],
+    },
+    "attention_quant": {
+        # bits, qkv, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, scratch, counters,
+        # blocks, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, fused, write_kv, scale, status, stream
+        "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                            c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+        "siar_attn_quant_supported": [c_int, c_int, c_int, c_int, c_longlong],
+        "siar_attn_quant_blocks": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+        "siar_attn_quant_scratch_floats": [c_int, c_int, c_int, c_int, c_int],
+        "siar_capture_id": [c_void_p],
     },
     "sampling": {
         "siar_sample": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -545,7 +557,8 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     cache entry ``kv``; returns [N, n_heads * head_dim] in qkv's dtype.  bfloat16
     with head_dim 64 or 128 runs on the tensor cores, everything else on the CUDA cores.
     ``window`` = w: a query at position p sees keys p - w + 1 .. p only (CUDA-core kernels).
-    A ``QuantizedKVEntry`` is read back as pages of qkv's dtype first (``read_kv``)."""
+    Over a ``QuantizedKVEntry`` single tokens and short runs in bfloat16 (head_dim 64 or 128) work on the
+    codes, everything else on the cache read back as pages of qkv's dtype (``read_kv``)."""
     if kv_quant.is_quantized(kv):
         return kv_quant.attention(qkv, kv, meta, n_heads, n_kv_heads, head_dim, scale, window, options)
     if window is not None and window <= 0:
