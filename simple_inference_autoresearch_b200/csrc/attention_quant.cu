@@ -28,6 +28,8 @@
 #include "kv_quant.cuh"
 #include "tcgen05.cuh"
 
+#include <type_traits>
+
 namespace siar {
 
 struct QuantAttnParams {
@@ -46,6 +48,7 @@ struct QuantAttnParams {
   int* counters;                 // [units], zero between launches
   int* status;
   int B, Hq, Hkv, page_tokens, max_pages, n_pages;
+  int page_shift;                // log2(page_tokens), or -1
   int fused;                     // rotate and (write_kv) store the new token here; one token a sequence
   int write_kv;
   float sl2;                     // scale * log2(e)
@@ -204,6 +207,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   int l_rt = c_rt, l_kvh = c_kvh, l_t = c_t, l_left = n_steps;
   int issued = 0, consumed = 0;
   bool absent_page = false;
+  auto page_index = [&](int pos) { return P.page_shift >= 0 ? pos >> P.page_shift : pos / P.page_tokens; };
   auto next_seq = [&](const QuantSeq& s) {        // the next sequence that has steps (there is one)
     int b = s.b + 1;
     QuantSeq n = load_seq(b);
@@ -212,7 +216,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   };
   auto page_of = [&]() {                          // page of the load cursor's tile; asked for a step before its use
     const int w0 = l_t * C::kBlockKeys + warp * WK;
-    return l_left > 0 && w0 < lu.len ? P.block_table[(size_t)lu.slot * P.max_pages + w0 / P.page_tokens] : 0;
+    return l_left > 0 && w0 < lu.len ? P.block_table[(size_t)lu.slot * P.max_pages + page_index(w0)] : 0;
   };
   int page_ahead = page_of();
   auto issue_next = [&]() {
@@ -224,7 +228,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         if (page < 0 || page >= P.n_pages) { absent_page = true; page = 0; }
         if (lane == 0) {
           const int s = issued % C::kStages;
-          const int row = (page * P.Hkv + l_kvh) * P.page_tokens + w0 % P.page_tokens;
+          const int row = (page * P.Hkv + l_kvh) * P.page_tokens + w0 - page_index(w0) * P.page_tokens;
           unsigned char* kt = smem + C::kTiles + (s * 4 + warp) * 2 * C::kTileBytes;
           unsigned char* sc = smem + C::kScales + (s * 4 + warp) * 2 * C::kScaleBytes;
           uint64_t* bar = &bars[warp][s];
@@ -493,117 +497,114 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         }
       }
 
-      // ---- value scales of this lane's keys (g, g + 8 of each 16)
-      const bool masked = w0 + WK - 1 > min(first_limit, cu.len - 1);       // some row does not see some key of the tile
-      float sv[KT][2][NG], mv[KT][2][NG], top[KT][2];
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = 16 * k + 8 * h + g;
-          const bool in = w0 + key < cu.len;
-          if (BITS == 8) {
-            sv[k][h][0] = in ? reinterpret_cast<const float*>(sc + C::kScaleBytes)[key] : 0.f;
-            top[k][h] = sv[k][h][0];
-          } else {
-            float t = 0.f;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-              const uint32_t sm = in ? reinterpret_cast<const uint32_t*>(sc + C::kScaleBytes)[key * NG + gr] : 0u;
-              sv[k][h][gr] = __uint_as_float(sm << 16);
-              mv[k][h][gr] = __uint_as_float(sm & 0xffff0000u);
-              t = fmaxf(t, sv[k][h][gr]);
-            }
-            top[k][h] = t;
-          }
-          // a row of zeros (or of values below 127 x 2^-100) must not lift the reference without end
-          top[k][h] = fmaxf(top[k][h], 7.9e-31f);
-        }
-      // which of the lane's (key, query row) pairs count
-      uint32_t ok = 0xffffffffu;
-      if (masked) {
-        ok = 0;
-#pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = w0 + 16 * k + 8 * (e >> 1) + g, row = row0 + 8 * nt + 2 * q4 + (e & 1);
-              const int limit = min(cu.base + min(row / G, cu.q_len - 1), cu.len - 1);
-              ok |= (uint32_t)(key <= limit) << (((k * NT + nt) * 4 + e) & 31);
-            }
-      }
-      static_assert(KT * NT * 4 <= 32, "one bit per pair");
-      float p[KT][NT][4];
-      auto exponentials = [&]() {                           // returns the largest p sv
-        float most = 0.f;
-#pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = fast_exp2(fmaf(x[k][nt][e], f_r[nt][e & 1], -m_r[nt][e & 1]));
-              if (masked && !((ok >> ((k * NT + nt) * 4 + e)) & 1)) v = 0.f;
-              p[k][nt][e] = v;
-              most = fmaxf(most, v * top[k][e >> 1]);
-            }
-        return most;
-      };
-      if (__any_sync(0xffffffffu, exponentials() > 256.f)) {
-        // move the reference to the largest s + log2 sv seen so far (the first tile, and rarely after)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = m_r[nt][e];
-#pragma unroll
-            for (int k = 0; k < KT; ++k)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if (!masked || ((ok >> ((k * NT + nt) * 4 + 2 * h + e)) & 1))
-                  mx = fmaxf(mx, fmaf(x[k][nt][2 * h + e], f_r[nt][e], __log2f(top[k][h])));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float alpha = mx == m_r[nt][e] ? 1.f : fast_exp2(m_r[nt][e] - mx);
-            m_r[nt][e] = mx;
-            l_r[nt][e] *= alpha;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) z[nt][e][gr] *= alpha;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) { o[mt][nt][e] *= alpha; o[mt][nt][e + 2] *= alpha; }
-          }
-        exponentials();
-      }
-      // ---- sums, and P as the second product's operand (keys on k, query rows on n)
+      // ---- probabilities: value scales of this lane's keys (g, g + 8 of each 16), exponentials, sums, and P as
+      // the second product's operand (keys on k, query rows on n)
       uint32_t pb[KT][NT][NG][2];
+      auto softmax = [&](auto masked_c) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        const unsigned char* scv = sc + C::kScaleBytes;
+        float sv[KT][2][NG], mv[KT][2][NG], top[KT][2];
+        bool seen[KT][NT][4];                               // which of the lane's (key, query row) pairs count
+        if (MASKED) {
 #pragma unroll
-      for (int k = 0; k < KT; ++k)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          l_r[nt][0] += p[k][nt][0] + p[k][nt][2];
-          l_r[nt][1] += p[k][nt][1] + p[k][nt][3];
+            for (int e = 0; e < 2; ++e) {
+              const int limit = min(cu.base + min((row0 + 8 * nt + 2 * q4 + e) / G, cu.q_len - 1), cu.len - 1);
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            float v[4];
+              for (int k = 0; k < KT; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = p[k][nt][e] * sv[k][e >> 1][gr];
-              if (masked && !((ok >> ((k * NT + nt) * 4 + e)) & 1)) v[e] = 0.f;      // not 0 x NaN of a key nobody sees
+                for (int h = 0; h < 2; ++h) seen[k][nt][2 * h + e] = w0 + 16 * k + 8 * h + g <= limit;
             }
-            if (BITS == 4) {
+        }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float t = p[k][nt][e] * mv[k][e >> 1][gr];
-                z[nt][e & 1][gr] += masked && !((ok >> ((k * NT + nt) * 4 + e)) & 1) ? 0.f : t;
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = 16 * k + 8 * h + g;
+            const bool in = !MASKED || w0 + key < cu.len;
+            if (BITS == 8) {
+              sv[k][h][0] = in ? reinterpret_cast<const float*>(scv)[key] : 0.f;
+              top[k][h] = sv[k][h][0];
+            } else {
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) {
+                const uint32_t sm = in ? reinterpret_cast<const uint32_t*>(scv)[key * NG + gr] : 0u;
+                sv[k][h][gr] = __uint_as_float(sm << 16);
+                mv[k][h][gr] = __uint_as_float(sm & 0xffff0000u);
+                top[k][h] = gr ? fmaxf(top[k][h], sv[k][h][gr]) : sv[k][h][gr];
               }
             }
-            pb[k][nt][gr][0] = transpose_8x8(pack_f16(v[0], v[1]));
-            pb[k][nt][gr][1] = transpose_8x8(pack_f16(v[2], v[3]));
+            // a row of zeros (or of values below 127 x 2^-100) must not lift the reference without end
+            top[k][h] = fmaxf(top[k][h], 7.9e-31f);
           }
+        float p[KT][NT][4];
+        auto exponentials = [&]() {                         // returns the largest p sv
+          float most = 0.f;
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v = fast_exp2(fmaf(x[k][nt][e], f_r[nt][e & 1], -m_r[nt][e & 1]));
+                if (MASKED && !seen[k][nt][e]) v = 0.f;
+                p[k][nt][e] = v;
+                most = fmaxf(most, v * top[k][e >> 1]);
+              }
+          return most;
+        };
+        if (__any_sync(0xffffffffu, exponentials() > 256.f)) {
+          // move the reference to the largest s + log2 sv seen so far (the first tile, and rarely after)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = m_r[nt][e];
+#pragma unroll
+              for (int k = 0; k < KT; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (!MASKED || seen[k][nt][2 * h + e])
+                    mx = fmaxf(mx, fmaf(x[k][nt][2 * h + e], f_r[nt][e], __log2f(top[k][h])));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float alpha = mx == m_r[nt][e] ? 1.f : fast_exp2(m_r[nt][e] - mx);
+              m_r[nt][e] = mx;
+              l_r[nt][e] *= alpha;
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) z[nt][e][gr] *= alpha;
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) { o[mt][nt][e] *= alpha; o[mt][nt][e + 2] *= alpha; }
+            }
+          exponentials();
         }
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            l_r[nt][0] += p[k][nt][0] + p[k][nt][2];
+            l_r[nt][1] += p[k][nt][1] + p[k][nt][3];
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                // a key that the row does not see adds nothing, not 0 x NaN
+                v[e] = !MASKED || seen[k][nt][e] ? p[k][nt][e] * sv[k][e >> 1][gr] : 0.f;
+                if (BITS == 4)
+                  z[nt][e & 1][gr] = !MASKED || seen[k][nt][e] ? fmaf(p[k][nt][e], mv[k][e >> 1][gr], z[nt][e & 1][gr])
+                                                               : z[nt][e & 1][gr];
+              }
+              pb[k][nt][gr][0] = transpose_8x8(pack_f16(v[0], v[1]));
+              pb[k][nt][gr][1] = transpose_8x8(pack_f16(v[2], v[3]));
+            }
+          }
+      };
+      // some row does not see some key of the tile
+      if (w0 + WK - 1 > min(first_limit, cu.len - 1)) softmax(std::true_type{});
+      else softmax(std::false_type{});
       // ---- O^T += V^T P^T: value dims on the rows
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
@@ -922,7 +923,7 @@ extern "C" int siar_attn_quant(int bits, const void* qkv, void* k_pool, void* v_
     return (int)cudaErrorInvalidValue;
   QuantAttnParams p = {(const __nv_bfloat16*)qkv, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
                        q_start, base_len, inv_freq, (__nv_bfloat16*)out, scratch, counters, status, B, Hq, Hkv, page_tokens,
-                       max_pages, n_pages, fused, write_kv, scale * 1.4426950408889634f};
+                       max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused, write_kv, scale * 1.4426950408889634f};
   cudaStream_t s = (cudaStream_t)stream;
   const int nt = row_tiles_of(max_q_len * (Hq / Hkv));
 #define SIAR_GO(BITS, DIM) \
