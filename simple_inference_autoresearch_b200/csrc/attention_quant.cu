@@ -2,23 +2,26 @@
 // kv_quant.cu): single tokens of a decode step, with their rotary encoding and cache write inside, and
 // short runs of tokens already stored.  head_dim 64 or 128, any group size, pages of a multiple of 64.
 //
-// Mathematics.  The codes go through the tensor cores as the small whole numbers they are; scales
-// enter outside the products:
+// Mathematics.  The codes go through the integer tensor cores as they are; scales enter outside:
 //   8 bits  s_j = sk_j (q . ck_j),                            out = sum_j (p_j sv_j) cv_j / sum_j p_j
 //   4 bits  s_j = sum_g sk_jg (q_g . (ck_jg - 8)) + mk_jg sum(q_g),
-//           out_g = (sum_j (p_j sv_jg) (cv_jg - 8) + sum_j p_j mv_jg) / sum_j p_j
-// with one pass over the keys and a running reference of the exponent.  A code becomes a float16 by
-// placing its bits in the mantissa of 1024 (0x6400 | u = 1024 + u); for keys the constant this adds is
-// taken off in the accumulator's start value, for values (whose sums run over thousands of keys) from
-// the operand, exactly.  q is scaled by a power of two per row and rounded once to float16 (11 bits where
-// bfloat16 keeps 8); p_j sv_j is at most 2^8 by choice of the reference (the running maximum of
-// s_j + log2 sv_j, moved only when a product would pass 2^8) and rounded once to float16.  Scores,
-// statistics and sums are 32 bits.
+//           out_g = (sum_j (p_j sv_jg) cv_jg + sum_j p_j (mv_jg - 8 sv_jg)) / sum_j p_j
+// A query row becomes whole numbers of 16 bits (largest element 32512; a step is 2^-16 of it, where
+// bfloat16 keeps 8 bits of every element), split into two bytes that take two columns of the product;
+// the integer scores are exact.  For the value product the p_j sv_j of one step of keys become
+// whole numbers of 16 bits too, against the largest of the step, again two bytes in two columns: within a
+// step 2^-17 of the largest is lost, and a step's integer sum goes into the 32-bit accumulators with the
+// step's own factor, so nothing is lost between steps.  Statistics and sums are 32 bits.
 //
 // Shape.  The products are taken transposed, keys (then value dims) on the MMA's 16 rows and the query
-// heads that share a kv head on its 8 columns: half the instructions of heads on the rows, and P moves
-// from one product to the other by movmatrix.  What bounds it is memory: a key and value of a head are
-// 264 bytes (8 bits, head_dim 128) or 144 (4 bits).
+// rows on its columns, four of them (times two bytes) a tile of eight: with four query heads to a
+// kv head no column is empty, an accumulator pair is one score, and P moves from one product to the
+// other by a byte permutation and a movmatrix.  Codes need no conversion: a key's row is the operand
+// (4 bits: an AND or a shift and an AND for four codes), values are brought to four keys a
+// register by two byte permutations for eight codes.  (Tried first: codes converted to float16 for
+// m16n8k16 products, 490 instructions for 32 keys of 8 bits, 850 for 32 of 4 bits, bound by issue and
+// latency: 64 sequences of up to 4,500 keys 101 us, of 9,000 in 4 bits 194 us.)  What should bound it is
+// memory: a key and value of a head are 264 bytes (8 bits, head_dim 128) or 144 (4 bits).
 //
 // Work is cut evenly: all (sequence, kv head) units' key tiles stand in one row that is shared out over two
 // blocks an SM, so unequal lengths leave no tail; a warp's loads (TMA, its own ring of stages, the scales
@@ -57,49 +60,51 @@ struct QuantAttnParams {
 template <int BITS, int D, int NT>
 struct QuantAttn {
   static constexpr int kRowBytes = D * BITS / 8;
-  static constexpr int kWarpKeys = D == 128 ? 32 : 64;                // keys per warp and step
+  static constexpr int kWarpKeys = D == 128 ? 32 : 64;               // keys per warp and step
   static constexpr int kBlockKeys = 4 * kWarpKeys;
   static constexpr int kTileBytes = kWarpKeys * kRowBytes;
   static constexpr int kGroups = BITS == 8 ? 1 : D / kQuantGroup;
   static constexpr int kScaleBytes = kWarpKeys * 4 * kGroups;        // float32, or (scale, mid) bfloat16 per run
-  // what two blocks an SM leave room for
-  static constexpr int kStages = kTileBytes < 4096 ? (NT == 1 ? 5 : 4) : (NT == 1 ? 3 : 2);
-  static constexpr int kRows = 8 * NT;                               // query rows of a unit
+  // blocks an SM and pipeline depth: what shared memory (and, for many rows, registers) leave room for
+  static constexpr int kBlocksPerSM = NT == 4 ? 2 : 3;
+  static constexpr int kStages = kTileBytes < 4096 ? (NT == 4 ? 4 : 3) : 2;
+  static constexpr int kRows = 4 * NT;                               // query rows of a unit
   static constexpr int kMT = D / 16;                                 // row tiles of the value product
-  static constexpr int kQStride = D + 8;                             // float16 elements per query row in shared memory
-  static constexpr int kRegs = kMT * NT * 4;                         // accumulators of a lane
+  static constexpr int kQStride = D + 16;                            // bytes per column of query bytes in shared memory
+  static constexpr int kRegs = kMT * NT * 2;                         // accumulators of a lane
   // shared memory
   static constexpr int kTiles = 0;                                   // [stages][warp][K | V]
   static constexpr int kScales = kTiles + kStages * 4 * 2 * kTileBytes;
   static constexpr int kJoin = kScales + kStages * 4 * 2 * kScaleBytes;   // [2][kRegs][32] floats
   static constexpr int kQ = kJoin + 2 * kRegs * 32 * 4;
-  static constexpr int kSmem = kQ + kRows * kQStride * 2;
-  static constexpr int kSegFloats = (kRegs + 4 * NT) * 32;           // accumulators, maxima, sums
+  static constexpr int kSmem = kQ + 8 * NT * kQStride;
+  static constexpr int kSegFloats = (kRegs + 2 * NT) * 32;           // accumulators, references, sums
 };
+constexpr float kFixedP = 65500.f;                // p sv of a step's largest term, as a whole number
 
-__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                              uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D (int32) = C + A B for bytes; ASIGN / BSIGN: signed operands.
+template <bool ASIGN, bool BSIGN>
+__device__ __forceinline__ void mma_bytes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+#define SIAR_MMA(AT, BT)                                                                                              \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." AT "." BT ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                        \
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if (ASIGN && BSIGN) SIAR_MMA("s8", "s8");
+  else if (ASIGN) SIAR_MMA("s8", "u8");
+  else if (BSIGN) SIAR_MMA("u8", "s8");
+  else SIAR_MMA("u8", "u8");
+#undef SIAR_MMA
+}
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
-  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
-  return *reinterpret_cast<uint32_t*>(&r);
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
@@ -118,7 +123,7 @@ struct QuantSeq {
 };
 
 template <int BITS, int D, int NT>
-__global__ void __launch_bounds__(128, 2)
+__global__ void __launch_bounds__(128, (QuantAttn<BITS, D, NT>::kBlocksPerSM))
 attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map) {
   using C = QuantAttn<BITS, D, NT>;
@@ -129,8 +134,9 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   __shared__ __align__(8) uint64_t bars[4][C::kStages];
   __shared__ float cs_s[D];                       // cosines, sines of the new token's position
   __shared__ float row_s[D];                      // the new token's key, then value
-  __shared__ float f_s[C::kRows], qsum_s[C::kRows][NG];
-  __shared__ float ml_s[2][NT * 4][32];
+  __shared__ float f_s[C::kRows];
+  __shared__ int qsum_s[C::kRows][NG];
+  __shared__ float ml_s[2][NT * 2][32];
   __shared__ int last_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q4 = lane & 3;
@@ -257,15 +263,16 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   };
   for (int s = 0; s < C::kStages; ++s) issue_next();
 
-  float o[MT][NT][4];
-  float m_r[NT][2], l_r[NT][2], f_r[NT][2], z[NT][2][NG], qs[NT][2][NG];
-  uint32_t qb[D / 16][NT][2];
+  float o[MT][NT][2];                             // dims (row g, row g + 8 of tile mt) of query row 4 nt + t
+  float m_r[NT], l_r[NT], f_r[NT], z[NT][NG];
+  int qs[NT][NG];
+  uint32_t qb[D / 32][NT][2];
   bool expired = false;
   const size_t qkv_row = (size_t)(P.Hq + 2 * P.Hkv) * D;
   int cs_b = -1;
 
   for (int done = 0; done < n_steps;) {
-    // ---- the unit's query rows: rotated if asked, scaled by a power of two, float16
+    // ---- the unit's query rows: rotated if asked, whole numbers of 16 bits in two bytes
     const int rows = cu.q_len * G, row0 = c_rt * C::kRows;
     if (P.fused && cs_b != cu.b && P.inv_freq != nullptr) {
       __syncthreads();
@@ -273,92 +280,78 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       cs_b = cu.b;
     }
     __syncthreads();
-    __half* q_s = reinterpret_cast<__half*>(smem + C::kQ);
+    signed char* q_s = reinterpret_cast<signed char*>(smem + C::kQ);     // column 2r: high bytes of row r, 2r + 1: low bytes
     for (int r = warp; r < C::kRows; r += 4) {
       const int row = row0 + r;
-      float a[D / 64], c[D / 64], amax = 0.f;
+      float a[D / 32], amax = 0.f;                 // dims lane + 32 i
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        a[i] = c[i] = 0.f;
-        if (row < rows) {
-          const __nv_bfloat16* src = P.qkv + (size_t)(cu.t0 + row / G) * qkv_row + (size_t)(c_kvh * G + row % G) * D + i * 32 + lane;
-          a[i] = __bfloat162float(src[0]);
-          c[i] = __bfloat162float(src[D / 2]);
-          if (P.fused && P.inv_freq != nullptr) {
+      for (int i = 0; i < D / 32; ++i) a[i] = 0.f;
+      if (row < rows) {
+        const __nv_bfloat16* src = P.qkv + (size_t)(cu.t0 + row / G) * qkv_row + (size_t)(c_kvh * G + row % G) * D + lane;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) a[i] = __bfloat162float(src[32 * i]);
+        if (P.fused && P.inv_freq != nullptr) {
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
             const float cv = cs_s[i * 32 + lane], sv = cs_s[D / 2 + i * 32 + lane];
-            const float lo = rotate_lo(a[i], c[i], cv, sv);
-            c[i] = rotate_hi(a[i], c[i], cv, sv);
+            const float lo = rotate_lo(a[i], a[i + D / 64], cv, sv);
+            a[i + D / 64] = rotate_hi(a[i], a[i + D / 64], cv, sv);
             a[i] = lo;
           }
         }
-        amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(c[i])));
       }
-      amax = warp_max(amax);
-      // the row's largest element goes to [2^10, 2^11): what float16 then loses at the small end is
-      // 2^-35 of it
-      int ex = 0;
-      if (amax > 0.f && isfinite(amax)) frexpf(amax, &ex);
-      const float up = ldexpf(1.f, max(-100, min(100, 11 - ex)));
-      float sum[2] = {0.f, 0.f};                   // of the rounded elements, by halves of the head
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const __half ha = __float2half_rn(a[i] * up), hc = __float2half_rn(c[i] * up);
-        q_s[r * C::kQStride + i * 32 + lane] = ha;
-        q_s[r * C::kQStride + D / 2 + i * 32 + lane] = hc;
-        sum[0] += __half2float(ha);
-        sum[1] += __half2float(hc);
+      for (int i = 0; i < D / 32; ++i) amax = max_nan(amax, fabsf(a[i]));
+#pragma unroll
+      for (int sh = 16; sh > 0; sh >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
+      const bool fine = isfinite(amax) && amax > 1e-30f;       // else zeros; NaN through the factor where not finite
+      const float up = fine ? 32512.f / amax : 0.f;
+      int sum[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) sum[gr] = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const int v = fine ? __float2int_rn(a[i] * up) : 0;
+        const int hi = (v + 128) >> 8;             // v = 256 hi + lo, lo in -128 .. 127
+        // 4 bits: a word holds eight dims, the even ones in its low halves, the odd ones in its high halves
+        const int d = 32 * i + lane, at = BITS == 8 ? d : (d & ~7) + ((d & 1) << 2) + ((d & 7) >> 1);
+        q_s[(2 * r) * C::kQStride + at] = (signed char)hi;
+        q_s[(2 * r + 1) * C::kQStride + at] = (signed char)(v - (hi << 8));
+        sum[BITS == 8 ? 0 : 32 * i / kQuantGroup] += v;
       }
-      sum[0] = warp_sum(sum[0]);
-      sum[1] = warp_sum(sum[1]);
-      if (lane == 0) {
-        f_s[r] = P.sl2 / up;
-        if (NG == 2) { qsum_s[r][0] = sum[0]; qsum_s[r][NG - 1] = sum[1]; }
-        else qsum_s[r][0] = sum[0] + sum[1];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        sum[gr] = __reduce_add_sync(0xffffffffu, sum[gr]);
+        if (lane == 0) qsum_s[r][gr] = sum[gr];
       }
+      if (lane == 0) f_s[r] = fine ? P.sl2 * (amax / 32512.f) : amax - amax;
     }
     __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const __half* qr = q_s + (8 * nt + g) * C::kQStride;
-      if (BITS == 8) {
-        // k slots (2t, 2t+1 | 2t+8, 2t+9) of chunk c hold dims 16c + 4t + (0, 1 | 2, 3)
+      const signed char* qc = q_s + (8 * nt + g) * C::kQStride;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          const uint2 w = *reinterpret_cast<const uint2*>(qr + 16 * c + 4 * q4);
+      for (int c = 0; c < D / 32; ++c) {
+        if (BITS == 8) {                           // dims 32c + 4t .. + 3 and 16 more
+          qb[c][nt][0] = *reinterpret_cast<const uint32_t*>(qc + 32 * c + 4 * q4);
+          qb[c][nt][1] = *reinterpret_cast<const uint32_t*>(qc + 32 * c + 16 + 4 * q4);
+        } else {                                   // dims 32c + 8t + (0, 2, 4, 6 | 1, 3, 5, 7)
+          const uint2 w = *reinterpret_cast<const uint2*>(qc + 32 * c + 8 * q4);
           qb[c][nt][0] = w.x;
           qb[c][nt][1] = w.y;
         }
-      } else {
-        // steps 2c and 2c + 1 hold, of a word's eight dims 32c + 8t + i, (0, 4 | 1, 5) and (2, 6 | 3, 7);
-        // their codes stand four bits up in the mantissa, hence the sixteenth
+      }
+      f_r[nt] = f_s[4 * nt + q4];
+      m_r[nt] = -INFINITY;
+      l_r[nt] = 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          const __half* w = qr + 32 * c + 8 * q4;
-          const __half2 k16 = __float2half2_rn(0.0625f);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const __half2 v = __hmul2(__halves2half2(w[h], w[h + 4]), k16);
-            qb[2 * c + (h >> 1)][nt][h & 1] = *reinterpret_cast<const uint32_t*>(&v);
-          }
-        }
+      for (int gr = 0; gr < NG; ++gr) {
+        qs[nt][gr] = qsum_s[4 * nt + q4][gr];
+        z[nt][gr] = 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * nt + 2 * q4 + e;
-        f_r[nt][e] = f_s[r];
-        m_r[nt][e] = -INFINITY;
-        l_r[nt][e] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          qs[nt][e][gr] = qsum_s[r][gr];
-          z[nt][e][gr] = 0.f;
-        }
-      }
+      for (int mt = 0; mt < MT; ++mt) o[mt][nt][0] = o[mt][nt][1] = 0.f;
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
     const int first_limit = cu.base + row0 / G;    // the last key the unit's first row sees
 
     const int seg = min(cu.T - c_t, n_steps - done);
@@ -419,236 +412,216 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // before the next load into this stage
       }
 
-      // ---- scores: keys on the rows (g, g + 8 of each 16), query rows 2t, 2t + 1 on the columns
+      // ---- scores: keys on the rows (g, g + 8 of each 16), query row 4 nt + t on a lane's column pair
       const uint32_t k_addr = smem_u32(kt), v_addr = smem_u32(vt);
       const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lch = lane >> 4;     // ldmatrix: (keys 0-7 | 8-15) x (chunk, next)
-      float x[KT][NT][4];
+      float x[KT][NT][2];
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         const float* sk8 = reinterpret_cast<const float*>(sc) + 16 * k + g;
         const uint32_t* sk4 = reinterpret_cast<const uint32_t*>(sc) + (16 * k + g) * NG;
-        if (BITS == 8) {
-          float acc[NT][4];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          int acc[NT][4];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = acc[nt][2] = -1152.f * qs[nt][0][0];
-            acc[nt][1] = acc[nt][3] = -1152.f * qs[nt][1][0];
+            acc[nt][0] = acc[nt][2] = 0;
+            acc[nt][1] = acc[nt][3] = BITS == 8 ? 0 : -8 * qs[nt][gr];
           }
+          if (BITS == 8) {
 #pragma unroll
-          for (int c = 0; c < D / 16; c += 2) {
-            uint32_t w[4];
-            ldmatrix_x4(w, k_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
+            for (int c = 0; c < D / 16; c += 2) {
+              uint32_t w[4];
+              ldmatrix_x4(w, k_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] ^= 0x80808080u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t a0 = __byte_perm(w[2 * h], 0x64646464u, 0x4140), a2 = __byte_perm(w[2 * h], 0x64646464u, 0x4342);
-              const uint32_t a1 = __byte_perm(w[2 * h + 1], 0x64646464u, 0x4140), a3 = __byte_perm(w[2 * h + 1], 0x64646464u, 0x4342);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16_16816(acc[nt], a0, a1, a2, a3, qb[c + h][nt][0], qb[c + h][nt][1]);
+              for (int nt = 0; nt < NT; ++nt)
+                mma_bytes<true, true>(acc[nt], w[0], w[1], w[2], w[3], qb[c / 2][nt][0], qb[c / 2][nt][1]);
             }
-          }
-          const float s_lo = sk8[0], s_hi = sk8[8];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            x[k][nt][0] = acc[nt][0] * s_lo;
-            x[k][nt][1] = acc[nt][1] * s_lo;
-            x[k][nt][2] = acc[nt][2] * s_hi;
-            x[k][nt][3] = acc[nt][3] * s_hi;
-          }
-        } else {
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            float acc[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][0] = acc[nt][2] = -72.f * qs[nt][0][gr];
-              acc[nt][1] = acc[nt][3] = -72.f * qs[nt][1][gr];
-            }
-            uint32_t w[4];
+          } else {
+            uint32_t w[4];                         // 64 dims: chunks 2 gr and 2 gr + 1
             ldmatrix_x4(w, k_addr + swizzled<RB>((16 * k + lrow) * RB + (2 * gr + lch) * 16));
+            constexpr uint32_t M = 0x0f0f0f0fu;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t lo = w[2 * h], hi = w[2 * h + 1];
-              constexpr uint32_t M = 0x00f000f0u, E = 0x64006400u;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int s = 0; s < 2; ++s) {
-                const uint32_t a0 = ((s ? lo >> 4 : lo << 4) & M) | E, a1 = ((s ? hi >> 4 : hi << 4) & M) | E;
-                const uint32_t a2 = ((s ? lo >> 8 : lo) & M) | E, a3 = ((s ? hi >> 8 : hi) & M) | E;
-                const int st2 = 2 * (2 * gr + h) + s;
+              for (int nt = 0; nt < NT; ++nt)
+                mma_bytes<false, true>(acc[nt], w[2 * h] & M, w[2 * h + 1] & M, (w[2 * h] >> 4) & M, (w[2 * h + 1] >> 4) & M,
+                                       qb[2 * gr + h][nt][0], qb[2 * gr + h][nt][1]);
+          }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16_16816(acc[nt], a0, a1, a2, a3, qb[st2][nt][0], qb[st2][nt][1]);
+          for (int h = 0; h < 2; ++h) {
+            if (BITS == 8) {
+              const float s = sk8[8 * h];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) x[k][nt][h] = (float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]) * s;
+            } else {
+              const uint32_t sm = sk4[8 * h * NG + gr];
+              const float s = __uint_as_float(sm << 16), mid = __uint_as_float(sm & 0xffff0000u);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const float part = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), s, mid * (float)qs[nt][gr]);
+                x[k][nt][h] = gr ? x[k][nt][h] + part : part;
               }
-            }
-            const uint32_t sm_lo = sk4[gr], sm_hi = sk4[8 * NG + gr];
-            const float s_lo = __uint_as_float(sm_lo << 16), mid_lo = __uint_as_float(sm_lo & 0xffff0000u);
-            const float s_hi = __uint_as_float(sm_hi << 16), mid_hi = __uint_as_float(sm_hi & 0xffff0000u);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float q0 = qs[nt][0][gr], q1 = qs[nt][1][gr];
-              const float b0 = gr ? x[k][nt][0] : 0.f, b1 = gr ? x[k][nt][1] : 0.f;
-              const float b2 = gr ? x[k][nt][2] : 0.f, b3 = gr ? x[k][nt][3] : 0.f;
-              x[k][nt][0] = fmaf(acc[nt][0], s_lo, fmaf(mid_lo, q0, b0));
-              x[k][nt][1] = fmaf(acc[nt][1], s_lo, fmaf(mid_lo, q1, b1));
-              x[k][nt][2] = fmaf(acc[nt][2], s_hi, fmaf(mid_hi, q0, b2));
-              x[k][nt][3] = fmaf(acc[nt][3], s_hi, fmaf(mid_hi, q1, b3));
             }
           }
         }
       }
 
-      // ---- probabilities: value scales of this lane's keys (g, g + 8 of each 16), exponentials, sums, and P as
-      // the second product's operand (keys on k, query rows on n)
-      uint32_t pb[KT][NT][NG][2];
+      // ---- probabilities against the row's reference m, their sum, and p sv as whole numbers of 16 bits against
+      // the step's largest, two bytes in a column pair: the second product's operand (keys on k: 2t, 2t + 8,
+      // 2t + 1, 2t + 9 of each 16)
+      uint32_t pb[KT][NT][NG];
+      float beta[NT][NG];                                   // what the step's integer sums are worth
       auto softmax = [&](auto masked_c) {
         constexpr bool MASKED = decltype(masked_c)::value;
         const unsigned char* scv = sc + C::kScaleBytes;
-        float sv[KT][2][NG], mv[KT][2][NG], top[KT][2];
-        bool seen[KT][NT][4];                               // which of the lane's (key, query row) pairs count
-        if (MASKED) {
+        float sv[KT][2][NG], low[KT][2][NG];
+        bool seen[KT][NT][2];                               // which of the lane's (key, query row) pairs count
+        float top[NT][NG];                                  // the step's largest s + log2 sv
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int limit = min(cu.base + min((row0 + 8 * nt + 2 * q4 + e) / G, cu.q_len - 1), cu.len - 1);
+          for (int gr = 0; gr < NG; ++gr) top[nt][gr] = -INFINITY;
+          if (MASKED) {
+            const int limit = min(cu.base + min((row0 + 4 * nt + q4) / G, cu.q_len - 1), cu.len - 1);
 #pragma unroll
-              for (int k = 0; k < KT; ++k)
+            for (int k = 0; k < KT; ++k)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) seen[k][nt][2 * h + e] = w0 + 16 * k + 8 * h + g <= limit;
-            }
+              for (int h = 0; h < 2; ++h) seen[k][nt][h] = w0 + 16 * k + 8 * h + g <= limit;
+          }
         }
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int key = 16 * k + 8 * h + g;
-            const bool in = !MASKED || w0 + key < cu.len;
-            if (BITS == 8) {
-              sv[k][h][0] = in ? reinterpret_cast<const float*>(scv)[key] : 0.f;
-              top[k][h] = sv[k][h][0];
-            } else {
 #pragma unroll
-              for (int gr = 0; gr < NG; ++gr) {
-                const uint32_t sm = in ? reinterpret_cast<const uint32_t*>(scv)[key * NG + gr] : 0u;
+            for (int gr = 0; gr < NG; ++gr) {
+              if (BITS == 8) {
+                sv[k][h][gr] = reinterpret_cast<const float*>(scv)[key];
+              } else {
+                const uint32_t sm = reinterpret_cast<const uint32_t*>(scv)[key * NG + gr];
                 sv[k][h][gr] = __uint_as_float(sm << 16);
-                mv[k][h][gr] = __uint_as_float(sm & 0xffff0000u);
-                top[k][h] = gr ? fmaxf(top[k][h], sv[k][h][gr]) : sv[k][h][gr];
+                low[k][h][gr] = fmaf(-8.f, sv[k][h][gr], __uint_as_float(sm & 0xffff0000u));
               }
+              // a row of zeros (or of values below 127 x 2^-100) must not move the reference without end
+              const float lg = __log2f(max_nan(sv[k][h][gr], 7.9e-31f));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                if (!MASKED || seen[k][nt][h]) top[nt][gr] = max_nan(top[nt][gr], fmaf(x[k][nt][h], f_r[nt], lg));
             }
-            // a row of zeros (or of values below 127 x 2^-100) must not lift the reference without end
-            top[k][h] = fmaxf(top[k][h], 7.9e-31f);
           }
-        float p[KT][NT][4];
-        auto exponentials = [&]() {                         // returns the largest p sv
-          float most = 0.f;
+        bool move = false;
 #pragma unroll
-          for (int k = 0; k < KT; ++k)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int gr = 0; gr < NG; ++gr) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float v = fast_exp2(fmaf(x[k][nt][e], f_r[nt][e & 1], -m_r[nt][e & 1]));
-                if (MASKED && !seen[k][nt][e]) v = 0.f;
-                p[k][nt][e] = v;
-                most = fmaxf(most, v * top[k][e >> 1]);
-              }
-          return most;
-        };
-        if (__any_sync(0xffffffffu, exponentials() > 256.f)) {
-          // move the reference to the largest s + log2 sv seen so far (the first tile, and rarely after)
+            for (int sh = 4; sh <= 16; sh <<= 1) top[nt][gr] = max_nan(top[nt][gr], __shfl_xor_sync(0xffffffffu, top[nt][gr], sh));
+            move |= top[nt][gr] > m_r[nt] + 20.f;           // p stays below 2^(20 + 100)
+          }
+        if (__any_sync(0xffffffffu, move)) {                // the unit's first step, and hardly ever after
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            float m = top[nt][0];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float mx = m_r[nt][e];
+            for (int gr = 1; gr < NG; ++gr) m = fmaxf(m, top[nt][gr]);
+            if (!(m > m_r[nt])) continue;
+            const float alpha = fast_exp2(m_r[nt] - m);
+            m_r[nt] = m;
+            l_r[nt] *= alpha;
 #pragma unroll
-              for (int k = 0; k < KT; ++k)
+            for (int gr = 0; gr < NG; ++gr) z[nt][gr] *= alpha;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  if (!MASKED || seen[k][nt][2 * h + e])
-                    mx = fmaxf(mx, fmaf(x[k][nt][2 * h + e], f_r[nt][e], __log2f(top[k][h])));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float alpha = mx == m_r[nt][e] ? 1.f : fast_exp2(m_r[nt][e] - mx);
-              m_r[nt][e] = mx;
-              l_r[nt][e] *= alpha;
-#pragma unroll
-              for (int gr = 0; gr < NG; ++gr) z[nt][e][gr] *= alpha;
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) { o[mt][nt][e] *= alpha; o[mt][nt][e + 2] *= alpha; }
-            }
-          exponentials();
+            for (int mt = 0; mt < MT; ++mt) { o[mt][nt][0] *= alpha; o[mt][nt][1] *= alpha; }
+          }
         }
+        float up[NT][NG];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            // a step that far below the reference adds nothing that 32 bits hold
+            // (nor does one of which the row sees nothing: top is -inf, and m may be)
+            float d = top[nt][gr] - m_r[nt];
+            d = d < -80.f || top[nt][gr] == -INFINITY ? -80.f : d;
+            beta[nt][gr] = fast_exp2(d) * (1.f / kFixedP);
+            up[nt][gr] = fast_exp2(-d) * kFixedP;
+          }
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            l_r[nt][0] += p[k][nt][0] + p[k][nt][2];
-            l_r[nt][1] += p[k][nt][1] + p[k][nt][3];
+            float p[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              p[h] = fast_exp2(fmaf(x[k][nt][h], f_r[nt], -m_r[nt]));
+              if (MASKED && !seen[k][nt][h]) p[h] = 0.f;
+              l_r[nt] += p[h];
+            }
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-              float v[4];
+              uint32_t y[2];                                // low 16 bits: rint(p sv up), by adding 2^23
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                // a key that the row does not see adds nothing, not 0 x NaN
-                v[e] = !MASKED || seen[k][nt][e] ? p[k][nt][e] * sv[k][e >> 1][gr] : 0.f;
-                if (BITS == 4)
-                  z[nt][e & 1][gr] = !MASKED || seen[k][nt][e] ? fmaf(p[k][nt][e], mv[k][e >> 1][gr], z[nt][e & 1][gr])
-                                                               : z[nt][e & 1][gr];
+              for (int h = 0; h < 2; ++h) {
+                y[h] = __float_as_uint(fmaf(p[h] * sv[k][h][gr], up[nt][gr], 8388608.f));
+                if (MASKED && !seen[k][nt][h]) y[h] = 0;    // not 0 x NaN of a key nobody sees
+                if (BITS == 4) {
+                  const float t = fmaf(p[h], low[k][h][gr], z[nt][gr]);
+                  z[nt][gr] = !MASKED || seen[k][nt][h] ? t : z[nt][gr];
+                }
               }
-              pb[k][nt][gr][0] = transpose_8x8(pack_f16(v[0], v[1]));
-              pb[k][nt][gr][1] = transpose_8x8(pack_f16(v[2], v[3]));
+              pb[k][nt][gr] = transpose_8x8(__byte_perm(y[0], y[1], 0x4051));     // (high g, high g + 8 | low g, low g + 8)
             }
           }
       };
       // some row does not see some key of the tile
       if (w0 + WK - 1 > min(first_limit, cu.len - 1)) softmax(std::true_type{});
       else softmax(std::false_type{});
-      // ---- O^T += V^T P^T: value dims on the rows
+      // ---- O^T += V^T P^T: value dims on the rows, four keys a register
+      // 8 bits: rows g and g + 8 of tile mt hold dims 16 mt + 2g and one more; 4 bits: of tile 2c + i dims
+      // 32c + 4g + 2i and one more
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        if (BITS == 8) {
-          // rows g and g + 8 of tile c hold dims 16c + 2g and 16c + 2g + 1
+      for (int c = 0; c < RB / 16; c += 2) {
+        uint32_t even[KT][2], odd[KT][2];                   // bytes 2g and 2g + 1 of chunks c, c + 1
 #pragma unroll
-          for (int c = 0; c < D / 16; c += 2) {
-            uint32_t w[4];
-            ldmatrix_x4_trans(w, v_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
+        for (int k = 0; k < KT; ++k) {
+          uint32_t w[4];
+          ldmatrix_x4_trans(w, v_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] ^= 0x80808080u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              constexpr uint32_t K1152 = 0x64806480u;        // 1024 + 128
-              const uint32_t a0 = h2_sub(__byte_perm(w[2 * h], 0x64646464u, 0x4240), K1152);
-              const uint32_t a1 = h2_sub(__byte_perm(w[2 * h], 0x64646464u, 0x4341), K1152);
-              const uint32_t a2 = h2_sub(__byte_perm(w[2 * h + 1], 0x64646464u, 0x4240), K1152);
-              const uint32_t a3 = h2_sub(__byte_perm(w[2 * h + 1], 0x64646464u, 0x4341), K1152);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[c + h][nt], a0, a1, a2, a3, pb[k][nt][0][0], pb[k][nt][0][1]);
-            }
-          }
-        } else {
-          // rows g and g + 8 of tile 2c + h hold dims 32c + 4g + 2h and one more
-#pragma unroll
-          for (int c = 0; c < D / 32; c += 2) {
-            uint32_t w[4];
-            ldmatrix_x4_trans(w, v_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u, E = 0x64006400u;
-              constexpr uint32_t K1032 = 0x64086408u, K16TH = 0x2c002c00u, KM72 = 0xd480d480u;   // 1032, 1/16, -72
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t u = h ? w[2 * i] >> 8 : w[2 * i], v = h ? w[2 * i + 1] >> 8 : w[2 * i + 1];
-                const uint32_t a0 = h2_sub((u & LO) | E, K1032), a1 = h2_fma((u & HI) | E, K16TH, KM72);
-                const uint32_t a2 = h2_sub((v & LO) | E, K1032), a3 = h2_fma((v & HI) | E, K16TH, KM72);
-                const int mt = 2 * (c + i) + h, gr = mt * 16 / kQuantGroup;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[mt][nt], a0, a1, a2, a3, pb[k][nt][gr][0], pb[k][nt][gr][1]);
-              }
-            }
+          for (int i = 0; i < 2; ++i) {
+            even[k][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x6240);
+            odd[k][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7351);
           }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int part = 0; part < 8 / BITS; ++part) {
+            const int mt = BITS == 8 ? c + i : 2 * (c + i) + part, gr = BITS == 8 ? 0 : mt * 16 / kQuantGroup;
+            int acc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
+#pragma unroll
+            for (int k = 0; k < KT; k += 2) {
+              constexpr uint32_t M = 0x0f0f0f0fu;
+              uint32_t a[4];
+              if (BITS == 8) {
+                a[0] = even[k][i]; a[1] = odd[k][i]; a[2] = even[k + 1][i]; a[3] = odd[k + 1][i];
+              } else {
+                const uint32_t u = part ? odd[k][i] : even[k][i], v = part ? odd[k + 1][i] : even[k + 1][i];
+                a[0] = u & M; a[1] = (u >> 4) & M; a[2] = v & M; a[3] = (v >> 4) & M;
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_bytes<BITS == 8, false>(acc[nt], a[0], a[1], a[2], a[3], pb[k][nt][gr], pb[k + 1][nt][gr]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                o[mt][nt][h] = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), beta[nt][gr], o[mt][nt][h]);
+          }
       }
       ++consumed;
       __syncwarp();                                          // every lane has read the stage
@@ -657,57 +630,55 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 
     // ---- the unit's end in this block: lanes, then warps
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int sh = 4; sh <= 16; sh <<= 1) {
+        l_r[nt] += __shfl_xor_sync(0xffffffffu, l_r[nt], sh);
 #pragma unroll
-        for (int sh = 4; sh <= 16; sh <<= 1) {
-          l_r[nt][e] += __shfl_xor_sync(0xffffffffu, l_r[nt][e], sh);
+        for (int gr = 0; gr < NG; ++gr) z[nt][gr] += __shfl_xor_sync(0xffffffffu, z[nt][gr], sh);
+      }
+      if (BITS == 4) {
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) z[nt][e][gr] += __shfl_xor_sync(0xffffffffu, z[nt][e][gr], sh);
-        }
-        if (BITS == 4) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            o[mt][nt][e] += z[nt][e][mt * 16 / kQuantGroup];
-            o[mt][nt][e + 2] += z[nt][e][mt * 16 / kQuantGroup];
-          }
+        for (int mt = 0; mt < MT; ++mt) {
+          o[mt][nt][0] += z[nt][mt * 16 / kQuantGroup];
+          o[mt][nt][1] += z[nt][mt * 16 / kQuantGroup];
         }
       }
+    }
     float* join = reinterpret_cast<float*>(smem + C::kJoin);
     auto put = [&](int buf) {
-      float* j = join + buf * C::kRegs * 32 + lane;
+      float2* j = reinterpret_cast<float2*>(join + buf * C::kRegs * 32) + lane;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) j[(mt * NT + nt) * 32] = make_float2(o[mt][nt][0], o[mt][nt][1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) j[((mt * NT + nt) * 4 + e) * 32] = o[mt][nt][e];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          ml_s[buf][nt * 4 + e][lane] = m_r[nt][e];
-          ml_s[buf][nt * 4 + 2 + e][lane] = l_r[nt][e];
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        ml_s[buf][nt * 2][lane] = m_r[nt];
+        ml_s[buf][nt * 2 + 1][lane] = l_r[nt];
+      }
+    };
+    // (m, l, o) of two parts of a row's keys as one
+    auto factors = [](float& m, float& l, float m2, float l2, float& fa, float& fb) {
+      const float mx = fmaxf(m, m2);
+      fa = m == mx ? 1.f : fast_exp2(m - mx);
+      fb = m2 == mx ? 1.f : fast_exp2(m2 - mx);
+      m = mx;
+      l = l * fa + l2 * fb;
     };
     auto add = [&](int buf) {
-      const float* j = join + buf * C::kRegs * 32 + lane;
+      const float2* j = reinterpret_cast<const float2*>(join + buf * C::kRegs * 32) + lane;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float fa, fb;
+        factors(m_r[nt], l_r[nt], ml_s[buf][nt * 2][lane], ml_s[buf][nt * 2 + 1][lane], fa, fb);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float m2 = ml_s[buf][nt * 4 + e][lane], l2 = ml_s[buf][nt * 4 + 2 + e][lane];
-          const float mx = fmaxf(m_r[nt][e], m2);
-          const float fa = m_r[nt][e] == mx ? 1.f : fast_exp2(m_r[nt][e] - mx), fb = m2 == mx ? 1.f : fast_exp2(m2 - mx);
-          m_r[nt][e] = mx;
-          l_r[nt][e] = l_r[nt][e] * fa + l2 * fb;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              o[mt][nt][e + 2 * h] = o[mt][nt][e + 2 * h] * fa + j[((mt * NT + nt) * 4 + e + 2 * h) * 32] * fb;
+        for (int mt = 0; mt < MT; ++mt) {
+          const float2 v = j[(mt * NT + nt) * 32];
+          o[mt][nt][0] = o[mt][nt][0] * fa + v.x * fb;
+          o[mt][nt][1] = o[mt][nt][1] * fa + v.y * fb;
         }
+      }
     };
     if (warp & 1) put(warp >> 1);
     __syncthreads();
@@ -716,38 +687,29 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     __syncthreads();
     const long long unit_end = unit_begin + cu.T;
     const bool whole = unit_begin >= begin && unit_end <= end;
-    const int dim0 = BITS == 8 ? 2 * g : 4 * g;
-    auto store = [&](int mt, int nt, float (&acc)[4], const float (&inv)[2]) {
-      const int dim = BITS == 8 ? 16 * mt + dim0 : 32 * (mt >> 1) + dim0 + 2 * (mt & 1);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = row0 + 8 * nt + 2 * q4 + e;
-        if (row < rows)
-          *reinterpret_cast<uint32_t*>(P.out + (size_t)(cu.t0 + row / G) * P.Hq * D + (size_t)(c_kvh * G + row % G) * D + dim) =
-              pack_bf16(acc[e] * inv[e], acc[e + 2] * inv[e]);
-      }
+    auto store = [&](int mt, int nt, float a, float b) {
+      const int dim = BITS == 8 ? 16 * mt + 2 * g : 32 * (mt >> 1) + 4 * g + 2 * (mt & 1), row = row0 + 4 * nt + q4;
+      if (row < rows)
+        *reinterpret_cast<uint32_t*>(P.out + (size_t)(cu.t0 + row / G) * P.Hq * D + (size_t)(c_kvh * G + row % G) * D + dim) =
+            pack_bf16(a, b);
     };
     if (warp == 0) {
       add(1);
       if (whole) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float inv[2] = {1.f / l_r[nt][0], 1.f / l_r[nt][1]};
+          const float inv = 1.f / l_r[nt];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) store(mt, nt, o[mt][nt], inv);
+          for (int mt = 0; mt < MT; ++mt) store(mt, nt, o[mt][nt][0] * inv, o[mt][nt][1] * inv);
         }
       } else {
-        float* seg_out = P.scratch + ((size_t)blockIdx.x * 2 + (begin >= unit_begin ? 0 : 1)) * C::kSegFloats;
+        float2* seg_out = reinterpret_cast<float2*>(P.scratch + ((size_t)blockIdx.x * 2 + (begin >= unit_begin ? 0 : 1)) * C::kSegFloats) + lane;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            __stcg(reinterpret_cast<float4*>(seg_out) + (mt * NT + nt) * 32 + lane,
-                   make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]));
+          for (int nt = 0; nt < NT; ++nt) __stcg(seg_out + (mt * NT + nt) * 32, make_float2(o[mt][nt][0], o[mt][nt][1]));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          __stcg(reinterpret_cast<float4*>(seg_out) + (MT * NT + nt) * 32 + lane,
-                 make_float4(m_r[nt][0], m_r[nt][1], l_r[nt][0], l_r[nt][1]));
+        for (int nt = 0; nt < NT; ++nt) __stcg(seg_out + (MT * NT + nt) * 32, make_float2(m_r[nt], l_r[nt]));
       }
     }
     if (!whole) {
@@ -767,23 +729,23 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       __syncthreads();
       if (last_s) {
         __threadfence();
-        // warp w joins the row tiles mt = w, w + 4, ... of all segments
+        // warp w joins the tiles mt = w, w + 4, ... of all segments, U segments asked for together
         auto seg_at = [&](int i) {
           const long long bi = total * i / nb;
-          return reinterpret_cast<const float4*>(P.scratch + ((size_t)i * 2 + (bi >= unit_begin ? 0 : 1)) * C::kSegFloats) + lane;
+          return reinterpret_cast<const float2*>(P.scratch + ((size_t)i * 2 + (bi >= unit_begin ? 0 : 1)) * C::kSegFloats) + lane;
         };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.f, 0.f};
-          float4 acc[MT / 4];
+          float mx = -INFINITY, ls = 0.f;
+          float2 acc[MT / 4];
 #pragma unroll
-          for (int j = 0; j < MT / 4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < MT / 4; ++j) acc[j] = make_float2(0.f, 0.f);
           constexpr int U = 8;
           for (int i0 = first; i0 <= last; i0 += U) {
-            float4 ml[U], a[U][MT / 4];
+            float2 ml[U], a[U][MT / 4];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-              const float4* s = seg_at(min(i0 + u, last));
+              const float2* s = seg_at(min(i0 + u, last));
               ml[u] = __ldcg(s + (MT * NT + nt) * 32);
 #pragma unroll
               for (int j = 0; j < MT / 4; ++j) a[u][j] = __ldcg(s + ((4 * j + warp) * NT + nt) * 32);
@@ -791,31 +753,18 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               if (i0 + u > last) break;
-              const float m2[2] = {ml[u].x, ml[u].y}, l2[2] = {ml[u].z, ml[u].w};
-              float fa[2], fb[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float m = fmaxf(mx[e], m2[e]);
-                fa[e] = mx[e] == m ? 1.f : fast_exp2(mx[e] - m);
-                fb[e] = m2[e] == m ? 1.f : fast_exp2(m2[e] - m);
-                mx[e] = m;
-                ls[e] = ls[e] * fa[e] + l2[e] * fb[e];
-              }
+              float fa, fb;
+              factors(mx, ls, ml[u].x, ml[u].y, fa, fb);
 #pragma unroll
               for (int j = 0; j < MT / 4; ++j) {
-                acc[j].x = acc[j].x * fa[0] + a[u][j].x * fb[0];
-                acc[j].y = acc[j].y * fa[1] + a[u][j].y * fb[1];
-                acc[j].z = acc[j].z * fa[0] + a[u][j].z * fb[0];
-                acc[j].w = acc[j].w * fa[1] + a[u][j].w * fb[1];
+                acc[j].x = acc[j].x * fa + a[u][j].x * fb;
+                acc[j].y = acc[j].y * fa + a[u][j].y * fb;
               }
             }
           }
-          const float inv[2] = {1.f / ls[0], 1.f / ls[1]};
+          const float inv = 1.f / ls;
 #pragma unroll
-          for (int j = 0; j < MT / 4; ++j) {
-            float r[4] = {acc[j].x, acc[j].y, acc[j].z, acc[j].w};
-            store(4 * j + warp, nt, r, inv);
-          }
+          for (int j = 0; j < MT / 4; ++j) store(4 * j + warp, nt, acc[j].x * inv, acc[j].y * inv);
         }
       }
     }
@@ -871,8 +820,13 @@ static int launch_quant(const QuantAttnParams& p, int blocks, cudaStream_t strea
   return (int)launch_kernel(kern, dim3(blocks), dim3(128), smem, stream, p, k_map, v_map);
 }
 
-// Query rows of a unit for up to `rows` (new tokens x heads of a group) rows a sequence.
-static int row_tiles_of(int rows) { return rows <= 8 ? 1 : 2; }
+// Column tiles (of four query rows) of a unit for up to `rows` (new tokens x heads of a group) a sequence.
+static int column_tiles_of(int rows) { return rows <= 4 ? 1 : rows <= 8 ? 2 : 4; }
+
+template <int BITS, int D>
+static int blocks_per_sm(int nt) {
+  return nt == 1 ? QuantAttn<BITS, D, 1>::kBlocksPerSM : nt == 2 ? QuantAttn<BITS, D, 2>::kBlocksPerSM : QuantAttn<BITS, D, 4>::kBlocksPerSM;
+}
 
 }  // namespace siar
 
@@ -887,17 +841,19 @@ extern "C" int siar_attn_quant_supported(int Hq, int Hkv, int D, int page_tokens
 }
 
 // Blocks of a launch (the counters it needs); more never help: a block step is the least share.
-extern "C" int siar_attn_quant_blocks(int B, int Hq, int Hkv, int D, int max_q_len, int max_kv_len, int sm_count) {
-  const int rows = max_q_len * (Hq / Hkv), per_unit = 8 * row_tiles_of(rows);
-  const int keys = D == 128 ? 128 : 256;
-  const long long steps = (long long)B * Hkv * ((rows + per_unit - 1) / per_unit) * ((max_kv_len + keys - 1) / keys);
-  return (int)(steps < 2ll * sm_count ? (steps > 0 ? steps : 1) : 2ll * sm_count);
+extern "C" int siar_attn_quant_blocks(int bits, int B, int Hq, int Hkv, int D, int max_q_len, int max_kv_len, int sm_count) {
+  const int rows = max_q_len * (Hq / Hkv), nt = column_tiles_of(rows);
+  const int keys = D == 128 ? QuantAttn<8, 128, 1>::kBlockKeys : QuantAttn<8, 64, 1>::kBlockKeys;
+  const long long steps = (long long)B * Hkv * ((rows + 4 * nt - 1) / (4 * nt)) * ((max_kv_len + keys - 1) / keys);
+  const long long most = (long long)sm_count * (bits == 8 ? D == 128 ? blocks_per_sm<8, 128>(nt) : blocks_per_sm<8, 64>(nt)
+                                                          : D == 128 ? blocks_per_sm<4, 128>(nt) : blocks_per_sm<4, 64>(nt));
+  return (int)(steps < most ? (steps > 0 ? steps : 1) : most);
 }
 
 // Scratch floats for that many blocks.
 extern "C" long long siar_attn_quant_scratch_floats(int Hq, int Hkv, int D, int max_q_len, int blocks) {
-  const int nt = row_tiles_of(max_q_len * (Hq / Hkv));
-  return (long long)blocks * 2 * ((long long)(D / 16) * nt * 4 + 4 * nt) * 32;
+  const int nt = column_tiles_of(max_q_len * (Hq / Hkv));
+  return (long long)blocks * 2 * ((D / 16) * nt * 2 + 2 * nt) * 32;
 }
 
 // What tells one capture of a stream from another (0: the stream is not being captured).
@@ -925,9 +881,10 @@ extern "C" int siar_attn_quant(int bits, const void* qkv, void* k_pool, void* v_
                        q_start, base_len, inv_freq, (__nv_bfloat16*)out, scratch, counters, status, B, Hq, Hkv, page_tokens,
                        max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused, write_kv, scale * 1.4426950408889634f};
   cudaStream_t s = (cudaStream_t)stream;
-  const int nt = row_tiles_of(max_q_len * (Hq / Hkv));
-#define SIAR_GO(BITS, DIM) \
-  return nt == 1 ? launch_quant<BITS, DIM, 1>(p, blocks, s) : launch_quant<BITS, DIM, 2>(p, blocks, s)
+  const int nt = column_tiles_of(max_q_len * (Hq / Hkv));
+#define SIAR_GO(BITS, DIM)                                                                     \
+  return nt == 1 ? launch_quant<BITS, DIM, 1>(p, blocks, s) : nt == 2 ? launch_quant<BITS, DIM, 2>(p, blocks, s) \
+                                                                      : launch_quant<BITS, DIM, 4>(p, blocks, s)
   if (bits == 8) {
     if (D == 64) { SIAR_GO(8, 64); }
     SIAR_GO(8, 128);

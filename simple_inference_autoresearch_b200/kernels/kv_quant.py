@@ -170,7 +170,7 @@ def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fus
     out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
     with ops._on_device(qkv):
         blocks = ops._fn("attention_quant", "siar_attn_quant_blocks")(
-            meta.n_seqs, n_heads, n_kv_heads, head_dim, meta.max_q_len, meta.max_kv_len, ops._sm_count(device))
+            kv.bits, meta.n_seqs, n_heads, n_kv_heads, head_dim, meta.max_q_len, meta.max_kv_len, ops._sm_count(device))
         fn = ops._fn("attention_quant", "siar_attn_quant_scratch_floats")
         fn.restype = ops.c_longlong
         scratch = torch.empty(fn(n_heads, n_kv_heads, head_dim, meta.max_q_len, blocks), dtype=torch.float32, device=device)

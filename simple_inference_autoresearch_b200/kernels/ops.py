@@ -91,7 +91,7 @@ _signatures = {
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
         "siar_attn_quant_supported": [c_int, c_int, c_int, c_int, c_longlong],
-        "siar_attn_quant_blocks": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+        "siar_attn_quant_blocks": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int],
         "siar_attn_quant_scratch_floats": [c_int, c_int, c_int, c_int, c_int],
         "siar_capture_id": [c_void_p],
     },

@@ -180,6 +180,13 @@ def attention_bounds(batch, q, kv, scale, window=None):
         exp(+-2 d) (its own score and the sum's), and the result by at most
         ((exp(2 d_max) - 1) + 3 u) sum_j p_j |v_j| + u |out|          (float32: + 2^-12 for the sums).
 
+    The kernel that works on the codes (bfloat16) rounds p_j s_j (s_j the value's scale) to 16 bits of the
+    largest P of a step of keys: by at most P / (2 x 65500) each, times a code of at most 127 (8 bits, 127 s
+    <= max|v|) or 15 (4 bits, 15 s = a run's range <= 2 max|v|), so n keys add at most n p_max max|v| 2^-16;
+    and in 4 bits it forms a value as code x s + (mid - 8 s), two sums whose terms are at most 4 max|v|
+    together and whose factors (two exponentials of 2^-22, a handful of roundings of 2^-24) are right to
+    2^-20 of that: 2^-18 max|v| more, also where the value itself is zero.
+
     The rms counts those roundings as independent and even within half a step (variance u^2 / 3), and the
     float32 sums too, w = 2^-24: a score is a sum of D terms, the result and its divisor are sums of n terms;
     each addition rounds a partial sum, which is at most the sum of the absolute terms, so they add at most
@@ -211,7 +218,12 @@ def attention_bounds(batch, q, kv, scale, window=None):
             pv = (p[..., None] * vv.abs()).sum(0)
             small = 2.0 ** -12 if batch.qkv.dtype == torch.float32 else 0.0
             out[t0 + i] = o
-            bound[t0 + i] = (torch.expm1(2 * dmax)[:, None] + 3 * u + small * u) * pv + u * o.abs() + 1e-7 * pv
+            if batch.qkv.dtype == torch.bfloat16:
+                vmax = vv.abs().amax((0, 2))[:, None]
+                extra = len(kk) * p.amax(0)[:, None] * vmax * 2.0 ** -16 + vmax * 2.0 ** -18
+            else:
+                extra = 0.0
+            bound[t0 + i] = extra + (torch.expm1(2 * dmax)[:, None] + 3 * u + small * u) * pv + u * o.abs() + 1e-7 * pv
             dvar = (u * scale) ** 2 * 2 / 3 * terms.square().sum(-1) + \
                 d * w * w / 3 * (scale * terms.abs().sum(-1)).square()  # of a score
             var[t0 + i] = ((dvar[..., None] + 2 * u * u / 3) * (p[..., None] * (vv - o)).square()).sum(0) + \
