@@ -66,8 +66,8 @@ struct QuantAttn {
   static constexpr int kGroups = BITS == 8 ? 1 : D / kQuantGroup;
   static constexpr int kScaleBytes = kWarpKeys * 4 * kGroups;        // float32, or (scale, mid) bfloat16 per run
   // blocks an SM and pipeline depth: what shared memory (and, for many rows, registers) leave room for
-  static constexpr int kBlocksPerSM = NT == 4 ? 2 : 3;
-  static constexpr int kStages = kTileBytes < 4096 ? (NT == 4 ? 4 : 3) : 2;
+  static constexpr int kBlocksPerSM = NT == 1 ? 3 : 2;
+  static constexpr int kStages = kTileBytes < 4096 ? (NT == 1 ? 3 : NT == 2 ? 5 : 4) : NT == 2 ? 3 : 2;
   static constexpr int kRows = 4 * NT;                               // query rows of a unit
   static constexpr int kMT = D / 16;                                 // row tiles of the value product
   static constexpr int kQStride = D + 16;                            // bytes per column of query bytes in shared memory
@@ -79,6 +79,8 @@ struct QuantAttn {
   static constexpr int kQ = kJoin + 2 * kRegs * 32 * 4;
   static constexpr int kSmem = kQ + 8 * NT * kQStride;
   static constexpr int kSegFloats = (kRegs + 2 * NT) * 32;           // accumulators, references, sums
+  // an SM has 228 KB, of which every block takes 1 KB, its static arrays (under 4.2 KB) and what aligns the tiles
+  static_assert(kBlocksPerSM * (kSmem + 1024 + 1024 + (NT == 1 ? 1500 : NT == 2 ? 2100 : 3300)) <= 228 * 1024, "blocks an SM");
 };
 constexpr float kFixedP = 65500.f;                // p sv of a step's largest term, as a whole number
 
@@ -133,7 +135,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   unsigned char* smem = smem_base + ((1024 - (smem_u32(smem_base) & 1023)) & 1023);     // the swizzle pattern's period
   __shared__ __align__(8) uint64_t bars[4][C::kStages];
   __shared__ float cs_s[D];                       // cosines, sines of the new token's position
-  __shared__ float row_s[D];                      // the new token's key, then value
+  __shared__ __align__(16) uint32_t new_codes[2][RB / 4];     // the new token's key and value,
+  __shared__ uint32_t new_scale[2][NG];                       // codes and scales
   __shared__ float f_s[C::kRows];
   __shared__ int qsum_s[C::kRows][NG];
   __shared__ float ml_s[2][NT * 2][32];
@@ -145,6 +148,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
+  float freq = 0.f;                               // a constant of the model, so it may be read in front of the wait
+  if (P.fused && P.inv_freq != nullptr && threadIdx.x < D / 2) freq = P.inv_freq[threadIdx.x];
   pdl_wait();
   asm volatile("fence.proxy.async.global;" ::: "memory");      // rows that the kernel in front stored, for the TMA
 
@@ -169,25 +174,33 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     const QuantSeq s = load_seq(b);
     return (long long)s.T * s.row_tiles * P.Hkv;
   };
-  long long total = 0;
-  for (int b = lane; b < P.B; b += 32) total += steps_of(b);
+  long long sum = 0;
+  for (int b = lane; b < P.B; b += 32) sum += steps_of(b);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (sum > 0x7fffffff) {
+    if (threadIdx.x == 0) atomicOr(P.status, kStatusLengthPastGrid);
+    return;
+  }
+  const int total = (int)sum;
   // at least one step a block: a block without one would be waited for by the join of a unit around it
-  const int nb = (int)min((long long)gridDim.x, total);
+  const int nb = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= nb) return;
-  const long long begin = total * blockIdx.x / nb, end = total * (blockIdx.x + 1) / nb;
+  const int each = total / nb, odd = total % nb;  // the first `odd` blocks take one step more
+  auto begin_of = [&](int i) { return i * each + min(i, odd); };
+  auto block_of = [&](int step) { return step < odd * (each + 1) ? step / (each + 1) : odd + (step - odd * (each + 1)) / each; };
+  const int begin = begin_of(blockIdx.x), end = begin_of(blockIdx.x + 1);
   QuantSeq cu;                                    // unit that is computed: sequence, row tile, kv head, step
   int c_rt, c_kvh, c_t;
-  long long unit_begin;                           // first step of the current unit in the whole row
+  int unit_begin;                                 // first step of the current unit in the whole row
   {
-    long long before = 0;
-    int b0 = 0;
+    int before = 0, b0 = 0;
     while (true) {                                // 32 sequences at a time
-      long long mine = b0 + lane < P.B ? steps_of(b0 + lane) : 0, incl = mine;
+      const int mine = b0 + lane < P.B ? (int)steps_of(b0 + lane) : 0;
+      int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
       const unsigned past = __ballot_sync(0xffffffffu, before + incl > begin);
@@ -200,20 +213,47 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       before += __shfl_sync(0xffffffffu, incl, 31);
       b0 += 32;
     }
-    const int in_seq = (int)(begin - before), unit = in_seq / cu.T;
+    const int in_seq = begin - before, unit = in_seq / cu.T;
     c_t = in_seq % cu.T;
     c_rt = unit / P.Hkv;
     c_kvh = unit % P.Hkv;
     unit_begin = begin - c_t;
   }
-  const int n_steps = (int)(end - begin);
+  const int n_steps = end - begin;
+  auto page_index = [&](int pos) { return P.page_shift >= 0 ? pos >> P.page_shift : pos / P.page_tokens; };
+
+  // ---- the unit's query rows (a warp takes rows warp, warp + 4, ...; a lane dims lane + 32 i) and, where the
+  // unit's last step falls into this block, the new token's key (warp 0) and value (warp 1).  They are asked for
+  // ahead of the block's first tiles, and ahead of the join in front of a later unit.
+  const size_t qkv_row = (size_t)(P.Hq + 2 * P.Hkv) * D;
+  float qa[NT][D / 32], ta[D / 32];
+  int t_page = -1;                                // the page of the new token
+  auto has_new = [&](const QuantSeq& s, int t, int left) {       // left: steps of the block from t on
+    return P.fused && P.write_kv && s.base < cap && s.base / C::kBlockKeys >= t && s.base / C::kBlockKeys < t + left;
+  };
+  auto fetch = [&](const QuantSeq& s, int rt, int kvh, int t, int left) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int row = rt * C::kRows + 4 * j + warp;
+      const bool in = row < s.q_len * G;
+      const __nv_bfloat16* src = P.qkv + (size_t)(s.t0 + (in ? row / G : 0)) * qkv_row + (size_t)(kvh * G + (in ? row % G : 0)) * D + lane;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) qa[j][i] = in ? __bfloat162float(src[32 * i]) : 0.f;
+    }
+    if (warp < 2 && has_new(s, t, left)) {
+      const __nv_bfloat16* src = P.qkv + (size_t)s.t0 * qkv_row + (size_t)(P.Hq + warp * P.Hkv + kvh) * D + lane;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) ta[i] = __bfloat162float(src[32 * i]);
+      t_page = P.block_table[(size_t)s.slot * P.max_pages + page_index(s.base)];
+    }
+  };
+  fetch(cu, c_rt, c_kvh, c_t, n_steps);
 
   // ---- this warp's loads: the same walk, ahead of the computation
   QuantSeq lu = cu;
   int l_rt = c_rt, l_kvh = c_kvh, l_t = c_t, l_left = n_steps;
   int issued = 0, consumed = 0;
   bool absent_page = false;
-  auto page_index = [&](int pos) { return P.page_shift >= 0 ? pos >> P.page_shift : pos / P.page_tokens; };
   auto next_seq = [&](const QuantSeq& s) {        // the next sequence that has steps (there is one)
     int b = s.b + 1;
     QuantSeq n = load_seq(b);
@@ -266,40 +306,67 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   float o[MT][NT][2];                             // dims (row g, row g + 8 of tile mt) of query row 4 nt + t
   float m_r[NT], l_r[NT], f_r[NT], z[NT][NG];
   int qs[NT][NG];
+  float qsf[NT][NG];
   uint32_t qb[D / 32][NT][2];
   bool expired = false;
-  const size_t qkv_row = (size_t)(P.Hq + 2 * P.Hkv) * D;
   int cs_b = -1;
 
   for (int done = 0; done < n_steps;) {
     // ---- the unit's query rows: rotated if asked, whole numbers of 16 bits in two bytes
-    const int rows = cu.q_len * G, row0 = c_rt * C::kRows;
-    if (P.fused && cs_b != cu.b && P.inv_freq != nullptr) {
+    const int rows = cu.q_len * G, row0 = c_rt * C::kRows, seg = min(cu.T - c_t, n_steps - done);
+    const bool turn = P.fused && P.inv_freq != nullptr, fresh = has_new(cu, c_t, seg);
+    if (turn && cs_b != cu.b) {
       __syncthreads();
-      if (threadIdx.x < D / 2) rotation(cu.base, P.inv_freq[threadIdx.x], &cs_s[threadIdx.x], &cs_s[D / 2 + threadIdx.x]);
+      if (threadIdx.x < D / 2) rotation(cu.base, freq, &cs_s[threadIdx.x], &cs_s[D / 2 + threadIdx.x]);
       cs_b = cu.b;
     }
     __syncthreads();
-    signed char* q_s = reinterpret_cast<signed char*>(smem + C::kQ);     // column 2r: high bytes of row r, 2r + 1: low bytes
-    for (int r = warp; r < C::kRows; r += 4) {
-      const int row = row0 + r;
-      float a[D / 32], amax = 0.f;                 // dims lane + 32 i
+    auto rotate = [&](float (&a)[D / 32]) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) a[i] = 0.f;
-      if (row < rows) {
-        const __nv_bfloat16* src = P.qkv + (size_t)(cu.t0 + row / G) * qkv_row + (size_t)(c_kvh * G + row % G) * D + lane;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) a[i] = __bfloat162float(src[32 * i]);
-        if (P.fused && P.inv_freq != nullptr) {
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            const float cv = cs_s[i * 32 + lane], sv = cs_s[D / 2 + i * 32 + lane];
-            const float lo = rotate_lo(a[i], a[i + D / 64], cv, sv);
-            a[i + D / 64] = rotate_hi(a[i], a[i + D / 64], cv, sv);
-            a[i] = lo;
-          }
-        }
+      for (int i = 0; i < D / 64; ++i) {
+        const float cv = cs_s[i * 32 + lane], sv = cs_s[D / 2 + i * 32 + lane];
+        const float lo = rotate_lo(a[i], a[i + D / 64], cv, sv);
+        a[i + D / 64] = rotate_hi(a[i], a[i + D / 64], cv, sv);
+        a[i] = lo;
       }
+    };
+    if (fresh && warp < 2) {
+      // the new token's row: rotated, quantised, into the cache and, for the tile that it belongs to, shared memory
+      if (turn && warp == 0) rotate(ta);
+      float* row_s = reinterpret_cast<float*>(smem + C::kJoin) + warp * D;      // (no join is under way)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) row_s[32 * i + lane] = ta[i];
+      __syncwarp();
+      const bool held = t_page >= 0 && t_page < P.n_pages;
+      absent_page |= !held;
+      const size_t prow = ((size_t)(held ? t_page : 0) * P.Hkv + c_kvh) * P.page_tokens + cu.base - page_index(cu.base) * P.page_tokens;
+      uint8_t* dst = (warp == 0 ? P.k_pool : P.v_pool) + prow * RB;
+      uint32_t* scale_dst = reinterpret_cast<uint32_t*>(warp == 0 ? P.k_scale : P.v_scale) + prow * NG;
+      uint8_t* tile = reinterpret_cast<uint8_t*>(new_codes[warp]);
+      quantize_row<BITS>(
+          row_s, D, lane,
+          [&](int d, uint32_t c) {
+            if (BITS == 8) {
+              *reinterpret_cast<uint16_t*>(tile + d) = (uint16_t)c;
+              if (held) *reinterpret_cast<uint16_t*>(dst + d) = (uint16_t)c;
+            } else {
+              tile[d / 2] = (uint8_t)c;
+              if (held) dst[d / 2] = (uint8_t)c;
+            }
+          },
+          [&](int gr, float s, __nv_bfloat162 sm) {
+            const uint32_t w = BITS == 8 ? __float_as_uint(s) : *reinterpret_cast<const uint32_t*>(&sm);
+            new_scale[warp][gr] = w;
+            if (held) scale_dst[gr] = w;
+          });
+    }
+    signed char* q_s = reinterpret_cast<signed char*>(smem + C::kQ);     // column 2r: high bytes of row r, 2r + 1: low bytes
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int r = 4 * j + warp;
+      float (&a)[D / 32] = qa[j];
+      if (turn) rotate(a);
+      float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) amax = max_nan(amax, fabsf(a[i]));
 #pragma unroll
@@ -347,6 +414,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         qs[nt][gr] = qsum_s[4 * nt + q4][gr];
+        qsf[nt][gr] = (float)qs[nt][gr];
         z[nt][gr] = 0.f;
       }
 #pragma unroll
@@ -354,7 +422,6 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     }
     const int first_limit = cu.base + row0 / G;    // the last key the unit's first row sees
 
-    const int seg = min(cu.T - c_t, n_steps - done);
     for (int st = 0; st < seg; ++st) {
       const int w0 = (c_t + st) * C::kBlockKeys + warp * WK;
       if (w0 >= cu.len) break;
@@ -364,52 +431,20 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       unsigned char* vt = kt + C::kTileBytes;
       unsigned char* sc = smem + C::kScales + (stage * 4 + warp) * 2 * C::kScaleBytes;
 
-      if (P.fused && P.write_kv && cu.base >= w0 && cu.base < w0 + WK && cu.base < cap) {
-        // the new token's row: rotated, quantised, into the cache and over the row that was loaded
+      if (fresh && cu.base >= w0 && cu.base < w0 + WK) {
+        // over the row that was loaded
         const int at = cu.base - w0;
-        const int page = P.block_table[(size_t)cu.slot * P.max_pages + cu.base / P.page_tokens];
-        const bool held = page >= 0 && page < P.n_pages;
-        absent_page |= !held;
-        const size_t prow = ((size_t)(held ? page : 0) * P.Hkv + c_kvh) * P.page_tokens + cu.base % P.page_tokens;
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          const __nv_bfloat16* src = P.qkv + (size_t)cu.t0 * qkv_row + (size_t)(P.Hq + kv * P.Hkv + c_kvh) * D;
-          for (int i = lane; i < D / 2; i += 32) {
-            const float a = __bfloat162float(src[i]), c = __bfloat162float(src[i + D / 2]);
-            const bool turn = kv == 0 && P.inv_freq != nullptr;
-            row_s[i] = turn ? rotate_lo(a, c, cs_s[i], cs_s[D / 2 + i]) : a;
-            row_s[i + D / 2] = turn ? rotate_hi(a, c, cs_s[i], cs_s[D / 2 + i]) : c;
-          }
-          __syncwarp();
-          uint8_t* dst = (kv == 0 ? P.k_pool : P.v_pool) + prow * RB;
-          float* s8 = reinterpret_cast<float*>(kv == 0 ? P.k_scale : P.v_scale) + prow;
-          __nv_bfloat162* s4 = reinterpret_cast<__nv_bfloat162*>(kv == 0 ? P.k_scale : P.v_scale) + prow * NG;
-          unsigned char* tile = kv == 0 ? kt : vt;
-          unsigned char* scl = sc + kv * C::kScaleBytes + at * 4 * NG;
-          quantize_row<BITS>(
-              row_s, D, lane,
-              [&](int d, uint32_t c) {
-                const uint32_t off = swizzled<RB>((uint32_t)(at * RB + d * BITS / 8));
-                if (BITS == 8) {
-                  *reinterpret_cast<uint16_t*>(tile + off) = (uint16_t)c;
-                  if (held) *reinterpret_cast<uint16_t*>(dst + d) = (uint16_t)c;
-                } else {
-                  tile[off] = (uint8_t)c;
-                  if (held) dst[d / 2] = (uint8_t)c;
-                }
-              },
-              [&](int gr, float s, __nv_bfloat162 sm) {
-                if (BITS == 8) {
-                  *reinterpret_cast<float*>(scl) = s;
-                  if (held) *s8 = s;
-                } else {
-                  reinterpret_cast<__nv_bfloat162*>(scl)[gr] = sm;
-                  if (held) s4[gr] = sm;
-                }
-              });
-          __syncwarp();
+        if (lane < RB / 4) {
+          const uint32_t off = swizzled<RB>((uint32_t)(at * RB + lane * 4));
+          *reinterpret_cast<uint32_t*>(kt + off) = new_codes[0][lane];
+          *reinterpret_cast<uint32_t*>(vt + off) = new_codes[1][lane];
+        }
+        if (lane < NG) {
+          reinterpret_cast<uint32_t*>(sc)[at * NG + lane] = new_scale[0][lane];
+          reinterpret_cast<uint32_t*>(sc + C::kScaleBytes)[at * NG + lane] = new_scale[1][lane];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // before the next load into this stage
+        __syncwarp();
       }
 
       // ---- scores: keys on the rows (g, g + 8 of each 16), query row 4 nt + t on a lane's column pair
@@ -459,8 +494,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
               const float s = __uint_as_float(sm << 16), mid = __uint_as_float(sm & 0xffff0000u);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                const float part = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), s, mid * (float)qs[nt][gr]);
-                x[k][nt][h] = gr ? x[k][nt][h] + part : part;
+                x[k][nt][h] = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), s,
+                                   gr ? fmaf(mid, qsf[nt][gr], x[k][nt][h]) : mid * qsf[nt][gr]);
               }
             }
           }
@@ -477,11 +512,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         const unsigned char* scv = sc + C::kScaleBytes;
         float sv[KT][2][NG], low[KT][2][NG];
         bool seen[KT][NT][2];                               // which of the lane's (key, query row) pairs count
-        float top[NT][NG];                                  // the step's largest s + log2 sv
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) top[nt][gr] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt)
           if (MASKED) {
             const int limit = min(cu.base + min((row0 + 4 * nt + q4) / G, cu.q_len - 1), cu.len - 1);
 #pragma unroll
@@ -489,14 +521,13 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
               for (int h = 0; h < 2; ++h) seen[k][nt][h] = w0 + 16 * k + 8 * h + g <= limit;
           }
-        }
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = 16 * k + 8 * h + g;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
+              const int key = 16 * k + 8 * h + g;
               if (BITS == 8) {
                 sv[k][h][gr] = reinterpret_cast<const float*>(scv)[key];
               } else {
@@ -504,30 +535,51 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
                 sv[k][h][gr] = __uint_as_float(sm << 16);
                 low[k][h][gr] = fmaf(-8.f, sv[k][h][gr], __uint_as_float(sm & 0xffff0000u));
               }
-              // a row of zeros (or of values below 127 x 2^-100) must not move the reference without end
-              const float lg = __log2f(max_nan(sv[k][h][gr], 7.9e-31f));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                if (!MASKED || seen[k][nt][h]) top[nt][gr] = max_nan(top[nt][gr], fmaf(x[k][nt][h], f_r[nt], lg));
             }
-          }
-        bool move = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-#pragma unroll
-            for (int sh = 4; sh <= 16; sh <<= 1) top[nt][gr] = max_nan(top[nt][gr], __shfl_xor_sync(0xffffffffu, top[nt][gr], sh));
-            move |= top[nt][gr] > m_r[nt] + 20.f;           // p stays below 2^(20 + 100)
-          }
-        if (__any_sync(0xffffffffu, move)) {                // the unit's first step, and hardly ever after
+        float p[KT][NT][2], top[NT][NG];                    // probabilities; the step's largest p sv
+        auto exponentials = [&]() {
+          bool far = false;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float m = top[nt][0];
 #pragma unroll
-            for (int gr = 1; gr < NG; ++gr) m = fmaxf(m, top[nt][gr]);
-            if (!(m > m_r[nt])) continue;
-            const float alpha = fast_exp2(m_r[nt] - m);
+            for (int gr = 0; gr < NG; ++gr) top[nt][gr] = 1e-30f;      // below it a step adds nothing that counts
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                p[k][nt][h] = fast_exp2(fmaf(x[k][nt][h], f_r[nt], -m_r[nt]));
+                // a key that the row does not see adds nothing (not 0 x NaN)
+                if (MASKED && !seen[k][nt][h]) { p[k][nt][h] = 0.f; continue; }
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) top[nt][gr] = max_nan(top[nt][gr], p[k][nt][h] * sv[k][h][gr]);
+                far |= p[k][nt][h] > 1e30f;                 // a value's scale may hide how far the score is
+              }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+#pragma unroll
+              for (int sh = 4; sh <= 16; sh <<= 1) top[nt][gr] = max_nan(top[nt][gr], __shfl_xor_sync(0xffffffffu, top[nt][gr], sh));
+              far |= top[nt][gr] > 1048576.f;
+            }
+          }
+          return far;
+        };
+        if (__any_sync(0xffffffffu, exponentials())) {      // the unit's first step, and hardly ever after
+          // the reference moves to the largest s + log2 sv seen so far; a row of zeros (or of values below
+          // 127 x 2^-80) must not move it without end
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float m = m_r[nt];
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (!MASKED || seen[k][nt][h])
+#pragma unroll
+                  for (int gr = 0; gr < NG; ++gr)
+                    m = fmaxf(m, fmaf(x[k][nt][h], f_r[nt], __log2f(fmaxf(sv[k][h][gr], 8.3e-25f))));
+#pragma unroll
+            for (int sh = 4; sh <= 16; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
+            const float alpha = m == m_r[nt] ? 1.f : fast_exp2(m_r[nt] - m);
             m_r[nt] = m;
             l_r[nt] *= alpha;
 #pragma unroll
@@ -535,45 +587,35 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) { o[mt][nt][0] *= alpha; o[mt][nt][1] *= alpha; }
           }
+          exponentials();
         }
-        float up[NT][NG];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float up[NG];
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) {
-            // a step that far below the reference adds nothing that 32 bits hold
-            // (nor does one of which the row sees nothing: top is -inf, and m may be)
-            float d = top[nt][gr] - m_r[nt];
-            d = d < -80.f || top[nt][gr] == -INFINITY ? -80.f : d;
-            beta[nt][gr] = fast_exp2(d) * (1.f / kFixedP);
-            up[nt][gr] = fast_exp2(-d) * kFixedP;
+            beta[nt][gr] = top[nt][gr] * (1.f / kFixedP);
+            up[gr] = __fdividef(kFixedP, top[nt][gr]);
           }
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float p[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              p[h] = fast_exp2(fmaf(x[k][nt][h], f_r[nt], -m_r[nt]));
-              if (MASKED && !seen[k][nt][h]) p[h] = 0.f;
-              l_r[nt] += p[h];
-            }
+          for (int k = 0; k < KT; ++k) {
+            l_r[nt] += p[k][nt][0] + p[k][nt][1];
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               uint32_t y[2];                                // low 16 bits: rint(p sv up), by adding 2^23
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                y[h] = __float_as_uint(fmaf(p[h] * sv[k][h][gr], up[nt][gr], 8388608.f));
-                if (MASKED && !seen[k][nt][h]) y[h] = 0;    // not 0 x NaN of a key nobody sees
+                y[h] = __float_as_uint(fmaf(p[k][nt][h] * sv[k][h][gr], up[gr], 8388608.f));
+                if (MASKED && !seen[k][nt][h]) y[h] = 0;
                 if (BITS == 4) {
-                  const float t = fmaf(p[h], low[k][h][gr], z[nt][gr]);
+                  const float t = fmaf(p[k][nt][h], low[k][h][gr], z[nt][gr]);
                   z[nt][gr] = !MASKED || seen[k][nt][h] ? t : z[nt][gr];
                 }
               }
               pb[k][nt][gr] = transpose_8x8(__byte_perm(y[0], y[1], 0x4051));     // (high g, high g + 8 | low g, low g + 8)
             }
           }
+        }
       };
       // some row does not see some key of the tile
       if (w0 + WK - 1 > min(first_limit, cu.len - 1)) softmax(std::true_type{});
@@ -628,7 +670,23 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       issue_next();
     }
 
-    // ---- the unit's end in this block: lanes, then warps
+    // ---- the unit's end in this block: the next unit's rows asked for; then lanes, then warps
+    const QuantSeq u = cu;                          // (the join below still speaks of this unit)
+    const int u_begin = unit_begin, u_kvh = c_kvh;
+    done += seg;
+    c_t += seg;
+    if (c_t == cu.T && done < n_steps) {
+      unit_begin += cu.T;
+      c_t = 0;
+      if (++c_kvh == P.Hkv) {
+        c_kvh = 0;
+        if (++c_rt == cu.row_tiles) {
+          c_rt = 0;
+          cu = next_seq(cu);
+        }
+      }
+      fetch(cu, c_rt, c_kvh, 0, n_steps - done);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -685,12 +743,12 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     if (!(warp & 1)) add(warp >> 1);
     if (warp == 2) put(1);
     __syncthreads();
-    const long long unit_end = unit_begin + cu.T;
-    const bool whole = unit_begin >= begin && unit_end <= end;
+    const int u_end = u_begin + u.T;
+    const bool whole = u_begin >= begin && u_end <= end;
     auto store = [&](int mt, int nt, float a, float b) {
       const int dim = BITS == 8 ? 16 * mt + 2 * g : 32 * (mt >> 1) + 4 * g + 2 * (mt & 1), row = row0 + 4 * nt + q4;
       if (row < rows)
-        *reinterpret_cast<uint32_t*>(P.out + (size_t)(cu.t0 + row / G) * P.Hq * D + (size_t)(c_kvh * G + row % G) * D + dim) =
+        *reinterpret_cast<uint32_t*>(P.out + (size_t)(u.t0 + row / G) * P.Hq * D + (size_t)(u_kvh * G + row % G) * D + dim) =
             pack_bf16(a, b);
     };
     if (warp == 0) {
@@ -703,7 +761,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
           for (int mt = 0; mt < MT; ++mt) store(mt, nt, o[mt][nt][0] * inv, o[mt][nt][1] * inv);
         }
       } else {
-        float2* seg_out = reinterpret_cast<float2*>(P.scratch + ((size_t)blockIdx.x * 2 + (begin >= unit_begin ? 0 : 1)) * C::kSegFloats) + lane;
+        float2* seg_out = reinterpret_cast<float2*>(P.scratch + ((size_t)blockIdx.x * 2 + (begin >= u_begin ? 0 : 1)) * C::kSegFloats) + lane;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -714,7 +772,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     }
     if (!whole) {
       // blocks whose share meets this unit: first .. last; the one that comes last joins them in order
-      const int first = (int)(((unit_begin + 1) * nb - 1) / total), last = (int)((unit_end * nb - 1) / total);
+      const int first = block_of(u_begin), last = block_of(u_end - 1);
       // counters are indexed by the unit's first block: a block begins at most one cut unit, whose other
       // segments are the first ones of later blocks
       if (warp == 0) {
@@ -730,55 +788,41 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       if (last_s) {
         __threadfence();
         // warp w joins the tiles mt = w, w + 4, ... of all segments, U segments asked for together
-        auto seg_at = [&](int i) {
-          const long long bi = total * i / nb;
-          return reinterpret_cast<const float2*>(P.scratch + ((size_t)i * 2 + (bi >= unit_begin ? 0 : 1)) * C::kSegFloats) + lane;
-        };
+        // (of the unit's blocks all but the first begin inside the unit)
+        const int first_seg = first * 2 + (begin_of(first) >= u_begin ? 0 : 1);
+        const float2* segs = reinterpret_cast<const float2*>(P.scratch) + lane;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float mx = -INFINITY, ls = 0.f;
           float2 acc[MT / 4];
 #pragma unroll
           for (int j = 0; j < MT / 4; ++j) acc[j] = make_float2(0.f, 0.f);
-          constexpr int U = 8;
+          constexpr int U = 16 / (MT / 4);
           for (int i0 = first; i0 <= last; i0 += U) {
             float2 ml[U], a[U][MT / 4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const float2* s = seg_at(min(i0 + u, last));
-              ml[u] = __ldcg(s + (MT * NT + nt) * 32);
+            for (int v = 0; v < U; ++v) {
+              const int i = min(i0 + v, last);
+              const float2* s = segs + (size_t)(i == first ? first_seg : 2 * i) * (C::kSegFloats / 2);
+              ml[v] = __ldcg(s + (MT * NT + nt) * 32);
 #pragma unroll
-              for (int j = 0; j < MT / 4; ++j) a[u][j] = __ldcg(s + ((4 * j + warp) * NT + nt) * 32);
+              for (int j = 0; j < MT / 4; ++j) a[v][j] = __ldcg(s + ((4 * j + warp) * NT + nt) * 32);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              if (i0 + u > last) break;
+            for (int v = 0; v < U; ++v) {
+              if (i0 + v > last) break;
               float fa, fb;
-              factors(mx, ls, ml[u].x, ml[u].y, fa, fb);
+              factors(mx, ls, ml[v].x, ml[v].y, fa, fb);
 #pragma unroll
               for (int j = 0; j < MT / 4; ++j) {
-                acc[j].x = acc[j].x * fa + a[u][j].x * fb;
-                acc[j].y = acc[j].y * fa + a[u][j].y * fb;
+                acc[j].x = acc[j].x * fa + a[v][j].x * fb;
+                acc[j].y = acc[j].y * fa + a[v][j].y * fb;
               }
             }
           }
           const float inv = 1.f / ls;
 #pragma unroll
           for (int j = 0; j < MT / 4; ++j) store(4 * j + warp, nt, acc[j].x * inv, acc[j].y * inv);
-        }
-      }
-    }
-    // ---- on to the next unit
-    done += seg;
-    c_t += seg;
-    if (c_t == cu.T && done < n_steps) {
-      unit_begin += cu.T;
-      c_t = 0;
-      if (++c_kvh == P.Hkv) {
-        c_kvh = 0;
-        if (++c_rt == cu.row_tiles) {
-          c_rt = 0;
-          cu = next_seq(cu);
         }
       }
     }
