@@ -169,41 +169,67 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     s.row_tiles = (s.q_len * G + C::kRows - 1) / C::kRows;
     return s;
   };
-  // ---- this block's share [begin, end) of all block steps, and the sequence it begins in
-  auto steps_of = [&](int b) {
-    const QuantSeq s = load_seq(b);
-    return (long long)s.T * s.row_tiles * P.Hkv;
-  };
-  long long sum = 0;
-  for (int b = lane; b < P.B; b += 32) sum += steps_of(b);
+  // ---- this block's share of all block steps
+  auto total_of = [&](auto weight) {
+    long long sum = 0;
+    for (int b = lane; b < P.B; b += 32) sum += weight(load_seq(b));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+  };
+  long long units = 0;                            // of the lane's sequences, then all
+  const long long sum = total_of([&](const QuantSeq& s) {
+    units += s.T > 0 ? (long long)s.row_tiles * P.Hkv : 0;
+    return (long long)s.T * s.row_tiles * P.Hkv;
+  });
+  units = __reduce_add_sync(0xffffffffu, (unsigned)min(units, 0x7ffffffll));
   if (sum > 0x7fffffff) {
     if (threadIdx.x == 0) atomicOr(P.status, kStatusLengthPastGrid);
     return;
   }
   const int total = (int)sum;
   // at least one step a block: a block without one would be waited for by the join of a unit around it
-  const int nb = min((int)gridDim.x, total);
+  int nb = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= nb) return;
   const int each = total / nb, odd = total % nb;  // the first `odd` blocks take one step more
+  // Where it costs a block at most kCrossing steps more than an even share, no block meets two units: every unit
+  // gets ceil(T / chunk) blocks (a border between two units costs a block about that many steps: a join of its
+  // warps, a partial result, the next query).
+  constexpr int kCrossing = 2;
+  int chunk = each + (odd > 0);
+  bool by_unit = false;
+  for (const int most = chunk + kCrossing; chunk <= most && units <= gridDim.x; ++chunk) {
+    const long long need = total_of([&](const QuantSeq& s) { return (long long)((s.T + chunk - 1) / chunk) * s.row_tiles * P.Hkv; });
+    by_unit = need <= gridDim.x;
+    if (by_unit) {
+      nb = (int)need;
+      break;
+    }
+  }
+  if ((int)blockIdx.x >= nb) return;
+  auto parts_of = [&](const QuantSeq& s) { return by_unit ? (s.T + chunk - 1) / chunk : s.T; };   // blocks, or steps, of a unit
   auto begin_of = [&](int i) { return i * each + min(i, odd); };
   auto block_of = [&](int step) { return step < odd * (each + 1) ? step / (each + 1) : odd + (step - odd * (each + 1)) / each; };
-  const int begin = begin_of(blockIdx.x), end = begin_of(blockIdx.x + 1);
+  const int start = by_unit ? blockIdx.x : begin_of(blockIdx.x);
   QuantSeq cu;                                    // unit that is computed: sequence, row tile, kv head, step
-  int c_rt, c_kvh, c_t;
-  int unit_begin;                                 // first step of the current unit in the whole row
+  int c_rt, c_kvh, c_t, n_steps;
+  int unit_begin, begin, end;                     // the current unit's first step and the block's steps, in one row of all steps
+  int part = 0;                                   // by_unit: the block's place among its unit's blocks
   {
     int before = 0, b0 = 0;
     while (true) {                                // 32 sequences at a time
-      const int mine = b0 + lane < P.B ? (int)steps_of(b0 + lane) : 0;
+      int mine = 0;
+      if (b0 + lane < P.B) {
+        const QuantSeq s = load_seq(b0 + lane);
+        mine = parts_of(s) * s.row_tiles * P.Hkv;
+      }
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, before + incl > begin);
+      const unsigned past = __ballot_sync(0xffffffffu, before + incl > start);
       if (past != 0 || b0 + 32 >= P.B) {
         const int at = past != 0 ? __ffs(past) - 1 : 31;
         before += __shfl_sync(0xffffffffu, incl - mine, at);
@@ -213,13 +239,24 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       before += __shfl_sync(0xffffffffu, incl, 31);
       b0 += 32;
     }
-    const int in_seq = begin - before, unit = in_seq / cu.T;
-    c_t = in_seq % cu.T;
+    const int parts = parts_of(cu), in_seq = start - before, unit = in_seq / parts;
+    part = in_seq % parts;
     c_rt = unit / P.Hkv;
     c_kvh = unit % P.Hkv;
-    unit_begin = begin - c_t;
+    if (by_unit) {                                // the unit's steps shared out evenly over its blocks
+      const int per = cu.T / parts, more = cu.T % parts;
+      unit_begin = 0;
+      begin = part * per + min(part, more);
+      end = begin + per + (part < more);
+      c_t = begin;
+    } else {
+      begin = start;
+      end = begin_of(blockIdx.x + 1);
+      c_t = part;
+      unit_begin = begin - c_t;
+    }
+    n_steps = end - begin;
   }
-  const int n_steps = end - begin;
   auto page_index = [&](int pos) { return P.page_shift >= 0 ? pos >> P.page_shift : pos / P.page_tokens; };
 
   // ---- the unit's query rows (a warp takes rows warp, warp + 4, ...; a lane dims lane + 32 i) and, where the
@@ -738,41 +775,54 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         }
       }
     };
-    if (warp & 1) put(warp >> 1);
-    __syncthreads();
-    if (!(warp & 1)) add(warp >> 1);
-    if (warp == 2) put(1);
-    __syncthreads();
+    auto join_warps = [&]() {                       // warp 0 ends with the block's sums
+      if (warp & 1) put(warp >> 1);
+      __syncthreads();
+      if (!(warp & 1)) add(warp >> 1);
+      if (warp == 2) put(1);
+      __syncthreads();
+      if (warp == 0) add(1);
+    };
+    join_warps();
     const int u_end = u_begin + u.T;
     const bool whole = u_begin >= begin && u_end <= end;
-    auto store = [&](int mt, int nt, float a, float b) {
-      const int dim = BITS == 8 ? 16 * mt + 2 * g : 32 * (mt >> 1) + 4 * g + 2 * (mt & 1), row = row0 + 4 * nt + q4;
-      if (row < rows)
-        *reinterpret_cast<uint32_t*>(P.out + (size_t)(u.t0 + row / G) * P.Hq * D + (size_t)(u_kvh * G + row % G) * D + dim) =
-            pack_bf16(a, b);
+    auto store_all = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float inv = 1.f / l_r[nt];
+        const int row = row0 + 4 * nt + q4;
+        __nv_bfloat16* dst = P.out + (size_t)(u.t0 + row / G) * P.Hq * D + (size_t)(u_kvh * G + row % G) * D + (BITS == 8 ? 2 : 4) * g;
+        if (row < rows)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            *reinterpret_cast<uint32_t*>(dst + (BITS == 8 ? 16 * mt : 32 * (mt >> 1) + 2 * (mt & 1))) =
+                pack_bf16(o[mt][nt][0] * inv, o[mt][nt][1] * inv);
+      }
     };
     if (warp == 0) {
-      add(1);
       if (whole) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float inv = 1.f / l_r[nt];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) store(mt, nt, o[mt][nt][0] * inv, o[mt][nt][1] * inv);
-        }
+        store_all();
       } else {
-        float2* seg_out = reinterpret_cast<float2*>(P.scratch + ((size_t)blockIdx.x * 2 + (begin >= u_begin ? 0 : 1)) * C::kSegFloats) + lane;
+        float4* seg_out = reinterpret_cast<float4*>(P.scratch + ((size_t)blockIdx.x * 2 + (begin >= u_begin ? 0 : 1)) * C::kSegFloats);
+        float r[C::kRegs];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) __stcg(seg_out + (mt * NT + nt) * 32, make_float2(o[mt][nt][0], o[mt][nt][1]));
+          for (int nt = 0; nt < NT; ++nt) {
+            r[(mt * NT + nt) * 2] = o[mt][nt][0];
+            r[(mt * NT + nt) * 2 + 1] = o[mt][nt][1];
+          }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) __stcg(seg_out + (MT * NT + nt) * 32, make_float2(m_r[nt], l_r[nt]));
+        for (int i = 0; i < C::kRegs / 4; ++i) __stcg(seg_out + i * 32 + lane, make_float4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          __stcg(reinterpret_cast<float2*>(seg_out + C::kRegs / 4 * 32) + nt * 32 + lane, make_float2(m_r[nt], l_r[nt]));
       }
     }
     if (!whole) {
       // blocks whose share meets this unit: first .. last; the one that comes last joins them in order
-      const int first = block_of(u_begin), last = block_of(u_end - 1);
+      const int first = by_unit ? blockIdx.x - part : block_of(u_begin);
+      const int last = by_unit ? first + parts_of(u) - 1 : block_of(u_end - 1);
       // counters are indexed by the unit's first block: a block begins at most one cut unit, whose other
       // segments are the first ones of later blocks
       if (warp == 0) {
@@ -787,43 +837,50 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       __syncthreads();
       if (last_s) {
         __threadfence();
-        // warp w joins the tiles mt = w, w + 4, ... of all segments, U segments asked for together
-        // (of the unit's blocks all but the first begin inside the unit)
-        const int first_seg = first * 2 + (begin_of(first) >= u_begin ? 0 : 1);
-        const float2* segs = reinterpret_cast<const float2*>(P.scratch) + lane;
+        // warp w joins segments w, w + 4, ... in order, then the four warps join as above; kAhead segments are
+        // asked for together.  (Of the unit's blocks all but the first begin inside the unit.)
+        const int first_seg = first * 2 + (by_unit || begin_of(first) >= u_begin ? 0 : 1);
+        const float4* segs = reinterpret_cast<const float4*>(P.scratch) + lane;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float mx = -INFINITY, ls = 0.f;
-          float2 acc[MT / 4];
+          m_r[nt] = -INFINITY;
+          l_r[nt] = 0.f;
 #pragma unroll
-          for (int j = 0; j < MT / 4; ++j) acc[j] = make_float2(0.f, 0.f);
-          constexpr int U = 16 / (MT / 4);
-          for (int i0 = first; i0 <= last; i0 += U) {
-            float2 ml[U], a[U][MT / 4];
+          for (int mt = 0; mt < MT; ++mt) o[mt][nt][0] = o[mt][nt][1] = 0.f;
+        }
+        constexpr int kAhead = C::kRegs <= 16 ? 4 : 1;
+        for (int i0 = first + warp; i0 <= last; i0 += 4 * kAhead) {
+          float4 a[kAhead][C::kRegs / 4];
+          float2 ml[kAhead][NT];
 #pragma unroll
-            for (int v = 0; v < U; ++v) {
-              const int i = min(i0 + v, last);
-              const float2* s = segs + (size_t)(i == first ? first_seg : 2 * i) * (C::kSegFloats / 2);
-              ml[v] = __ldcg(s + (MT * NT + nt) * 32);
+          for (int v = 0; v < kAhead; ++v) {
+            const int i = min(i0 + 4 * v, last);
+            const float4* s = segs + (size_t)(i == first ? first_seg : 2 * i) * (C::kSegFloats / 4);
 #pragma unroll
-              for (int j = 0; j < MT / 4; ++j) a[v][j] = __ldcg(s + ((4 * j + warp) * NT + nt) * 32);
-            }
+            for (int r = 0; r < C::kRegs / 4; ++r) a[v][r] = __ldcg(s + r * 32);
 #pragma unroll
-            for (int v = 0; v < U; ++v) {
-              if (i0 + v > last) break;
+            for (int nt = 0; nt < NT; ++nt)
+              ml[v][nt] = __ldcg(reinterpret_cast<const float2*>(s - lane + C::kRegs / 4 * 32) + nt * 32 + lane);
+          }
+#pragma unroll
+          for (int v = 0; v < kAhead; ++v) {
+            if (i0 + 4 * v > last) break;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
               float fa, fb;
-              factors(mx, ls, ml[v].x, ml[v].y, fa, fb);
+              factors(m_r[nt], l_r[nt], ml[v][nt].x, ml[v][nt].y, fa, fb);
 #pragma unroll
-              for (int j = 0; j < MT / 4; ++j) {
-                acc[j].x = acc[j].x * fa + a[v][j].x * fb;
-                acc[j].y = acc[j].y * fa + a[v][j].y * fb;
+              for (int mt = 0; mt < MT; ++mt) {
+                const int r = (mt * NT + nt) * 2;
+                const float4 w = a[v][r / 4];
+                o[mt][nt][0] = o[mt][nt][0] * fa + (r & 2 ? w.z : w.x) * fb;
+                o[mt][nt][1] = o[mt][nt][1] * fa + (r & 2 ? w.w : w.y) * fb;
               }
             }
           }
-          const float inv = 1.f / ls;
-#pragma unroll
-          for (int j = 0; j < MT / 4; ++j) store(4 * j + warp, nt, acc[j].x * inv, acc[j].y * inv);
         }
+        join_warps();
+        if (warp == 0) store_all();
       }
     }
   }
