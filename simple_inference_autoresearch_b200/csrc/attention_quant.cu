@@ -60,14 +60,14 @@ struct QuantAttnParams {
 template <int BITS, int D, int NT>
 struct QuantAttn {
   static constexpr int kRowBytes = D * BITS / 8;
-  static constexpr int kWarpKeys = D == 128 ? 32 : 64;               // keys per warp and step
+  static constexpr int kWarpKeys = D == 128 && (BITS == 8 || NT == 4) ? 32 : 64;     // keys per warp and step
   static constexpr int kBlockKeys = 4 * kWarpKeys;
   static constexpr int kTileBytes = kWarpKeys * kRowBytes;
   static constexpr int kGroups = BITS == 8 ? 1 : D / kQuantGroup;
   static constexpr int kScaleBytes = kWarpKeys * 4 * kGroups;        // float32, or (scale, mid) bfloat16 per run
   // blocks an SM and pipeline depth: what shared memory (and, for many rows, registers) leave room for
-  static constexpr int kBlocksPerSM = NT == 1 ? 3 : 2;
-  static constexpr int kStages = kTileBytes < 4096 ? (NT == 1 ? 3 : NT == 2 ? 5 : 4) : NT == 2 ? 3 : 2;
+  static constexpr int kBlocksPerSM = NT == 1 && D == 64 ? 3 : 2;
+  static constexpr int kStages = kTileBytes < 4096 && NT > 1 ? 4 : 2;
   static constexpr int kRows = 4 * NT;                               // query rows of a unit
   static constexpr int kMT = D / 16;                                 // row tiles of the value product
   static constexpr int kQStride = D + 16;                            // bytes per column of query bytes in shared memory
@@ -83,18 +83,27 @@ struct QuantAttn {
   static_assert(kBlocksPerSM * (kSmem + 1024 + 1024 + (NT == 1 ? 1500 : NT == 2 ? 2100 : 3300)) <= 228 * 1024, "blocks an SM");
 };
 constexpr float kFixedP = 65500.f;                // p sv of a step's largest term, as a whole number
+// A query row's largest element as a whole number.  8 bits: 127 x 256.  4 bits: 2032; the even dims' numbers are
+// taken 16 times, because their codes are read from the low halves of the cache's bytes and the odd dims' from
+// the high halves, where they stand for 16 times as much: both sums are 16 times q . code, with no shift.
+template <int BITS> constexpr float kFixedQ = BITS == 8 ? 32512.f : 2032.f;
 
-// D (int32) = C + A B for bytes; ASIGN / BSIGN: signed operands.
-template <bool ASIGN, bool BSIGN>
+// D (int32) = C + A B for bytes; ASIGN / BSIGN: signed operands, FIRST: C is zero.
+template <bool ASIGN, bool BSIGN, bool FIRST>
 __device__ __forceinline__ void mma_bytes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-#define SIAR_MMA(AT, BT)                                                                                              \
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." AT "." BT ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                        \
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
-  if (ASIGN && BSIGN) SIAR_MMA("s8", "s8");
-  else if (ASIGN) SIAR_MMA("s8", "u8");
-  else if (BSIGN) SIAR_MMA("u8", "s8");
-  else SIAR_MMA("u8", "u8");
+#define SIAR_MMA(AT, BT)                                                                                                    \
+  if (FIRST)                                                                                                                \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." AT "." BT ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                            \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));                                            \
+  else                                                                                                                      \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." AT "." BT ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"     \
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                            \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if (ASIGN && BSIGN) { SIAR_MMA("s8", "s8"); }
+  else if (ASIGN) { SIAR_MMA("s8", "u8"); }
+  else if (BSIGN) { SIAR_MMA("u8", "s8"); }
+  else { SIAR_MMA("u8", "u8"); }
 #undef SIAR_MMA
 }
 // The larger of two, NaN if either is.
@@ -346,6 +355,12 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   float qsf[NT][NG];
   uint32_t qb[D / 32][NT][2];
   bool expired = false;
+  // where the lane's row of an ldmatrix stands: (keys 0-7 | 8-15) x (chunk 2c, 2c + 1) of a tile's first 16 keys; 16
+  // keys on is 16 rows on, whole periods of the swizzle
+  uint32_t at16[RB / 32];
+#pragma unroll
+  for (int c = 0; c < RB / 32; ++c)
+    at16[c] = swizzled<RB>(((lane & 7) + ((lane >> 3) & 1) * 8) * RB + (2 * c + (lane >> 4)) * 16);
   int cs_b = -1;
 
   for (int done = 0; done < n_steps;) {
@@ -409,26 +424,27 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
       for (int sh = 16; sh > 0; sh >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
       const bool fine = isfinite(amax) && amax > 1e-30f;       // else zeros; NaN through the factor where not finite
-      const float up = fine ? 32512.f / amax : 0.f;
+      const float up = fine ? kFixedQ<BITS> / amax : 0.f;
       int sum[NG];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) sum[gr] = 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        const int v = fine ? __float2int_rn(a[i] * up) : 0;
+        int v = fine ? __float2int_rn(a[i] * up) : 0;
+        sum[BITS == 8 ? 0 : 32 * i / kQuantGroup] += v;
+        if (BITS == 4 && !(lane & 1)) v *= 16;
         const int hi = (v + 128) >> 8;             // v = 256 hi + lo, lo in -128 .. 127
         // 4 bits: a word holds eight dims, the even ones in its low halves, the odd ones in its high halves
         const int d = 32 * i + lane, at = BITS == 8 ? d : (d & ~7) + ((d & 1) << 2) + ((d & 7) >> 1);
         q_s[(2 * r) * C::kQStride + at] = (signed char)hi;
         q_s[(2 * r + 1) * C::kQStride + at] = (signed char)(v - (hi << 8));
-        sum[BITS == 8 ? 0 : 32 * i / kQuantGroup] += v;
       }
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         sum[gr] = __reduce_add_sync(0xffffffffu, sum[gr]);
         if (lane == 0) qsum_s[r][gr] = sum[gr];
       }
-      if (lane == 0) f_s[r] = fine ? P.sl2 * (amax / 32512.f) : amax - amax;
+      if (lane == 0) f_s[r] = fine ? P.sl2 * (amax / (kFixedQ<BITS> * (BITS == 8 ? 1.f : 16.f))) : amax - amax;
     }
     __syncthreads();
 #pragma unroll
@@ -450,7 +466,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       l_r[nt] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        qs[nt][gr] = qsum_s[4 * nt + q4][gr];
+        qs[nt][gr] = 16 * qsum_s[4 * nt + q4][gr];      // (4 bits only)
         qsf[nt][gr] = (float)qs[nt][gr];
         z[nt][gr] = 0.f;
       }
@@ -486,49 +502,60 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 
       // ---- scores: keys on the rows (g, g + 8 of each 16), query row 4 nt + t on a lane's column pair
       const uint32_t k_addr = smem_u32(kt), v_addr = smem_u32(vt);
-      const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lch = lane >> 4;     // ldmatrix: (keys 0-7 | 8-15) x (chunk, next)
+      auto load_scales = [](uint32_t (&w)[NG], const unsigned char* from, int key) {
+        if (NG == 2) {
+          const uint2 v = reinterpret_cast<const uint2*>(from)[key];
+          w[0] = v.x;
+          w[NG - 1] = v.y;
+        } else {
+          w[0] = reinterpret_cast<const uint32_t*>(from)[key];
+        }
+      };
       float x[KT][NT][2];
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-        const float* sk8 = reinterpret_cast<const float*>(sc) + 16 * k + g;
-        const uint32_t* sk4 = reinterpret_cast<const uint32_t*>(sc) + (16 * k + g) * NG;
+        // the two keys' scales
+        uint32_t ksc[2][NG];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_scales(ksc[h], sc, 16 * k + 8 * h + g);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           int acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = acc[nt][2] = 0;
-            acc[nt][1] = acc[nt][3] = BITS == 8 ? 0 : -8 * qs[nt][gr];
-          }
           if (BITS == 8) {
 #pragma unroll
-            for (int c = 0; c < D / 16; c += 2) {
+            for (int c = 0; c < D / 32; ++c) {
               uint32_t w[4];
-              ldmatrix_x4(w, k_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
+              ldmatrix_x4(w, k_addr + at16[c] + k * 16 * RB);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma_bytes<true, true>(acc[nt], w[0], w[1], w[2], w[3], qb[c / 2][nt][0], qb[c / 2][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) {
+                if (c == 0) mma_bytes<true, true, true>(acc[nt], w[0], w[1], w[2], w[3], qb[c][nt][0], qb[c][nt][1]);
+                else mma_bytes<true, true, false>(acc[nt], w[0], w[1], w[2], w[3], qb[c][nt][0], qb[c][nt][1]);
+              }
             }
           } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              acc[nt][0] = acc[nt][2] = 0;
+              acc[nt][1] = acc[nt][3] = -8 * qs[nt][gr];
+            }
             uint32_t w[4];                         // 64 dims: chunks 2 gr and 2 gr + 1
-            ldmatrix_x4(w, k_addr + swizzled<RB>((16 * k + lrow) * RB + (2 * gr + lch) * 16));
-            constexpr uint32_t M = 0x0f0f0f0fu;
+            ldmatrix_x4(w, k_addr + at16[gr] + k * 16 * RB);
+            constexpr uint32_t LO = 0x0f0f0f0fu, HI = 0xf0f0f0f0u;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma_bytes<false, true>(acc[nt], w[2 * h] & M, w[2 * h + 1] & M, (w[2 * h] >> 4) & M, (w[2 * h + 1] >> 4) & M,
-                                       qb[2 * gr + h][nt][0], qb[2 * gr + h][nt][1]);
+                mma_bytes<false, true, false>(acc[nt], w[2 * h] & LO, w[2 * h + 1] & LO, w[2 * h] & HI, w[2 * h + 1] & HI,
+                                              qb[2 * gr + h][nt][0], qb[2 * gr + h][nt][1]);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (BITS == 8) {
-              const float s = sk8[8 * h];
+              const float s = __uint_as_float(ksc[h][0]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) x[k][nt][h] = (float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]) * s;
             } else {
-              const uint32_t sm = sk4[8 * h * NG + gr];
-              const float s = __uint_as_float(sm << 16), mid = __uint_as_float(sm & 0xffff0000u);
+              const float s = __uint_as_float(ksc[h][gr] << 16), mid = __uint_as_float(ksc[h][gr] & 0xffff0000u);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 x[k][nt][h] = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), s,
@@ -561,18 +588,19 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[NG];
+            load_scales(w, scv, 16 * k + 8 * h + g);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-              const int key = 16 * k + 8 * h + g;
               if (BITS == 8) {
-                sv[k][h][gr] = reinterpret_cast<const float*>(scv)[key];
+                sv[k][h][gr] = __uint_as_float(w[gr]);
               } else {
-                const uint32_t sm = reinterpret_cast<const uint32_t*>(scv)[key * NG + gr];
-                sv[k][h][gr] = __uint_as_float(sm << 16);
-                low[k][h][gr] = fmaf(-8.f, sv[k][h][gr], __uint_as_float(sm & 0xffff0000u));
+                sv[k][h][gr] = __uint_as_float(w[gr] << 16);
+                low[k][h][gr] = fmaf(-8.f, sv[k][h][gr], __uint_as_float(w[gr] & 0xffff0000u));
               }
             }
+          }
         float p[KT][NT][2], top[NT][NG];                    // probabilities; the step's largest p sv
         auto exponentials = [&]() {
           bool far = false;
@@ -661,12 +689,12 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       // 8 bits: rows g and g + 8 of tile mt hold dims 16 mt + 2g and one more; 4 bits: of tile 2c + i dims
       // 32c + 4g + 2i and one more
 #pragma unroll
-      for (int c = 0; c < RB / 16; c += 2) {
-        uint32_t even[KT][2], odd[KT][2];                   // bytes 2g and 2g + 1 of chunks c, c + 1
+      for (int c = 0; c < RB / 32; ++c) {
+        uint32_t even[KT][2], odd[KT][2];                   // bytes 2g and 2g + 1 of chunks 2c, 2c + 1
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
           uint32_t w[4];
-          ldmatrix_x4_trans(w, v_addr + swizzled<RB>((16 * k + lrow) * RB + (c + lch) * 16));
+          ldmatrix_x4_trans(w, v_addr + at16[c] + k * 16 * RB);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             even[k][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x6240);
@@ -677,29 +705,30 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int part = 0; part < 8 / BITS; ++part) {
-            const int mt = BITS == 8 ? c + i : 2 * (c + i) + part, gr = BITS == 8 ? 0 : mt * 16 / kQuantGroup;
+            const int mt = BITS == 8 ? 2 * c + i : 2 * (2 * c + i) + part, gr = BITS == 8 ? 0 : mt * 16 / kQuantGroup;
             int acc[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
-#pragma unroll
             for (int k = 0; k < KT; k += 2) {
-              constexpr uint32_t M = 0x0f0f0f0fu;
+              constexpr uint32_t LO = 0x0f0f0f0fu, HI = 0xf0f0f0f0u;
               uint32_t a[4];
               if (BITS == 8) {
                 a[0] = even[k][i]; a[1] = odd[k][i]; a[2] = even[k + 1][i]; a[3] = odd[k + 1][i];
-              } else {
+              } else {                                      // (the high halves as they stand: 16 times the code)
                 const uint32_t u = part ? odd[k][i] : even[k][i], v = part ? odd[k + 1][i] : even[k + 1][i];
-                a[0] = u & M; a[1] = (u >> 4) & M; a[2] = v & M; a[3] = (v >> 4) & M;
+                a[0] = u & LO; a[1] = u & HI; a[2] = v & LO; a[3] = v & HI;
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma_bytes<BITS == 8, false>(acc[nt], a[0], a[1], a[2], a[3], pb[k][nt][gr], pb[k + 1][nt][gr]);
+              for (int nt = 0; nt < NT; ++nt) {
+                if (k == 0) mma_bytes<BITS == 8, false, true>(acc[nt], a[0], a[1], a[2], a[3], pb[k][nt][gr], pb[k + 1][nt][gr]);
+                else mma_bytes<BITS == 8, false, false>(acc[nt], a[0], a[1], a[2], a[3], pb[k][nt][gr], pb[k + 1][nt][gr]);
+              }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                o[mt][nt][h] = fmaf((float)(acc[nt][2 * h] * 256 + acc[nt][2 * h + 1]), beta[nt][gr], o[mt][nt][h]);
+            for (int nt = 0; nt < NT; ++nt) {
+              o[mt][nt][0] = fmaf((float)(acc[nt][0] * 256 + acc[nt][1]), beta[nt][gr], o[mt][nt][0]);
+              o[mt][nt][1] = fmaf((float)(acc[nt][2] * 256 + acc[nt][3]), BITS == 8 ? beta[nt][gr] : beta[nt][gr] * 0.0625f,
+                                  o[mt][nt][1]);
+            }
           }
       }
       ++consumed;
@@ -944,7 +973,7 @@ extern "C" int siar_attn_quant_supported(int Hq, int Hkv, int D, int page_tokens
 // Blocks of a launch (the counters it needs); more never help: a block step is the least share.
 extern "C" int siar_attn_quant_blocks(int bits, int B, int Hq, int Hkv, int D, int max_q_len, int max_kv_len, int sm_count) {
   const int rows = max_q_len * (Hq / Hkv), nt = column_tiles_of(rows);
-  const int keys = D == 128 ? QuantAttn<8, 128, 1>::kBlockKeys : QuantAttn<8, 64, 1>::kBlockKeys;
+  const int keys = D == 128 && (bits == 8 || nt == 4) ? 128 : 256;
   const long long steps = (long long)B * Hkv * ((rows + 4 * nt - 1) / (4 * nt)) * ((max_kv_len + keys - 1) / keys);
   const long long most = (long long)sm_count * (bits == 8 ? D == 128 ? blocks_per_sm<8, 128>(nt) : blocks_per_sm<8, 64>(nt)
                                                           : D == 128 ? blocks_per_sm<4, 128>(nt) : blocks_per_sm<4, 64>(nt));
