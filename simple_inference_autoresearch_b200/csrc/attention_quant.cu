@@ -179,24 +179,19 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     return s;
   };
   // ---- this block's share of all block steps
+  // Sums over all sequences, 32 a time; a sum beyond 2^31 is refused below, so a lane's part may stop at 2^26.
   auto total_of = [&](auto weight) {
-    long long sum = 0;
-    for (int b = lane; b < P.B; b += 32) sum += weight(load_seq(b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+    long long mine = 0;
+    for (int b = lane; b < P.B; b += 32) mine += weight(load_seq(b));
+    return __reduce_add_sync(0xffffffffu, (unsigned)min(mine, 1ll << 26));
   };
-  long long units = 0;                            // of the lane's sequences, then all
-  const long long sum = total_of([&](const QuantSeq& s) {
-    units += s.T > 0 ? (long long)s.row_tiles * P.Hkv : 0;
-    return (long long)s.T * s.row_tiles * P.Hkv;
-  });
-  units = __reduce_add_sync(0xffffffffu, (unsigned)min(units, 0x7ffffffll));
-  if (sum > 0x7fffffff) {
+  const unsigned sum = total_of([&](const QuantSeq& s) { return (long long)s.T * s.row_tiles * P.Hkv; });
+  if (sum >= 1u << 26) {
     if (threadIdx.x == 0) atomicOr(P.status, kStatusLengthPastGrid);
     return;
   }
   const int total = (int)sum;
+  const unsigned units = total_of([&](const QuantSeq& s) { return s.T > 0 ? (long long)s.row_tiles * P.Hkv : 0ll; });
   // at least one step a block: a block without one would be waited for by the join of a unit around it
   int nb = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= nb) return;
@@ -208,7 +203,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   int chunk = each + (odd > 0);
   bool by_unit = false;
   for (const int most = chunk + kCrossing; chunk <= most && units <= gridDim.x; ++chunk) {
-    const long long need = total_of([&](const QuantSeq& s) { return (long long)((s.T + chunk - 1) / chunk) * s.row_tiles * P.Hkv; });
+    const unsigned need = total_of([&](const QuantSeq& s) { return (long long)((s.T + chunk - 1) / chunk) * s.row_tiles * P.Hkv; });
     by_unit = need <= gridDim.x;
     if (by_unit) {
       nb = (int)need;
@@ -293,7 +288,6 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       t_page = P.block_table[(size_t)s.slot * P.max_pages + page_index(s.base)];
     }
   };
-  fetch(cu, c_rt, c_kvh, c_t, n_steps);
 
   // ---- this warp's loads: the same walk, ahead of the computation
   QuantSeq lu = cu;
@@ -306,17 +300,22 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     while (n.T * n.row_tiles == 0) n = load_seq(++b);
     return n;
   };
-  auto page_of = [&]() {                          // page of the load cursor's tile; asked for a step before its use
-    const int w0 = l_t * C::kBlockKeys + warp * WK;
-    return l_left > 0 && w0 < lu.len ? P.block_table[(size_t)lu.slot * P.max_pages + page_index(w0)] : 0;
+  // Lane i holds the page of the warp's tile i steps on from l_page0 in the load cursor's unit; asked for ahead
+  // of its use, 32 steps at a time.
+  int l_page0 = 0, l_pages = 0;
+  auto ask_pages = [&]() {
+    const int w0 = (l_t + lane) * C::kBlockKeys + warp * WK;
+    l_page0 = l_t;
+    l_pages = l_left > 0 && w0 < lu.len ? P.block_table[(size_t)lu.slot * P.max_pages + page_index(w0)] : 0;
   };
-  int page_ahead = page_of();
+  ask_pages();
+  fetch(cu, c_rt, c_kvh, c_t, n_steps);
   auto issue_next = [&]() {
     while (l_left > 0) {
       const int w0 = l_t * C::kBlockKeys + warp * WK;
       const bool has = w0 < lu.len;
       if (has) {
-        int page = page_ahead;
+        int page = __shfl_sync(0xffffffffu, l_pages, l_t - l_page0);
         if (page < 0 || page >= P.n_pages) { absent_page = true; page = 0; }
         if (lane == 0) {
           const int s = issued % C::kStages;
@@ -342,8 +341,10 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
             if (l_left > 0) lu = next_seq(lu);
           }
         }
+        ask_pages();
+      } else if (l_t == l_page0 + 32) {
+        ask_pages();
       }
-      page_ahead = page_of();
       if (has) return;
     }
   };
