@@ -965,15 +965,9 @@ using namespace siar;
 
 SIAR_DEFINE_PDL_SWITCH()
 
-// 1 when the kernel takes these sizes (bfloat16 activations).
-extern "C" int siar_attn_quant_supported(int Hq, int Hkv, int D, int page_tokens, long long n_pages) {
-  if (Hkv <= 0 || Hq % Hkv != 0 || page_tokens <= 0) return 0;
-  return (D == 64 || D == 128) && page_tokens % 64 == 0 && n_pages * Hkv * page_tokens < (1ll << 31);
-}
-
-// Blocks of a launch (the counters it needs); more never help: a block step is the least share.
-extern "C" int siar_attn_quant_blocks(int bits, int B, int Hq, int Hkv, int D, int max_q_len, int max_kv_len, int sm_count) {
-  const int rows = max_q_len * (Hq / Hkv), nt = column_tiles_of(rows);
+// Blocks of a launch: a block step is the least share.
+static int blocks_of(int bits, int B, int Hkv, int D, int rows, int max_kv_len, int sm_count) {
+  const int nt = column_tiles_of(rows);
   const int keys = D == 128 && (bits == 8 || nt == 4) ? 128 : 256;
   const long long steps = (long long)B * Hkv * ((rows + 4 * nt - 1) / (4 * nt)) * ((max_kv_len + keys - 1) / keys);
   const long long most = (long long)sm_count * (bits == 8 ? D == 128 ? blocks_per_sm<8, 128>(nt) : blocks_per_sm<8, 64>(nt)
@@ -981,10 +975,12 @@ extern "C" int siar_attn_quant_blocks(int bits, int B, int Hq, int Hkv, int D, i
   return (int)(steps < most ? (steps > 0 ? steps : 1) : most);
 }
 
-// Scratch floats for that many blocks.
-extern "C" long long siar_attn_quant_scratch_floats(int Hq, int Hkv, int D, int max_q_len, int blocks) {
-  const int nt = column_tiles_of(max_q_len * (Hq / Hkv));
-  return (long long)blocks * 2 * ((D / 16) * nt * 2 + 2 * nt) * 32;
+// What every launch on a GPU of so many SMs finds room in: counters (int32), and floats of scratch behind them.
+extern "C" long long siar_attn_quant_counters(int sm_count) { return 3ll * sm_count; }
+extern "C" long long siar_attn_quant_scratch_floats(int sm_count) {
+  constexpr long long narrow = 3 * QuantAttn<8, 64, 1>::kSegFloats, wide = 2 * QuantAttn<8, 128, 4>::kSegFloats;
+  static_assert(QuantAttn<8, 64, 1>::kBlocksPerSM == 3 && QuantAttn<8, 128, 4>::kBlocksPerSM == 2, "the most of either");
+  return 2ll * sm_count * (narrow > wide ? narrow : wide);
 }
 
 // What tells one capture of a stream from another (0: the stream is not being captured).
@@ -998,20 +994,23 @@ extern "C" unsigned long long siar_capture_id(void* stream) {
 // Attention of the batch's new tokens over the quantised cache.  fused: one new token a sequence, whose
 // query and key are rotated here (inv_freq; nullptr: not rotated) and whose key and value are stored
 // (write_kv) and attended to; else the tokens' rows are in the cache and the queries are as they are to be
-// used.  counters: `blocks` zeros, left zero.
+// used.  counters: siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
 extern "C" int siar_attn_quant(int bits, const void* qkv, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
                                const int* block_table, const int* slot_ids, const int* q_start, const int* base_len,
-                               const float* inv_freq, void* out, float* scratch, int* counters, int blocks, int B, int Hq,
-                               int Hkv, int D, int page_tokens, int max_pages, int n_pages, int max_q_len, int fused,
-                               int write_kv, float scale, int* status, void* stream) {
+                               const float* inv_freq, void* out, int* counters, float* scratch, int B, int Hq, int Hkv, int D,
+                               int page_tokens, int max_pages, int n_pages, int max_q_len, int max_kv_len, int sm_count,
+                               int fused, int write_kv, float scale, int* status, void* stream) {
   if (B == 0 || max_q_len == 0) return 0;
-  if (!siar_attn_quant_supported(Hq, Hkv, D, page_tokens, n_pages) || (bits != 8 && bits != 4) || blocks <= 0 ||
-      n_pages <= 0 || max_pages <= 0 || (long long)max_pages * page_tokens >= (1ll << 31) || (fused && max_q_len != 1))
+  if (Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || page_tokens <= 0 || page_tokens % 64 != 0 || (bits != 8 && bits != 4) ||
+      n_pages <= 0 || max_pages <= 0 || max_kv_len <= 0 || sm_count <= 0 || (fused && max_q_len != 1) ||
+      (long long)n_pages * Hkv * page_tokens >= (1ll << 31) || (long long)max_pages * page_tokens >= (1ll << 31))
     return (int)cudaErrorInvalidValue;
   QuantAttnParams p = {(const __nv_bfloat16*)qkv, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
                        q_start, base_len, inv_freq, (__nv_bfloat16*)out, scratch, counters, status, B, Hq, Hkv, page_tokens,
-                       max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused, write_kv, scale * 1.4426950408889634f};
+                       max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused,
+                       write_kv, scale * 1.4426950408889634f};
   cudaStream_t s = (cudaStream_t)stream;
+  const int blocks = blocks_of(bits, B, Hkv, D, max_q_len * (Hq / Hkv), max_kv_len, sm_count);
   const int nt = column_tiles_of(max_q_len * (Hq / Hkv));
 #define SIAR_GO(BITS, DIM)                                                                     \
   return nt == 1 ? launch_quant<BITS, DIM, 1>(p, blocks, s) : nt == 2 ? launch_quant<BITS, DIM, 2>(p, blocks, s) \

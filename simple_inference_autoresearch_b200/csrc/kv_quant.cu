@@ -109,6 +109,159 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
   }
 }
 
+// The same for bfloat16, head_dim 64 or 128 and whole-head rotation in pairs (i, i + D/2), 8 bytes an access: D/8
+// lanes share a head, a lane holds dims 4j .. 4j + 3 and D/2 + 4j .. + 3, so the pairs of a rotation are its own
+// and a row's statistics take a few shuffles.  A block of 256 threads takes a token's heads kPasses x 256 / (D/8)
+// at a time, all of their loads asked for before the rotation angles are formed.
+template <int D, int BITS>
+__global__ void __launch_bounds__(256)
+rope_quantize_wide_kernel(const __nv_bfloat16* qkv, __nv_bfloat16* q_out, const float* __restrict__ inv_freq,
+                          uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, void* __restrict__ k_scale,
+                          void* __restrict__ v_scale, const int* block_table, const int* slot_ids, const int* q_start,
+                          const int* base_len, int B, int Hq, int Hkv, int page_tokens, int max_pages, int n_pages,
+                          int write_kv, int* __restrict__ status) {
+  constexpr int LANES = D / 8, HEADS = 256 / LANES, kPasses = 3, NG = D / kQuantGroup;
+  pdl_launch_dependents();
+  __shared__ float cos_s[D / 2], sin_s[D / 2];
+  float freq = 0.f;
+  if (inv_freq != nullptr && threadIdx.x < D / 2) freq = inv_freq[threadIdx.x];
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int j = threadIdx.x % LANES, h0 = threadIdx.x / LANES;
+  const int heads = Hq + 2 * Hkv, stride = gridDim.y * HEADS;
+  const __nv_bfloat16* row = qkv + (size_t)t * heads * D + 4 * j;
+  uint2 lo[kPasses], hi[kPasses];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int head = first + p * stride;
+      if (head < heads) {
+        lo[p] = *reinterpret_cast<const uint2*>(row + (size_t)head * D);
+        hi[p] = *reinterpret_cast<const uint2*>(row + (size_t)head * D + D / 2);
+      }
+    }
+  };
+  int first = blockIdx.y * HEADS + h0;
+  load(first);
+  const int b = sequence_of(q_start, B, t);
+  const int pos = base_len[b] + (t - q_start[b]);
+  if (inv_freq != nullptr && threadIdx.x < D / 2) rotation(pos, freq, &cos_s[threadIdx.x], &sin_s[threadIdx.x]);
+  int page = -1;
+  if (write_kv) {
+    page = pos / page_tokens < max_pages ? block_table[(size_t)slot_ids[b] * max_pages + pos / page_tokens] : -1;
+    if (page < 0 || page >= n_pages) {
+      page = -1;
+      if (threadIdx.x == 0) atomicOr(status, kStatusBadPage);
+    }
+  }
+  __syncthreads();
+  const size_t row0 = (size_t)max(page, 0) * Hkv * page_tokens + pos % page_tokens;      // kv head 0
+  float cv[4], sv[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    cv[e] = inv_freq != nullptr ? cos_s[4 * j + e] : 1.f;
+    sv[e] = inv_freq != nullptr ? sin_s[4 * j + e] : 0.f;
+  }
+  // of the lanes that share a head
+  auto group_max = [](float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  // every thread runs every round: the shuffles take whole warps
+  for (int base = blockIdx.y * HEADS; base < heads; base += kPasses * stride) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int head = base + h0 + p * stride;
+      if (base + p * stride >= heads) break;
+      const bool in = head < heads;
+      float x[8];
+      const uint2 l = in ? lo[p] : make_uint2(0u, 0u), u = in ? hi[p] : make_uint2(0u, 0u);
+      const uint32_t w[4] = {l.x, l.y, u.x, u.y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(w[e] << 16);
+        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+      if (inv_freq != nullptr && head < Hq + Hkv) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = x[e], c = x[4 + e];
+          x[e] = rotate_lo(a, c, cv[e], sv[e]);
+          x[4 + e] = rotate_hi(a, c, cv[e], sv[e]);
+        }
+      }
+      if (in && head < Hq) {
+        __nv_bfloat16* dst = q_out + (size_t)t * heads * D + (size_t)head * D + 4 * j;
+        uint2 o[2];
+        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o2[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint2*>(dst) = o[0];
+        *reinterpret_cast<uint2*>(dst + D / 2) = o[1];
+      }
+      // (lanes of query heads in a warp with key heads go along for the shuffles)
+      const bool is_k = head < Hq + Hkv, stores = in && head >= Hq && page >= 0;
+      if (!__any_sync(0xffffffffu, stores)) continue;
+      const int kvh = is_k ? head - Hq : head - Hq - Hkv;
+      const size_t at = row0 + (size_t)max(kvh, 0) * page_tokens;
+      uint8_t* codes = (is_k ? k_pool : v_pool) + at * (D * BITS / 8);
+      float top[NG], bot[NG];                       // per run (8 bits: per row, of |x|)
+      bool bad[NG];
+      if (BITS == 8 || NG == 1) {
+        float m = 0.f, n = INFINITY, a = -INFINITY;
+        bool wrong = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          m = fmaxf(m, fabsf(x[e]));
+          n = fminf(n, x[e]);
+          a = fmaxf(a, x[e]);
+          wrong |= !isfinite(x[e]);
+        }
+        top[0] = group_max(BITS == 8 ? m : a);
+        bot[0] = BITS == 8 ? 0.f : -group_max(-n);
+        bad[0] = group_max(wrong ? 1.f : 0.f) > 0.f;
+      } else {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float* y = x + 4 * g;
+          const bool wrong = !isfinite(y[0]) || !isfinite(y[1]) || !isfinite(y[2]) || !isfinite(y[3]);
+          top[g] = group_max(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+          bot[g] = -group_max(-fminf(fminf(y[0], y[1]), fminf(y[2], y[3])));
+          bad[g] = group_max(wrong ? 1.f : 0.f) > 0.f;
+        }
+      }
+      if (!stores) continue;
+      if (BITS == 8) {
+        const float s = scale8(top[0]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t c = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c |= (uint32_t)(code8(x[4 * h + e], s, bad[0]) & 0xff) << (8 * e);
+          *reinterpret_cast<uint32_t*>(codes + h * (D / 2) + 4 * j) = c;
+        }
+        if (j == 0) reinterpret_cast<float*>(is_k ? k_scale : v_scale)[at] = bad[0] ? __int_as_float(0x7fc00000) : s;
+      } else {
+        __nv_bfloat162* sc = reinterpret_cast<__nv_bfloat162*>(is_k ? k_scale : v_scale) + at * NG;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int g = NG == 1 ? 0 : h;
+          const __nv_bfloat162 sm = scale4(bot[g], top[g], bad[g]);
+          const float s = __low2float(sm), m = __high2float(sm);
+          uint32_t c = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c |= (uint32_t)code4(x[4 * h + e], s, m) << (4 * e);
+          *reinterpret_cast<uint16_t*>(codes + h * (D / 4) + 2 * j) = (uint16_t)c;
+          if (j == 0 && (NG == 2 || h == 0)) sc[g] = sm;
+        }
+      }
+    }
+    first += kPasses * stride;
+    load(first);
+  }
+}
+
 // ------------------------------------------------------------------ read back
 // Sequence b's pages go, in order, behind those of the sequences before it: page p of sequence b is
 // page first(b) + p of the output pools [pages][Hkv][page_tokens][D]; row b of `out_table` names them
@@ -215,6 +368,19 @@ extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* 
   if ((bits != 8 && bits != 4) || D % 16 != 0 || D <= 0 || D > 256 || rotary_dim < 0 || rotary_dim > D ||
       rotary_dim % 2 != 0 || page_tokens <= 0)
     return (int)cudaErrorInvalidValue;
+  if (is_bf16 && (D == 64 || D == 128) && (inv_freq == nullptr || (rotary_dim == D && !interleaved)) &&
+      (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0) {
+    const int per_block = 256 / (D / 8);            // few tokens: the heads of one token go to several blocks
+    const int most = (Hq + 2 * Hkv + per_block - 1) / per_block, split = N >= 296 ? 1 : min(most, (296 + N - 1) / N);
+    auto wide = [&](auto kernel) {
+      return (int)launch_kernel(kernel, dim3(N, split), dim3(256), 0, (cudaStream_t)stream, (const __nv_bfloat16*)qkv,
+                                (__nv_bfloat16*)q_out, inv_freq, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale,
+                                block_table, slot_ids, q_start, base_len, B, Hq, Hkv, page_tokens, max_pages, n_pages, write_kv,
+                                status);
+    };
+    if (bits == 8) return D == 64 ? wide(rope_quantize_wide_kernel<64, 8>) : wide(rope_quantize_wide_kernel<128, 8>);
+    return D == 64 ? wide(rope_quantize_wide_kernel<64, 4>) : wide(rope_quantize_wide_kernel<128, 4>);
+  }
   // few tokens: the heads of one token go to several blocks
   const int parts = N >= 592 ? 1 : min((Hq + 2 * Hkv + 3) / 4, (592 + N - 1) / N);
   auto go = [&](auto kernel, auto* typed) {

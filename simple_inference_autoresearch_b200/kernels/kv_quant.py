@@ -24,15 +24,16 @@ def check_entry(kv, n_kv_heads: int, head_dim: int, device) -> None:
     contiguity, one device."""
     if head_dim % 16 or not 0 < head_dim <= 256:
         raise ValueError(f"a quantised cache takes head_dim in steps of 16 up to 256, got {head_dim}")
-    page, pages = int(kv.page_tokens), kv.k.shape[0]
-    if kv.k.dtype == torch.int8:
-        want, scale_dtype, scale = (pages, n_kv_heads, page, head_dim), torch.float32, (pages, n_kv_heads, page)
-    elif kv.k.dtype == torch.uint8:
-        want, scale_dtype = (pages, n_kv_heads, page, head_dim // 2), torch.bfloat16
-        scale = (pages, n_kv_heads, page, -(-head_dim // 64), 2)
+    k, page = kv.k, int(kv.page_tokens)
+    code = k.dtype
+    rows = (k.shape[0], n_kv_heads, page)
+    if code == torch.int8:
+        want, scale, scale_dtype = rows + (head_dim,), rows, torch.float32
+    elif code == torch.uint8:
+        want, scale, scale_dtype = rows + (head_dim // 2,), rows + (-(-head_dim // 64), 2), torch.bfloat16
     else:
-        raise ValueError(f"a quantised cache holds int8 (8 bits) or uint8 (4 bits), got {kv.k.dtype}")
-    for name, t, shape, dtype in (("k", kv.k, want, kv.k.dtype), ("v", kv.v, want, kv.k.dtype),
+        raise ValueError(f"a quantised cache holds int8 (8 bits) or uint8 (4 bits), got {code}")
+    for name, t, shape, dtype in (("k", k, want, code), ("v", kv.v, want, code),
                                   ("k_scale", kv.k_scale, scale, scale_dtype), ("v_scale", kv.v_scale, scale, scale_dtype)):
         if t.shape != shape or t.dtype != dtype:
             raise ValueError(f"{name} of a cache entry in {kv.bits} bits must be {dtype} of shape {shape}, "
@@ -41,10 +42,11 @@ def check_entry(kv, n_kv_heads: int, head_dim: int, device) -> None:
             raise ValueError(f"{name} of a cache entry must be contiguous and 16-byte aligned")
         if t.device != device:
             raise ValueError(f"{name} of the cache entry is on {t.device}, the activations are on {device}")
-    if kv.block_table.dtype != torch.int32 or kv.block_table.dim() != 2 or not kv.block_table.is_contiguous():
+    table = kv.block_table
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise ValueError("block_table must be a contiguous int32 tensor [slots, pages per sequence]")
-    if kv.block_table.device != device:
-        raise ValueError(f"block_table is on {kv.block_table.device}, the activations are on {device}")
+    if table.device != device:
+        raise ValueError(f"block_table is on {table.device}, the activations are on {device}")
 
 
 def check_rows(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, meta) -> None:
@@ -139,48 +141,58 @@ def works_on_codes(kv, meta, dtype: torch.dtype, n_heads: int, n_kv_heads: int, 
         return False
     if not meta.is_decode and meta.max_q_len * (n_heads // n_kv_heads) > MOST_ROWS:
         return False
-    return bool(ops._fn("attention_quant", "siar_attn_quant_supported")(n_heads, n_kv_heads, head_dim, kv.page_tokens,
-                                                                        kv.k.shape[0]))
+    return kv.page_tokens % 64 == 0 and kv.k.shape[0] * n_kv_heads * kv.page_tokens < 1 << 31
 
 
-_eager_counters, _captured_counters = {}, {}
+_workspaces, _captured_workspaces = {}, {}
 
 
-def _zeroed_counters(n: int, device, stream: int) -> torch.Tensor:
-    """``n`` int32 zeros that a launch uses and leaves zero.  Launches of one stream follow one another and
-    share them; a captured graph may be replayed beside anything, so every capture has its own, zeroed by
-    the graph itself, shared by the launches that it holds on one stream."""
+def _workspace(index: int, stream: int):
+    """Pointers to the counters (zeros, which a launch uses and leaves zero) and the scratch of launches on
+    one stream of GPU ``index``.  Launches of one stream follow one another and share them; a captured graph may be
+    replayed beside anything, so every capture has its own, zeroed by the graph itself, for the launches that
+    it holds on one stream."""
+    key = (index, stream)
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        held = _workspaces.get(key)
+        if held is None:
+            held = _workspaces[key] = _new_workspace(index)
+        return held[:2]
     fn = ops._fn("attention_quant", "siar_capture_id")
     fn.restype = ops.c_ulonglong
     capture = fn(stream)
-    key = (device.index, stream)
-    if capture:
-        held = _captured_counters.get(key)
-        if held is None or held[0] != capture or held[1].numel() < n:
-            held = _captured_counters[key] = (capture, torch.zeros(n, dtype=torch.int32, device=device))
-        return held[1]
-    t = _eager_counters.get(key)
-    if t is None or t.numel() < n:
-        t = _eager_counters[key] = torch.zeros(n, dtype=torch.int32, device=device)
-    return t
+    held = _captured_workspaces.get(key)
+    if held is None or held[-1] != capture:
+        held = _captured_workspaces[key] = _new_workspace(index) + (capture,)
+    return held[:2]
+
+
+def _new_workspace(index: int):
+    sms = ops._sm_count(index)
+    sizes = []
+    for name in ("siar_attn_quant_counters", "siar_attn_quant_scratch_floats"):
+        fn = ops._fn("attention_quant", name)
+        fn.restype = ops.c_longlong
+        sizes.append(fn(sms))
+    counters = torch.zeros(sizes[0], dtype=torch.int32, device=f"cuda:{index}")
+    scratch = torch.empty(sizes[1], dtype=torch.float32, device=f"cuda:{index}")
+    return counters.data_ptr(), scratch.data_ptr(), counters, scratch
 
 
 def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
     device = qkv.device
-    out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
+    index = device.index
+    k, table = kv.k, kv.block_table
     with ops._on_device(qkv):
-        blocks = ops._fn("attention_quant", "siar_attn_quant_blocks")(
-            kv.bits, meta.n_seqs, n_heads, n_kv_heads, head_dim, meta.max_q_len, meta.max_kv_len, ops._sm_count(device))
-        fn = ops._fn("attention_quant", "siar_attn_quant_scratch_floats")
-        fn.restype = ops.c_longlong
-        scratch = torch.empty(fn(n_heads, n_kv_heads, head_dim, meta.max_q_len, blocks), dtype=torch.float32, device=device)
-        stream = ops._stream()
-        counters = _zeroed_counters(blocks, device, stream)
-        ops._launch("attention_quant", "siar_attn_quant", kv.bits, ops._ptr(qkv), ops._ptr(kv.k), ops._ptr(kv.v),
-                    ops._ptr(kv.k_scale), ops._ptr(kv.v_scale), ops._ptr(kv.block_table), *_batch(meta), ops._ptr(inv_freq),
-                    ops._ptr(out), ops._ptr(scratch), ops._ptr(counters), blocks, meta.n_seqs, n_heads, n_kv_heads, head_dim,
-                    kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], meta.max_q_len, int(fused), int(write_kv),
-                    float(scale), ops._ptr(ops.status_word(device)), stream)
+        out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        counters, scratch = _workspace(index, stream)
+        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), k.data_ptr(), kv.v.data_ptr(),
+                    kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), table.data_ptr(), meta.slot_ids.data_ptr(),
+                    meta.q_start.data_ptr(), meta.base_len.data_ptr(), ops._ptr(inv_freq), out.data_ptr(), counters, scratch,
+                    meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], meta.max_q_len,
+                    meta.max_kv_len, ops._sm_count(index), int(fused), int(write_kv), float(scale),
+                    ops.status_word(device).data_ptr(), stream)
     return out
 
 

@@ -85,14 +85,14 @@ _signatures = {
                          c_int, c_int, c_void_p, c_void_p],
     },
     "attention_quant": {
-        # bits, qkv, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, scratch, counters,
-        # blocks, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, fused, write_kv, scale, status, stream
+        # bits, qkv, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
+        # B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, max_kv_len, sm_count, fused, write_kv, scale, status,
+        # stream
         "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
-                            c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
-        "siar_attn_quant_supported": [c_int, c_int, c_int, c_int, c_longlong],
-        "siar_attn_quant_blocks": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int],
-        "siar_attn_quant_scratch_floats": [c_int, c_int, c_int, c_int, c_int],
+                            c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+        "siar_attn_quant_counters": [c_int],
+        "siar_attn_quant_scratch_floats": [c_int],
         "siar_capture_id": [c_void_p],
     },
     "sampling": {
@@ -125,7 +125,7 @@ def _launch(unit: str, name: str, *args, kernels: int = 1) -> None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class _Here:
@@ -143,7 +143,7 @@ _here = _Here()
 
 def _on_device(t: torch.Tensor):
     """A context in which ``t``'s device is the current one (its stream and launches are then that device's)."""
-    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _here if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -177,7 +177,7 @@ STATUS_MESSAGES = {
 
 
 def status_word(device) -> torch.Tensor:
-    dev = torch.device(device)
+    dev = device if isinstance(device, torch.device) else torch.device(device)
     key = dev.index if dev.index is not None else torch.cuda.current_device()
     t = _status.get(key)
     if t is None:
@@ -462,10 +462,11 @@ _sms = {}
 
 
 def _sm_count(device) -> int:
-    dev = torch.device(device)
-    key = dev.index if dev.index is not None else torch.cuda.current_device()
+    key = device if isinstance(device, int) else torch.device(device).index
+    if key is None:
+        key = torch.cuda.current_device()
     if key not in _sms:
-        _sms[key] = torch.cuda.get_device_properties(dev).multi_processor_count
+        _sms[key] = torch.cuda.get_device_properties(key).multi_processor_count
     return _sms[key]
 
 
