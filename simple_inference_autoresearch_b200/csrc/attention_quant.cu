@@ -106,12 +106,6 @@ __device__ __forceinline__ void mma_bytes(int (&d)[4], uint32_t a0, uint32_t a1,
   else { SIAR_MMA("u8", "u8"); }
 #undef SIAR_MMA
 }
-// The larger of two, NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));

@@ -109,156 +109,196 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
   }
 }
 
-// The same for bfloat16, head_dim 64 or 128 and whole-head rotation in pairs (i, i + D/2), 8 bytes an access: D/8
-// lanes share a head, a lane holds dims 4j .. 4j + 3 and D/2 + 4j .. + 3, so the pairs of a rotation are its own
-// and a row's statistics take a few shuffles.  A block of 256 threads takes a token's heads kPasses x 256 / (D/8)
-// at a time, all of their loads asked for before the rotation angles are formed.
+// The same for bfloat16, head_dim 64 or 128 and whole-head rotation in pairs (i, i + D/2), 16 bytes an access: D/16
+// lanes share a head, a lane holds dims 8j .. 8j + 7 and D/2 + 8j .. + 7, so the pairs of a rotation are its own
+// and a row's statistics take two or three shuffles.  A block walks a run of tokens, kTokens of them at a time:
+// their sequences, pages and angles are formed together, and a token's heads are asked for while the token in
+// front is worked on.  Instructions bound it before memory does: with 8 bytes an access and a division for every
+// code 200 warp instructions for two heads, 59 us for 9,500 tokens of the 8B heads where their bytes take 34.
 template <int D, int BITS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128, 5)
 rope_quantize_wide_kernel(const __nv_bfloat16* qkv, __nv_bfloat16* q_out, const float* __restrict__ inv_freq,
                           uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, void* __restrict__ k_scale,
                           void* __restrict__ v_scale, const int* block_table, const int* slot_ids, const int* q_start,
-                          const int* base_len, int B, int Hq, int Hkv, int page_tokens, int max_pages, int n_pages,
+                          const int* base_len, int N, int B, int Hq, int Hkv, int page_tokens, int max_pages, int n_pages,
                           int write_kv, int* __restrict__ status) {
-  constexpr int LANES = D / 8, HEADS = 256 / LANES, kPasses = 3, NG = D / kQuantGroup;
+  constexpr int LANES = D / 16, HEADS = 128 / LANES, kPasses = 3, NG = BITS == 8 ? 1 : D / kQuantGroup, kTokens = 4;
   pdl_launch_dependents();
-  __shared__ float cos_s[D / 2], sin_s[D / 2];
-  float freq = 0.f;
-  if (inv_freq != nullptr && threadIdx.x < D / 2) freq = inv_freq[threadIdx.x];
+  __shared__ __align__(16) float cos_s[kTokens][D / 2], sin_s[kTokens][D / 2];
+  __shared__ int pos_s[kTokens], page_s[kTokens];
+  const float freq = inv_freq != nullptr ? inv_freq[threadIdx.x % (D / 2)] : 0.f;
   pdl_wait();
-  const int t = blockIdx.x;
-  const int j = threadIdx.x % LANES, h0 = threadIdx.x / LANES;
+  const int t_begin = (int)((long long)N * blockIdx.x / gridDim.x), t_end = (int)((long long)N * (blockIdx.x + 1) / gridDim.x);
+  const int lane = threadIdx.x & 31, j = threadIdx.x % LANES, h0 = threadIdx.x / LANES;
+  const unsigned mates = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));       // the lanes that share the head
   const int heads = Hq + 2 * Hkv, stride = gridDim.y * HEADS;
-  const __nv_bfloat16* row = qkv + (size_t)t * heads * D + 4 * j;
-  uint2 lo[kPasses], hi[kPasses];
-  auto load = [&](int first) {
+  const size_t token_elems = (size_t)heads * D;
+  uint4 lo[kPasses], hi[kPasses];
+  auto load = [&](int t, int base) {                // kPasses heads of token t
+    if (t >= t_end) return;
+    const __nv_bfloat16* row = qkv + t * token_elems + (size_t)(base + h0) * D + 8 * j;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int head = first + p * stride;
-      if (head < heads) {
-        lo[p] = *reinterpret_cast<const uint2*>(row + (size_t)head * D);
-        hi[p] = *reinterpret_cast<const uint2*>(row + (size_t)head * D + D / 2);
+    for (int p = 0; p < kPasses; ++p)
+      if (base + h0 + p * stride < heads) {
+        lo[p] = *reinterpret_cast<const uint4*>(row + (size_t)p * stride * D);
+        hi[p] = *reinterpret_cast<const uint4*>(row + (size_t)p * stride * D + D / 2);
       }
-    }
   };
-  int first = blockIdx.y * HEADS + h0;
-  load(first);
-  const int b = sequence_of(q_start, B, t);
-  const int pos = base_len[b] + (t - q_start[b]);
-  if (inv_freq != nullptr && threadIdx.x < D / 2) rotation(pos, freq, &cos_s[threadIdx.x], &sin_s[threadIdx.x]);
-  int page = -1;
-  if (write_kv) {
-    page = pos / page_tokens < max_pages ? block_table[(size_t)slot_ids[b] * max_pages + pos / page_tokens] : -1;
-    if (page < 0 || page >= n_pages) {
-      page = -1;
-      if (threadIdx.x == 0) atomicOr(status, kStatusBadPage);
-    }
-  }
-  __syncthreads();
-  const size_t row0 = (size_t)max(page, 0) * Hkv * page_tokens + pos % page_tokens;      // kv head 0
-  float cv[4], sv[4];
+  load(t_begin, blockIdx.y * HEADS);
+  for (int t0 = t_begin; t0 < t_end; t0 += kTokens) {
+    __syncthreads();                                // the angles of the tokens in front have been used
+    if (threadIdx.x < 32) {
+      // sequence of each token: for up to 32 sequences all of their descriptions are asked for at once
+      const int t = t0 + lane;
+      int pos = 0, slot = 0;
+      if (B <= 32) {
+        const int next = lane < B ? q_start[lane + 1] : 0x7fffffff, first = lane < B ? q_start[lane] : 0;
+        const int base = lane < B ? base_len[lane] : 0, own = lane < B ? slot_ids[lane] : 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    cv[e] = inv_freq != nullptr ? cos_s[4 * j + e] : 1.f;
-    sv[e] = inv_freq != nullptr ? sin_s[4 * j + e] : 0.f;
-  }
-  // of the lanes that share a head
-  auto group_max = [](float v) {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-  };
-  // every thread runs every round: the shuffles take whole warps
-  for (int base = blockIdx.y * HEADS; base < heads; base += kPasses * stride) {
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int head = base + h0 + p * stride;
-      if (base + p * stride >= heads) break;
-      const bool in = head < heads;
-      float x[8];
-      const uint2 l = in ? lo[p] : make_uint2(0u, 0u), u = in ? hi[p] : make_uint2(0u, 0u);
-      const uint32_t w[4] = {l.x, l.y, u.x, u.y};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = __uint_as_float(w[e] << 16);
-        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        for (int i = 0; i < kTokens; ++i) {
+          const int b = min(__popc(__ballot_sync(0xffffffffu, next <= t0 + i)), B - 1);
+          const int at = __shfl_sync(0xffffffffu, base - first, b), sl = __shfl_sync(0xffffffffu, own, b);
+          if (lane == i) { pos = at + t; slot = sl; }
+        }
+      } else if (lane < kTokens && t < t_end) {
+        const int b = sequence_of(q_start, B, t);
+        pos = base_len[b] + (t - q_start[b]);
+        slot = slot_ids[b];
       }
-      if (inv_freq != nullptr && head < Hq + Hkv) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = x[e], c = x[4 + e];
-          x[e] = rotate_lo(a, c, cv[e], sv[e]);
-          x[4 + e] = rotate_hi(a, c, cv[e], sv[e]);
+      if (lane < kTokens && t < t_end) {
+        int page = -1;
+        if (write_kv) {
+          const int cell = pos / page_tokens;
+          page = cell < max_pages ? block_table[(size_t)slot * max_pages + cell] : -1;
+          if (page < 0 || page >= n_pages) {
+            page = -1;
+            atomicOr(status, kStatusBadPage);
+          }
         }
-      }
-      if (in && head < Hq) {
-        __nv_bfloat16* dst = q_out + (size_t)t * heads * D + (size_t)head * D + 4 * j;
-        uint2 o[2];
-        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o2[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        *reinterpret_cast<uint2*>(dst) = o[0];
-        *reinterpret_cast<uint2*>(dst + D / 2) = o[1];
-      }
-      // (lanes of query heads in a warp with key heads go along for the shuffles)
-      const bool is_k = head < Hq + Hkv, stores = in && head >= Hq && page >= 0;
-      if (!__any_sync(0xffffffffu, stores)) continue;
-      const int kvh = is_k ? head - Hq : head - Hq - Hkv;
-      const size_t at = row0 + (size_t)max(kvh, 0) * page_tokens;
-      uint8_t* codes = (is_k ? k_pool : v_pool) + at * (D * BITS / 8);
-      float top[NG], bot[NG];                       // per run (8 bits: per row, of |x|)
-      bool bad[NG];
-      if (BITS == 8 || NG == 1) {
-        float m = 0.f, n = INFINITY, a = -INFINITY;
-        bool wrong = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          m = fmaxf(m, fabsf(x[e]));
-          n = fminf(n, x[e]);
-          a = fmaxf(a, x[e]);
-          wrong |= !isfinite(x[e]);
-        }
-        top[0] = group_max(BITS == 8 ? m : a);
-        bot[0] = BITS == 8 ? 0.f : -group_max(-n);
-        bad[0] = group_max(wrong ? 1.f : 0.f) > 0.f;
-      } else {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const float* y = x + 4 * g;
-          const bool wrong = !isfinite(y[0]) || !isfinite(y[1]) || !isfinite(y[2]) || !isfinite(y[3]);
-          top[g] = group_max(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-          bot[g] = -group_max(-fminf(fminf(y[0], y[1]), fminf(y[2], y[3])));
-          bad[g] = group_max(wrong ? 1.f : 0.f) > 0.f;
-        }
-      }
-      if (!stores) continue;
-      if (BITS == 8) {
-        const float s = scale8(top[0]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t c = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c |= (uint32_t)(code8(x[4 * h + e], s, bad[0]) & 0xff) << (8 * e);
-          *reinterpret_cast<uint32_t*>(codes + h * (D / 2) + 4 * j) = c;
-        }
-        if (j == 0) reinterpret_cast<float*>(is_k ? k_scale : v_scale)[at] = bad[0] ? __int_as_float(0x7fc00000) : s;
-      } else {
-        __nv_bfloat162* sc = reinterpret_cast<__nv_bfloat162*>(is_k ? k_scale : v_scale) + at * NG;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int g = NG == 1 ? 0 : h;
-          const __nv_bfloat162 sm = scale4(bot[g], top[g], bad[g]);
-          const float s = __low2float(sm), m = __high2float(sm);
-          uint32_t c = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c |= (uint32_t)code4(x[4 * h + e], s, m) << (4 * e);
-          *reinterpret_cast<uint16_t*>(codes + h * (D / 4) + 2 * j) = (uint16_t)c;
-          if (j == 0 && (NG == 2 || h == 0)) sc[g] = sm;
-        }
+        pos_s[lane] = pos;
+        page_s[lane] = page;
       }
     }
-    first += kPasses * stride;
-    load(first);
+    __syncthreads();
+    if (inv_freq != nullptr) {
+      const int f = threadIdx.x % (D / 2);
+      for (int i = threadIdx.x / (D / 2); i < kTokens && t0 + i < t_end; i += 128 / (D / 2))
+        rotation(pos_s[i], freq, &cos_s[i][f], &sin_s[i][f]);
+      __syncthreads();
+    }
+    for (int t = t0; t < min(t0 + kTokens, t_end); ++t) {
+      const int page = page_s[t - t0];
+      const size_t row0 = (size_t)max(page, 0) * Hkv * page_tokens + pos_s[t - t0] % page_tokens;      // kv head 0
+      const float4* cs = reinterpret_cast<const float4*>(cos_s[t - t0]) + 2 * j;
+      const float4* sn = reinterpret_cast<const float4*>(sin_s[t - t0]) + 2 * j;
+      for (int base = blockIdx.y * HEADS; base < heads; base += kPasses * stride) {
+        uint4 now_lo[kPasses], now_hi[kPasses];
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          now_lo[p] = lo[p];
+          now_hi[p] = hi[p];
+        }
+        if (base + kPasses * stride < heads) load(t, base + kPasses * stride);
+        else load(t + 1, blockIdx.y * HEADS);
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          const int head = base + h0 + p * stride;
+          if (head >= heads || (head >= Hq && page < 0)) continue;          // the same for all lanes of a head
+          float x[16];
+          const uint32_t w[8] = {now_lo[p].x, now_lo[p].y, now_lo[p].z, now_lo[p].w,
+                                 now_hi[p].x, now_hi[p].y, now_hi[p].z, now_hi[p].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[2 * e] = __uint_as_float(w[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+          if (inv_freq != nullptr && head < Hq + Hkv) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float4 c4 = cs[q], s4 = sn[q];
+              const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float a = x[4 * q + e], c = x[8 + 4 * q + e];
+                x[4 * q + e] = rotate_lo(a, c, cv[e], sv[e]);
+                x[8 + 4 * q + e] = rotate_hi(a, c, cv[e], sv[e]);
+              }
+            }
+          }
+          if (head < Hq) {
+            __nv_bfloat16* dst = q_out + t * token_elems + (size_t)head * D + 8 * j;
+            uint4 o[2];
+            __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o2[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+            *reinterpret_cast<uint4*>(dst) = o[0];
+            *reinterpret_cast<uint4*>(dst + D / 2) = o[1];
+            continue;
+          }
+          const bool is_k = head < Hq + Hkv;
+          const size_t at = row0 + (size_t)(is_k ? head - Hq : head - Hq - Hkv) * page_tokens;
+          uint8_t* codes = (is_k ? k_pool : v_pool) + at * (D * BITS / 8);
+          // largest and smallest of a run (8 bits: largest |x| of the row); NaN if one is
+          constexpr int PER = 16 / NG;
+          float top[NG], bot[NG];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            float most = -INFINITY, least = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+              const float y = x[g * PER + e];
+              most = max_nan(most, BITS == 8 ? fabsf(y) : y);
+              if (BITS == 4) least = max_nan(least, -y);
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+              most = max_nan(most, __shfl_xor_sync(mates, most, o));
+              if (BITS == 4) least = max_nan(least, __shfl_xor_sync(mates, least, o));
+            }
+            top[g] = most;
+            bot[g] = -least;
+          }
+          if (BITS == 8) {
+            const float s = scale8(top[0]);
+            const bool bad = !isfinite(top[0]);
+            const Divisor by = divisor(s);
+            if (by.k != 1.f) {                      // (a scale near the ends of the range may itself be rounded coarsely)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = fmaxf(-127.f * by.s, fminf(127.f * by.s, x[e] * by.k));
+            }
+            uint32_t c[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) c[e] = whole_bits(corrected(x[e], by));       // |x| <= 127 s: no code leaves its byte
+            uint32_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              b[e] = __byte_perm(__byte_perm(c[4 * e], c[4 * e + 1], 0x0040), __byte_perm(c[4 * e + 2], c[4 * e + 3], 0x0040), 0x5410);
+            *reinterpret_cast<uint2*>(codes + 8 * j) = bad ? make_uint2(0u, 0u) : make_uint2(b[0], b[1]);
+            *reinterpret_cast<uint2*>(codes + D / 2 + 8 * j) = bad ? make_uint2(0u, 0u) : make_uint2(b[2], b[3]);
+            if (j == 0) reinterpret_cast<float*>(is_k ? k_scale : v_scale)[at] = bad ? __int_as_float(0x7fc00000) : s;
+          } else {
+            __nv_bfloat162* sc = reinterpret_cast<__nv_bfloat162*>(is_k ? k_scale : v_scale) + at * NG;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int g = NG == 1 ? 0 : h;
+              const bool bad = !isfinite(top[g]) || !isfinite(bot[g]);
+              const __nv_bfloat162 sm = scale4(bot[g], top[g], bad);
+              const Divisor by = divisor(__low2float(sm));
+              const float m = __high2float(sm);
+              uint32_t c = 0;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float y = __fsub_rn(x[8 * h + e], m);
+                if (by.k != 1.f) y *= by.k;
+                c |= ((whole_bits(fmaxf(-8.f, fminf(7.f, corrected(y, by)))) + 8u) & 15u) << (4 * e);
+              }
+              *reinterpret_cast<uint32_t*>(codes + h * (D / 4) + 4 * j) = bad ? 0x88888888u : c;
+              if (j == 0 && (NG == 2 || h == 0)) sc[g] = sm;
+            }
+          }
+        }
+      }
+    }
   }
 }
 
@@ -312,41 +352,71 @@ read_kv_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale
   const size_t out0 = ((size_t)(first + p) * Hkv + kvh) * page_tokens;
   const int rows_held = absent ? 0 : min(page_tokens, total - p * page_tokens);
   const int per_row = D / 16, groups = (D + kQuantGroup - 1) / kQuantGroup;
-  for (int idx = threadIdx.x; idx < 2 * page_tokens * per_row; idx += blockDim.x) {
-    const bool is_k = idx < page_tokens * per_row;
-    const int i = is_k ? idx : idx - page_tokens * per_row;
-    const int r = i / per_row, d = (i % per_row) * 16;
-    float x[16];
-    if (r >= rows_held) {
+  // 16 codes a thread and turn, kTurns turns asked for together
+  constexpr int kTurns = 1;
+  for (int first_idx = threadIdx.x; first_idx < 2 * page_tokens * per_row; first_idx += kTurns * blockDim.x) {
+    uint4 code[kTurns];
+    uint32_t scale[kTurns];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = 0.f;
-    } else if (BITS == 8) {
-      const float s = reinterpret_cast<const float*>(is_k ? k_scale : v_scale)[row0 + r];
-      const int4 c = *reinterpret_cast<const int4*>((is_k ? k_pool : v_pool) + (row0 + r) * D + d);
-      const int w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * s;
-    } else {
-      const __nv_bfloat162 sm = reinterpret_cast<const __nv_bfloat162*>(is_k ? k_scale : v_scale)[(row0 + r) * groups + d / kQuantGroup];
-      const float s = __low2float(sm), m = __high2float(sm);
-      const int2 c = *reinterpret_cast<const int2*>((is_k ? k_pool : v_pool) + ((row0 + r) * D + d) / 2);
-      const int w[2] = {c.x, c.y};
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        x[e] = __fadd_rn(__fmul_rn((float)(((w[e >> 3] >> (4 * (e & 7))) & 15) - 8), s), m);
+    for (int u = 0; u < kTurns; ++u) {
+      const int idx = first_idx + u * blockDim.x;
+      const bool is_k = idx < page_tokens * per_row;
+      const int i = is_k ? idx : idx - page_tokens * per_row;
+      const int r = i / per_row, d = (i % per_row) * 16;
+      code[u] = make_uint4(0u, 0u, 0u, 0u);
+      scale[u] = 0u;
+      if (idx >= 2 * page_tokens * per_row || r >= rows_held) continue;
+      const uint8_t* src = (is_k ? k_pool : v_pool) + ((row0 + r) * D + d) * BITS / 8;
+      const uint32_t* sc = reinterpret_cast<const uint32_t*>(is_k ? k_scale : v_scale);
+      if (BITS == 8) {
+        code[u] = *reinterpret_cast<const uint4*>(src);
+        scale[u] = sc[row0 + r];
+      } else {
+        const uint2 c = *reinterpret_cast<const uint2*>(src);
+        code[u].x = c.x;
+        code[u].y = c.y;
+        scale[u] = sc[(row0 + r) * groups + d / kQuantGroup];
+      }
     }
-    T* dst = (is_k ? k_out : v_out) + (out0 + r) * D + d;
-    if (sizeof(T) == 2) {
-      uint4 pk[2];
-      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(pk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-      reinterpret_cast<uint4*>(dst)[0] = pk[0];
-      reinterpret_cast<uint4*>(dst)[1] = pk[1];
-    } else {
+    for (int u = 0; u < kTurns; ++u) {
+      const int idx = first_idx + u * blockDim.x;
+      if (idx >= 2 * page_tokens * per_row) break;
+      const bool is_k = idx < page_tokens * per_row;
+      const int i = is_k ? idx : idx - page_tokens * per_row;
+      const int r = i / per_row, d = (i % per_row) * 16;
+      // a code as a float: its bits in the mantissa of 2^23, the constant taken off again (both exact).  Rows behind
+      // the last token have codes and scales of zero here; 4-bit codes stand for code - 8, so they are set apart
+      const uint32_t w[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
+      float x[16];
+      if (BITS == 8) {
+        const float s = __uint_as_float(scale[u]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        reinterpret_cast<float4*>(dst)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        for (int e = 0; e < 16; ++e)
+          x[e] = (__uint_as_float(__byte_perm(w[e >> 2] ^ 0x80808080u, 0x4b000000u, 0x7440 + (e & 3))) - 8388736.f) * s;
+      } else {
+        const float s = __uint_as_float(scale[u] << 16), m = __uint_as_float(scale[u] & 0xffff0000u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          x[e] = __fadd_rn(__fmul_rn(__uint_as_float(((w[e >> 3] >> (4 * (e & 7))) & 15u) | 0x4b000000u) - 8388616.f, s), m);
+      }
+      if (r >= rows_held) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+      }
+      T* dst = (is_k ? k_out : v_out) + (out0 + r) * D + d;
+      if (sizeof(T) == 2) {
+        uint4 pk[2];
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(pk);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        reinterpret_cast<uint4*>(dst)[0] = pk[0];
+        reinterpret_cast<uint4*>(dst)[1] = pk[1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<float4*>(dst)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+      }
     }
   }
 }
@@ -356,6 +426,12 @@ read_kv_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale
 using namespace siar;
 
 SIAR_DEFINE_PDL_SWITCH()
+
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+  return n;
+}
 
 // qkv [N, (Hq + 2 Hkv) D] (not changed unless q_out == qkv); q_out: the same layout, its query part is
 // written (rotated).  Pools and scales as at the top of the file.
@@ -370,13 +446,14 @@ extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* 
     return (int)cudaErrorInvalidValue;
   if (is_bf16 && (D == 64 || D == 128) && (inv_freq == nullptr || (rotary_dim == D && !interleaved)) &&
       (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0) {
-    const int per_block = 256 / (D / 8);            // few tokens: the heads of one token go to several blocks
+    const int per_block = 128 / (D / 16);           // few tokens: the heads of one token go to several blocks
     const int most = (Hq + 2 * Hkv + per_block - 1) / per_block, split = N >= 296 ? 1 : min(most, (296 + N - 1) / N);
+    const int blocks = min(N, 5 * sm_count());
     auto wide = [&](auto kernel) {
-      return (int)launch_kernel(kernel, dim3(N, split), dim3(256), 0, (cudaStream_t)stream, (const __nv_bfloat16*)qkv,
+      return (int)launch_kernel(kernel, dim3(blocks, split), dim3(128), 0, (cudaStream_t)stream, (const __nv_bfloat16*)qkv,
                                 (__nv_bfloat16*)q_out, inv_freq, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale,
-                                block_table, slot_ids, q_start, base_len, B, Hq, Hkv, page_tokens, max_pages, n_pages, write_kv,
-                                status);
+                                block_table, slot_ids, q_start, base_len, N, B, Hq, Hkv, page_tokens, max_pages, n_pages,
+                                write_kv, status);
     };
     if (bits == 8) return D == 64 ? wide(rope_quantize_wide_kernel<64, 8>) : wide(rope_quantize_wide_kernel<128, 8>);
     return D == 64 ? wide(rope_quantize_wide_kernel<64, 4>) : wide(rope_quantize_wide_kernel<128, 4>);

@@ -16,6 +16,13 @@ __device__ __forceinline__ float warp_min(float v) {
   return v;
 }
 
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // One pair of a rotation: rounded products, a rounded sum (no fused multiply-add), so that the codes
 // are a function of the row and the position alone, whatever kernel forms them.
 __device__ __forceinline__ float rotate_lo(float a, float c, float cosv, float sinv) {
@@ -58,20 +65,41 @@ __device__ __forceinline__ void rotation(int pos, float freq, float* cosv, float
   *cosv = (q == 1 || q == 2) ? -cf : cf;
 }
 
-// The scale of a row in 8 bits, and a code against it (0 without a scale).
-__device__ __forceinline__ float scale8(float amax) { return __fdiv_rn(amax, 127.f); }
-__device__ __forceinline__ int code8(float x, float s, bool bad) {
-  return bad || !(s > 0.f) ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
+// x / s rounded to nearest for all the values of a row, which share s: with r the rounded reciprocal of s, the
+// quotient x r is off by little more than its last bit, and Markstein's correction (q + (x - q s) r, both fused)
+// rounds it as a division does, while nothing under- or overflows on the way.  A scale outside 2^-90 .. 2^90 is
+// brought inside by a power of two (k), the values with it.  Without a scale (zero, infinite, NaN) quotients of
+// finite values are 0.
+struct Divisor {
+  float s, r, k;
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+  if (!(s > 0.f && s < INFINITY)) return Divisor{0.f, 0.f, 1.f};
+  const float k = s < 0x1p-90f ? 0x1p60f : s > 0x1p90f ? 0x1p-60f : 1.f;
+  return Divisor{s * k, __frcp_rn(s * k), k};
 }
-// Scale and mid of a run in 4 bits, and a code against them.
+__device__ __forceinline__ float corrected(float x, const Divisor& by) {       // x already times k
+  const float q = __fmul_rn(x, by.r);
+  return fmaf(fmaf(-q, by.s, x), by.r, q);
+}
+__device__ __forceinline__ float quotient(float x, const Divisor& by) { return corrected(x * by.k, by); }
+// rint(y) for |y| < 2^22, in the low bits (two's complement): adding 1.5 x 2^23 rounds to a whole number.
+__device__ __forceinline__ uint32_t whole_bits(float y) { return __float_as_uint(__fadd_rn(y, 12582912.f)); }
+
+// The scale of a row in 8 bits, and a code against it in the low byte (0 without a scale).
+__device__ __forceinline__ float scale8(float amax) { return __fdiv_rn(amax, 127.f); }
+__device__ __forceinline__ uint32_t code8(float x, const Divisor& by, bool bad) {
+  return bad ? 0u : whole_bits(fmaxf(-127.f, fminf(127.f, quotient(x, by))));
+}
+// Scale and mid of a run in 4 bits, and a code against them in the low four bits.
 __device__ __forceinline__ __nv_bfloat162 scale4(float lo, float hi, bool bad) {
   const __nv_bfloat16 s = __float2bfloat16_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)));
   const __nv_bfloat16 m = __float2bfloat16_rn(__fadd_rn(lo, 8.f * __bfloat162float(s)));
   const float nan = __int_as_float(0x7fc00000);
   return bad ? __floats2bfloat162_rn(nan, nan) : __halves2bfloat162(s, m);
 }
-__device__ __forceinline__ int code4(float x, float s, float m) {        // s, m: NaN for a bad run
-  return !(s > 0.f) ? 8 : max(0, min(15, __float2int_rn(__fdiv_rn(__fsub_rn(x, m), s)) + 8));
+__device__ __forceinline__ uint32_t code4(float x, const Divisor& by, float m, bool bad) {
+  return bad ? 8u : (whole_bits(fmaxf(-8.f, fminf(7.f, quotient(__fsub_rn(x, m), by)))) + 8u) & 15u;
 }
 
 // One warp quantises a row x[0 .. D) (shared memory): lane l holds dims 64 i + 2l, + 2l + 1 of run i.
@@ -89,8 +117,8 @@ __device__ __forceinline__ void quantize_row(const float* row, int D, int lane, 
     amax = warp_max(amax);
     bad = __any_sync(0xffffffffu, bad);
     const float s = scale8(amax);
-    for (int d = 2 * lane; d < D; d += 64)
-      codes(d, (uint32_t)((code8(row[d], s, bad) & 0xff) | ((code8(row[d + 1], s, bad) & 0xff) << 8)));
+    const Divisor by = divisor(s);
+    for (int d = 2 * lane; d < D; d += 64) codes(d, __byte_perm(code8(row[d], by, bad), code8(row[d + 1], by, bad), 0x7740) & 0xffffu);
     if (lane == 0) scales(0, bad ? __int_as_float(0x7fc00000) : s, __floats2bfloat162_rn(0.f, 0.f));
   } else {
     for (int g = 0; g * kQuantGroup < D; ++g) {
@@ -100,8 +128,9 @@ __device__ __forceinline__ void quantize_row(const float* row, int D, int lane, 
       const bool bad = __any_sync(0xffffffffu, !isfinite(x0) || !isfinite(x1));
       const float lo = warp_min(in ? fminf(x0, x1) : INFINITY), hi = warp_max(in ? fmaxf(x0, x1) : -INFINITY);
       const __nv_bfloat162 sm = scale4(lo, hi, bad);
-      const float s = __low2float(sm), m = __high2float(sm);
-      if (in) codes(d, (uint32_t)(code4(x0, s, m) | (code4(x1, s, m) << 4)));
+      const Divisor by = divisor(__low2float(sm));
+      const float m = __high2float(sm);
+      if (in) codes(d, code4(x0, by, m, bad) | (code4(x1, by, m, bad) << 4));
       if (lane == 0) scales(g, 0.f, sm);
     }
   }
