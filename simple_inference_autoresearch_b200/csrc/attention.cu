@@ -136,7 +136,9 @@ attn_prefill_kernel(const T* __restrict__ qkv, const T* __restrict__ k_pool, con
       m[i] = m_new;
 #pragma unroll
       for (int n = 0; n < NDIM; ++n) acc[i][n] *= alpha;
-      for (int j = 0; j < kTile; ++j) {
+      // only the keys that the row sees: 0 x a value that is no number would reach it from the others
+      const int j_end = min(kTile, kv_end[i] - j0);
+      for (int j = max(0, kv_begin[i] - j0); j < j_end; ++j) {
         const float pj = __shfl_sync(0xffffffffu, p, j);
 #pragma unroll
         for (int n = 0; n < NDIM; ++n) {
