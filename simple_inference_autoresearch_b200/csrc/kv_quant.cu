@@ -19,6 +19,8 @@
 // rounded products and a rounded sum, so a code depends on the token's row and position alone.
 #include "kv_quant.cuh"
 
+#include <cuda_fp16.h>
+
 namespace siar {
 
 // The batch description and the block table are read through plain pointers, behind pdl_wait(): the
@@ -115,9 +117,12 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
 // their sequences, pages and angles are formed together, and a token's heads are asked for while the token in
 // front is worked on.  Instructions bound it before memory does: with 8 bytes an access and a division for every
 // code 200 warp instructions for two heads, 59 us for 9,500 tokens of the 8B heads where their bytes take 34.
-template <int D, int BITS>
+// F16: queries leave as float16 [tokens, Hq, D], each row times a power of two that brings its largest element to
+// 2^9 .. 2^10, and that power's inverse as the row's factor (what the prompt attention on float16 tiles takes: 11 bits
+// of a query where bfloat16 keeps 8).
+template <int D, int BITS, bool F16>
 __global__ void __launch_bounds__(128, 5)
-rope_quantize_wide_kernel(const __nv_bfloat16* qkv, __nv_bfloat16* q_out, const float* __restrict__ inv_freq,
+rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor, const float* __restrict__ inv_freq,
                           uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, void* __restrict__ k_scale,
                           void* __restrict__ v_scale, const int* block_table, const int* slot_ids, const int* q_start,
                           const int* base_len, int N, int B, int Hq, int Hkv, int page_tokens, int max_pages, int n_pages,
@@ -226,11 +231,27 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, __nv_bfloat16* q_out, const 
             }
           }
           if (head < Hq) {
-            __nv_bfloat16* dst = q_out + t * token_elems + (size_t)head * D + 8 * j;
             uint4 o[2];
-            __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(o);
+            uint16_t* dst;
+            if (F16) {
+              float most = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o2[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+              for (int e = 0; e < 16; ++e) most = max_nan(most, fabsf(x[e]));
+#pragma unroll
+              for (int q = LANES / 2; q > 0; q >>= 1) most = max_nan(most, __shfl_xor_sync(mates, most, q));
+              const int up = max(-120, min(60, 9 + 127 - (int)(__float_as_uint(most) >> 23)));
+              const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+              __half2* o2 = reinterpret_cast<__half2*>(o);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o2[e] = __floats2half2_rn(x[2 * e] * f, x[2 * e + 1] * f);
+              if (j == 0) q_factor[(size_t)t * Hq + head] = isfinite(most) ? 1.f / f : __int_as_float(0x7fc00000);
+              dst = reinterpret_cast<uint16_t*>(q_to) + ((size_t)t * Hq + head) * D + 8 * j;
+            } else {
+              __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(o);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o2[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+              dst = reinterpret_cast<uint16_t*>(q_to) + t * token_elems + (size_t)head * D + 8 * j;
+            }
             *reinterpret_cast<uint4*>(dst) = o[0];
             *reinterpret_cast<uint4*>(dst + D / 2) = o[1];
             continue;
@@ -433,6 +454,23 @@ static int sm_count() {
   return n;
 }
 
+template <bool F16>
+static int launch_wide(int bits, const void* qkv, void* q_to, float* q_factor, const float* inv_freq, void* k_pool, void* v_pool,
+                       void* k_scale, void* v_scale, const int* block_table, const int* slot_ids, const int* q_start,
+                       const int* base_len, int N, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages, int n_pages,
+                       int write_kv, int* status, void* stream) {
+  const int per_block = 128 / (D / 16);             // few tokens: the heads of one token go to several blocks
+  const int most = (Hq + 2 * Hkv + per_block - 1) / per_block, split = N >= 296 ? 1 : min(most, (296 + N - 1) / N);
+  const int blocks = min(N, 5 * sm_count());
+  auto go = [&](auto kernel) {
+    return (int)launch_kernel(kernel, dim3(blocks, split), dim3(128), 0, (cudaStream_t)stream, (const __nv_bfloat16*)qkv, q_to,
+                              q_factor, inv_freq, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
+                              q_start, base_len, N, B, Hq, Hkv, page_tokens, max_pages, n_pages, write_kv, status);
+  };
+  if (bits == 8) return D == 64 ? go(rope_quantize_wide_kernel<64, 8, F16>) : go(rope_quantize_wide_kernel<128, 8, F16>);
+  return D == 64 ? go(rope_quantize_wide_kernel<64, 4, F16>) : go(rope_quantize_wide_kernel<128, 4, F16>);
+}
+
 // qkv [N, (Hq + 2 Hkv) D] (not changed unless q_out == qkv); q_out: the same layout, its query part is
 // written (rotated).  Pools and scales as at the top of the file.
 extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* q_out, const float* inv_freq,
@@ -445,19 +483,9 @@ extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* 
       rotary_dim % 2 != 0 || page_tokens <= 0)
     return (int)cudaErrorInvalidValue;
   if (is_bf16 && (D == 64 || D == 128) && (inv_freq == nullptr || (rotary_dim == D && !interleaved)) &&
-      (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0) {
-    const int per_block = 128 / (D / 16);           // few tokens: the heads of one token go to several blocks
-    const int most = (Hq + 2 * Hkv + per_block - 1) / per_block, split = N >= 296 ? 1 : min(most, (296 + N - 1) / N);
-    const int blocks = min(N, 5 * sm_count());
-    auto wide = [&](auto kernel) {
-      return (int)launch_kernel(kernel, dim3(blocks, split), dim3(128), 0, (cudaStream_t)stream, (const __nv_bfloat16*)qkv,
-                                (__nv_bfloat16*)q_out, inv_freq, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale,
-                                block_table, slot_ids, q_start, base_len, N, B, Hq, Hkv, page_tokens, max_pages, n_pages,
-                                write_kv, status);
-    };
-    if (bits == 8) return D == 64 ? wide(rope_quantize_wide_kernel<64, 8>) : wide(rope_quantize_wide_kernel<128, 8>);
-    return D == 64 ? wide(rope_quantize_wide_kernel<64, 4>) : wide(rope_quantize_wide_kernel<128, 4>);
-  }
+      (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0)
+    return launch_wide<false>(bits, qkv, q_out, nullptr, inv_freq, k_pool, v_pool, k_scale, v_scale, block_table, slot_ids, q_start,
+                              base_len, N, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, write_kv, status, stream);
   // few tokens: the heads of one token go to several blocks
   const int parts = N >= 592 ? 1 : min((Hq + 2 * Hkv + 3) / 4, (592 + N - 1) / N);
   auto go = [&](auto kernel, auto* typed) {
@@ -472,6 +500,20 @@ extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* 
                      : go(rope_quantize_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr);
   return bits == 8 ? go(rope_quantize_kernel<float, 8>, (float*)nullptr)
                    : go(rope_quantize_kernel<float, 4>, (float*)nullptr);
+}
+
+// The same for bfloat16, head_dim 64 or 128 and whole-head rotation (or none), with the queries as float16:
+// q16 [N, Hq, D], q_factor [N, Hq].
+extern "C" int siar_rope_quantize_q16(int bits, const void* qkv, void* q16, float* q_factor, const float* inv_freq, void* k_pool,
+                                      void* v_pool, void* k_scale, void* v_scale, const int* block_table, const int* slot_ids,
+                                      const int* q_start, const int* base_len, int N, int B, int Hq, int Hkv, int D, int page_tokens,
+                                      int max_pages, int n_pages, int write_kv, int* status, void* stream) {
+  if (N == 0) return 0;
+  if ((bits != 8 && bits != 4) || (D != 64 && D != 128) || page_tokens <= 0 ||
+      (((uintptr_t)qkv | (uintptr_t)q16 | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0)
+    return (int)cudaErrorInvalidValue;
+  return launch_wide<true>(bits, qkv, q16, q_factor, inv_freq, k_pool, v_pool, k_scale, v_scale, block_table, slot_ids, q_start,
+                           base_len, N, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, write_kv, status, stream);
 }
 
 // The keys and values of a batch as pages of the compute type; see read_kv_kernel.  out_table

@@ -37,7 +37,7 @@ EXTRA_FLAGS = os.environ.get("SIAR_NVCC_FLAGS", "").split()
 
 #: every unit of the library, in the order ``build_all`` compiles them
 ALL_UNITS = ("elementwise", "gemm_simt", "attention", "attention_mma", "attention_tc", "sampling", "kv_quant", "attention_quant",
-             "gemm_tc")
+             "attention_quant_tc", "gemm_tc")
 
 
 class ExtensionError(RuntimeError):

@@ -196,6 +196,70 @@ def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fus
     return out
 
 
+def works_on_tiles(kv, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                   window: Optional[int] = None, options: KernelOptions = DEFAULT) -> bool:
+    """True when prompts' attention over this entry runs on float16 tiles on the tensor cores (bfloat16, head_dim 64
+    or 128, at most 128 query heads per kv head, pages of a multiple of 64, no window); else the cache is read back
+    for the kernels of an ordinary cache."""
+    return (dtype == torch.bfloat16 and window is None and head_dim in (64, 128) and n_heads // n_kv_heads <= 128
+            and kv.page_tokens % 64 == 0 and scale > 0 and options.use_tc_attention and options.use_mma_attention)
+
+
+def key_parts(blocks: int, longest: int, average: float, row_floats: int, sms: int) -> int:
+    """Into how many parts the keys of a block of 256 rows are cut, for ``blocks`` of them of up to ``longest`` key
+    tiles: a tile takes a block 1.3 us and a block 6 us besides (B200, 128 dims); blocks run one to an SM; parts are
+    written and read once more as float32 (``row_floats`` of them a part) by a kernel of its own."""
+    best, best_cost = 1, None
+    for parts in range(1, min(16, longest) + 1):
+        one, mean = 6.0 + 1.3 * -(-longest // parts), 6.0 + 1.3 * average / parts
+        total = blocks * parts * mean / sms
+        cost = max(one, min(-(-blocks * parts // sms) * one, total + 0.5 * mean))
+        if parts > 1:
+            cost += 3.0 + parts * row_floats * 8 / 4e6
+        if best_cost is None or cost < best_cost:
+            best, best_cost = parts, cost
+    return best
+
+
+def _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv) -> torch.Tensor:
+    """Rotates (``inv_freq``) and stores (``write_kv``) the new tokens, widens the batch's cache to float16 tiles and
+    attends on those."""
+    device, index, n = qkv.device, qkv.device.index, qkv.shape[0]
+    k, table, heads = kv.k, kv.block_table, (n_heads, n_kv_heads, head_dim)
+    most = -(-min(meta.max_kv_len, table.shape[1] * kv.page_tokens) // 64)
+    if meta.base_lens is not None and meta.q_lens is not None:
+        tiles = sum(min(-(-(a + b) // 64), most) for a, b in zip(meta.base_lens, meta.q_lens))
+        q_lens = meta.q_lens
+    else:
+        tiles, q_lens = meta.n_seqs * most, [meta.max_q_len] * meta.n_seqs
+    sms, group = ops._sm_count(index), n_heads // n_kv_heads
+    block_rows = 2 * (128 // group * group)
+    blocks = n_kv_heads * sum(-(-m * group // block_rows) for m in q_lens)
+    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 4), sms)
+    empty = lambda shape, dt: torch.empty(shape, dtype=dt, device=device)  # noqa: E731
+    with ops._on_device(qkv):
+        stream, status = ops._stream(), ops._ptr(ops.status_word(device))
+        out = empty((n, n_heads * head_dim), torch.bfloat16)
+        q16, factor = empty((n, n_heads, head_dim), torch.float16), empty((n, n_heads), torch.float32)
+        wide = empty((2, tiles, n_kv_heads, 64, head_dim), torch.float16)
+        k16, v16 = wide.data_ptr(), wide.data_ptr() + wide.numel()
+        info = empty(tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), torch.uint8)
+        seq = empty((meta.n_seqs, 2), torch.int32)
+        scratch = empty(n * n_heads * splits * (head_dim + 4), torch.float32) if splits > 1 else None
+        pools = (ops._ptr(k), ops._ptr(kv.v), ops._ptr(kv.k_scale), ops._ptr(kv.v_scale), ops._ptr(table), *_batch(meta))
+        ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, ops._ptr(qkv), ops._ptr(q16), ops._ptr(factor),
+                    ops._ptr(inv_freq), *pools, n, meta.n_seqs, *heads, kv.page_tokens, table.shape[1], k.shape[0],
+                    int(write_kv), status, stream)
+        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, k16, v16, ops._ptr(info), ops._ptr(seq),
+                    meta.n_seqs, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], tiles, meta.max_kv_len,
+                    status, stream)
+        ops._launch("attention_quant_tc", "siar_attn_quant_tc", ops._ptr(q16), ops._ptr(factor), k16, v16, ops._ptr(info),
+                    ops._ptr(seq), ops._ptr(meta.q_start), ops._ptr(meta.base_len), ops._ptr(out), ops._ptr(scratch), n,
+                    meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
+                    kernels=2 if splits > 1 else 1)
+    return out
+
+
 def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
               window: Optional[int] = None, options: KernelOptions = DEFAULT) -> torch.Tensor:
     check_window(window)
@@ -205,6 +269,8 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     ops._check_if_asked(options, kv, meta, qkv.shape[0], False, window)
     if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
         return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, False)
+    if not meta.is_decode and works_on_tiles(kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
+        return _on_tiles(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False)
     pages, slots = _read(kv, meta, qkv.dtype, window)
     of_batch = copy.copy(meta)
     of_batch.slot_ids = slots
@@ -221,13 +287,19 @@ def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_h
     check_window(window)
     inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
     plain_layout = inv_freq is None or (rotary_dim == head_dim and not interleaved)
-    if meta.is_decode and plain_layout and options.fuse_decode_rope and works_on_codes(
-            kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
-        check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
+    check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
+    codes = works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options)
+    whole = None                            # a path that rotates and stores as well
+    if plain_layout and meta.is_decode and codes and options.fuse_decode_rope:
+        whole = lambda: _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, True, write_kv)  # noqa: E731
+    elif plain_layout and not meta.is_decode and not codes and works_on_tiles(
+            kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
+        whole = lambda: _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv)  # noqa: E731
+    if whole is not None:
         check_entry(kv, n_kv_heads, head_dim, qkv.device)
         ops._need_cuda(qkv, inv_freq)
         ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
-        return _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, True, write_kv)
+        return whole()
     q = torch.empty_like(qkv)               # the rotated queries; qkv stays as it is
     rope_kv_write(qkv, rotary, kv, meta, n_heads, n_kv_heads, head_dim, write_kv=write_kv, options=options, q_out=q)
     return attention(q, kv, meta, n_heads, n_kv_heads, head_dim, scale, window=window, options=options)

@@ -78,6 +78,11 @@ _signatures = {
         "siar_rope_quantize": [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int],
+        # bits, qkv, q16, q_factor, inv_freq, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len,
+        # N, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, write_kv, status, stream
+        "siar_rope_quantize_q16": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_int, c_void_p, c_void_p],
         # is_bf16, bits, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, k_out, v_out, out_table,
         # out_slots, B, Hkv, D, page_tokens, max_pages, n_pages, pages_out, max_kv_len, window, status, stream
         "siar_read_kv": [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -94,6 +99,18 @@ _signatures = {
         "siar_attn_quant_counters": [c_int],
         "siar_attn_quant_scratch_floats": [c_int],
         "siar_capture_id": [c_void_p],
+    },
+    "attention_quant_tc": {
+        # bits, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, k_out, v_out, tiles, seq_tiles, B, Hkv, D,
+        # page_tokens, max_pages, n_pages, tiles_out, max_kv_len, status, stream
+        "siar_widen_tiles": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                             c_void_p],
+        # q, q_factor, k_tiles, v_tiles, tiles, seq_tiles, q_start, base_len, out, scratch, N, B, Hq, Hkv, D, tiles_out,
+        # max_q_len, splits, scale, status, stream
+        "siar_attn_quant_tc": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+        "siar_attn_quant_tc_tile_info_bytes": [],
     },
     "sampling": {
         "siar_sample": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,

@@ -288,3 +288,67 @@ def test_command_line_takes_the_cache_format(capsys):
         assert inference.main(["--model", "tiny-a", "--random-weights", "--prompt-len", "9", "--max-new-tokens", "4",
                                "--temperature", "0", "--kv-cache", fmt]) == 0
     assert "new_tokens" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 1, 128), (4, 2, 64), (128, 1, 64)])
+def test_a_chunk_against_a_long_cache_is_cut_into_parts(bits, heads, kv_heads, dim):
+    from simple_inference_autoresearch_b200.kernels import kv_quant
+    held, new = ([1700, 3], [70, 90]) if heads < 100 else ([700], [9])
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=7)
+    assert kv_quant.key_parts(kv_heads, 28, 20.0, b.tokens * heads * (dim + 4), 148) > 1
+    kv, inv = b.entry(DEV), freqs(dim)
+    out = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV), *b.sizes(), dim ** -0.5)
+    ops.check_status(DEV)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), inv, want, b.meta(), *b.sizes())
+    pos = [c + i for c, n in zip(held, new) for i in range(n)]
+    check_attention(b, out, eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv), want, dim ** -0.5)
+    # the batch's lengths known on the device only, a launch sized for more, and other rotary layouts
+    again = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), b.entry(DEV), b.meta(DEV, host_lengths=False, max_kv_len=1900),
+                                   *b.sizes(), dim ** -0.5)
+    check_attention(b, again, eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv), want, dim ** -0.5)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("layout", ["partial", "interleaved"])
+def test_attention_behind_other_rotary_layouts(bits, layout):
+    for held, new in (([70, 3], [1, 1]), ([70, 3], [2, 3]), ([70, 3], [40, 75])):
+        b = eq.Batch(bits, 8, 2, 64, held, new, seed=3)
+        rotary = RotaryParams(freqs(32 if layout == "partial" else 64), 32 if layout == "partial" else 64, layout == "interleaved")
+        out = ops.rope_and_attention(b.qkv.to(DEV), on_device(rotary), b.entry(DEV), b.meta(DEV), *b.sizes(), 0.125)
+        want = b.entry()
+        eq.rope_kv_write(b.qkv.clone(), rotary, want, b.meta(), *b.sizes())
+        pos = [c + i for c, n in zip(held, new) for i in range(n)]
+        check_attention(b, out, eq.rotate(b.qkv.view(b.tokens, -1, 64)[:, :8].float(), pos, rotary), want, 0.125)
+    ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (4, 1, 128), (3, 1, 48)])
+@pytest.mark.parametrize("held,new", [([5, 30], [4, 3]), ([5, 90], [70, 40]), ([0, 63], [130, 1])])
+def test_numbers_that_are_none_reach_only_the_rows_that_see_them(bits, heads, kv_heads, dim, held, new):
+    """A key with an infinity and a value with a NaN among the new tokens: rows in front of them (the mask hides
+    them) are as without, rows behind are NaN: every dim for a bad key, the value's row (8 bits) or run of 64 dims
+    (4 bits) for a bad value."""
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=5)
+    x = b.qkv.view(b.tokens, heads + 2 * kv_heads, dim)
+    bad_v, bad_k = 1, int(b.q_start[1]) + new[1] - 1          # the first sequence's second token, the second's last
+    clean = b.qkv.clone()
+    x[bad_v, heads + kv_heads, 3] = float("nan")              # value of kv head 0
+    x[bad_k, heads + kv_heads - 1, 7] = float("inf")          # key of the last kv head
+    out = ops.rope_and_attention(b.qkv.to(DEV), None, b.entry(DEV), b.meta(DEV), *b.sizes(), 0.125).cpu().view(b.tokens, heads, dim)
+    ops.check_status(DEV)
+    group = heads // kv_heads
+    bad = torch.zeros(b.tokens, heads, dim, dtype=torch.bool)
+    bad[bad_v:new[0], :group, :dim if bits == 8 else 64] = True
+    bad[bad_k, heads - group:] = True
+    assert torch.equal(out.isnan(), bad)
+    b.qkv = clean
+    want = b.entry()
+    eq.rope_kv_write(clean.clone(), None, want, b.meta(), *b.sizes())
+    ref, bound, _ = eq.attention_bounds(b, clean.view(b.tokens, -1, dim)[:, :heads].float(), want, 0.125)
+    hidden = torch.ones(b.tokens, heads, dtype=torch.bool)    # rows that see neither
+    hidden[bad_v:new[0], :group] = False
+    hidden[bad_k, heads - group:] = False
+    assert bool(((out.double() - ref).abs() <= bound)[hidden].all())
