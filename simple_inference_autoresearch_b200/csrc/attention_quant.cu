@@ -31,12 +31,16 @@
 #include "kv_quant.cuh"
 #include "tcgen05.cuh"
 
+#include <cuda_fp16.h>
+
 #include <type_traits>
 
 namespace siar {
 
 struct QuantAttnParams {
   const __nv_bfloat16* qkv;      // [N, (Hq + 2 Hkv) D]
+  const __half* q16;             // or queries as float16 [N, Hq, D] times a power of two a row, q_factor [N, Hq]
+  const float* q_factor;
   uint8_t* k_pool;
   uint8_t* v_pool;
   void* k_scale;
@@ -271,9 +275,17 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     for (int j = 0; j < NT; ++j) {
       const int row = rt * C::kRows + 4 * j + warp;
       const bool in = row < s.q_len * G;
-      const __nv_bfloat16* src = P.qkv + (size_t)(s.t0 + (in ? row / G : 0)) * qkv_row + (size_t)(kvh * G + (in ? row % G : 0)) * D + lane;
+      const int token = s.t0 + (in ? row / G : 0), head = kvh * G + (in ? row % G : 0);
+      if (P.q16 != nullptr) {
+        const __half* src = P.q16 + ((size_t)token * P.Hq + head) * D + lane;
+        const float f = P.q_factor[(size_t)token * P.Hq + head];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) qa[j][i] = in ? __bfloat162float(src[32 * i]) : 0.f;
+        for (int i = 0; i < D / 32; ++i) qa[j][i] = in ? __half2float(src[32 * i]) * f : 0.f;
+      } else {
+        const __nv_bfloat16* src = P.qkv + (size_t)token * qkv_row + (size_t)head * D + lane;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) qa[j][i] = in ? __bfloat162float(src[32 * i]) : 0.f;
+      }
     }
     if (warp < 2 && has_new(s, t, left)) {
       const __nv_bfloat16* src = P.qkv + (size_t)s.t0 * qkv_row + (size_t)(P.Hq + warp * P.Hkv + kvh) * D + lane;
@@ -988,18 +1000,18 @@ extern "C" unsigned long long siar_capture_id(void* stream) {
 // Attention of the batch's new tokens over the quantised cache.  fused: one new token a sequence, whose
 // query and key are rotated here (inv_freq; nullptr: not rotated) and whose key and value are stored
 // (write_kv) and attended to; else the tokens' rows are in the cache and the queries are as they are to be
-// used.  counters: siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
-extern "C" int siar_attn_quant(int bits, const void* qkv, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+// used, in qkv or (q16 not nullptr; qkv is not read then) as siar_rope_quantize_q16 leaves them.  counters: siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
+extern "C" int siar_attn_quant(int bits, const void* qkv, const void* q16, const float* q_factor, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
                                const int* block_table, const int* slot_ids, const int* q_start, const int* base_len,
                                const float* inv_freq, void* out, int* counters, float* scratch, int B, int Hq, int Hkv, int D,
                                int page_tokens, int max_pages, int n_pages, int max_q_len, int max_kv_len, int sm_count,
                                int fused, int write_kv, float scale, int* status, void* stream) {
   if (B == 0 || max_q_len == 0) return 0;
   if (Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || page_tokens <= 0 || page_tokens % 64 != 0 || (bits != 8 && bits != 4) ||
-      n_pages <= 0 || max_pages <= 0 || max_kv_len <= 0 || sm_count <= 0 || (fused && max_q_len != 1) ||
+      n_pages <= 0 || max_pages <= 0 || max_kv_len <= 0 || sm_count <= 0 || (fused && (max_q_len != 1 || q16 != nullptr)) ||
       (long long)n_pages * Hkv * page_tokens >= (1ll << 31) || (long long)max_pages * page_tokens >= (1ll << 31))
     return (int)cudaErrorInvalidValue;
-  QuantAttnParams p = {(const __nv_bfloat16*)qkv, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
+  QuantAttnParams p = {(const __nv_bfloat16*)qkv, (const __half*)q16, q_factor, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
                        q_start, base_len, inv_freq, (__nv_bfloat16*)out, scratch, counters, status, B, Hq, Hkv, page_tokens,
                        max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused,
                        write_kv, scale * 1.4426950408889634f};

@@ -22,12 +22,14 @@
 namespace siar {
 
 constexpr int kRows = 128;       // rows per query tile
-constexpr int kQTiles = 2;       // query tiles per block
+constexpr int kQTiles = 1;       // query tiles per block
 constexpr int kKeys = 64;        // keys per tile
-constexpr int kStages = 3;       // K and V rings
+constexpr int kStages = 2;       // K and V rings
 constexpr int smem_bytes(int hd) { return kQTiles * kRows * hd * 2 + kStages * 2 * kKeys * hd * 2; }
-constexpr uint32_t kTmemCols = 512;                 // S[q][buf]: 64 columns each from 0; O[q]: 128 each from 256
+constexpr uint32_t kTmemCols = 256 * kQTiles;       // S[q][buf]: 64 columns each from 0; O[q]: head_dim each from kOColumn
+constexpr uint32_t kOColumn = 128 * kQTiles;
 constexpr float kHeadroom = 8.f, kRescaleGap = 7.f; // log2 of where p of the largest score starts, and of what it may grow by
+constexpr int kBlocksPerSM = 2 / kQTiles;
 constexpr int kThreads = 128 + kQTiles * 128;       // TMA warp, one MMA warp per query tile, a spare, the softmax warps
 
 // What the softmax has to know of a key tile and its value tile.
@@ -40,7 +42,7 @@ struct TileInfo {
 
 struct QuantTcParams {
   __nv_bfloat16* out;
-  float* scratch;                // parts of rows: [tokens x heads][splits][head_dim + 4]
+  float* scratch;                // parts of rows: [tokens x heads][splits][head_dim + 8]
   const TileInfo* tiles;         // [tiles][Hkv]
   const int* seq_tiles;          // [B]: the sequence's first tile, and how many it has
   const float* q_factor;         // [tokens][Hq]
@@ -55,6 +57,12 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 32 bytes, a whole sector, in one store (a thread owns a row: narrower stores leave sectors half written).
+__device__ __forceinline__ void store_sector(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
@@ -80,7 +88,7 @@ __host__ __device__ inline int key_tiles(int base, int q_len, int row0, int G, i
       : "memory")
 
 template <int kHd>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSM)
 attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const QuantTcParams prm) {
   extern __shared__ unsigned char smem_dyn[];
@@ -97,14 +105,15 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr int kTileBytes = kKeys * kHd * 2;        // 8 KiB per half
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.z, kvh = blockIdx.y;
+  // blocks with the most keys (the last rows, of all sequences and heads) start first: the tail of the grid is made
+  // of short blocks
+  const int part = blockIdx.x % prm.splits, kvh = blockIdx.x / prm.splits % prm.Hkv, b = blockIdx.x / prm.splits / prm.Hkv;
   const int G = prm.Hq / prm.Hkv;
   const int tile_rows = (kRows / G) * G;             // rows of a query tile in use: whole tokens only
   const int t0 = prm.q_start[b];
   const int q_len = prm.q_start[b + 1] - t0;
   const int rows_total = q_len * G;
-  // blocks with the most keys (the last rows) start first: the tail of the grid is made of short blocks
-  const int row0 = (gridDim.x / prm.splits - 1 - blockIdx.x / prm.splits) * (kQTiles * tile_rows);
+  const int row0 = (gridDim.y - 1 - blockIdx.y) * (kQTiles * tile_rows);
   if (row0 >= rows_total) return;
   const int base = prm.base_len[b];
   // both query tiles walk all the key tiles of the block (the first tile's last one may be masked entirely)
@@ -116,7 +125,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (rows_q[g] > 0) n_q = g + 1;
   }
   const int all_tiles = key_tiles(base, q_len, row0, G, tile_rows, prm.seq_tiles[2 * b + 1]);
-  const int parts = min(prm.splits, all_tiles), part = blockIdx.x % prm.splits;
+  const int parts = min(prm.splits, all_tiles);
   if (part >= parts) return;
   const int tile0 = all_tiles * part / parts, nt_max = all_tiles * (part + 1) / parts - tile0;
   const int seq_first = prm.seq_tiles[2 * b];        // the sequence's first tile of the widened cache
@@ -212,7 +221,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const uint32_t q_lo = (uint32_t)smem_desc_sw128(smem_u32(q_s + g * kQBytes));
       const uint32_t k_lo = (uint32_t)smem_desc_sw128(smem_u32(k_s));
       const uint32_t v_lo = (uint32_t)smem_desc_sw128_mn(smem_u32(v_s), kTileBytes / kHalves);
-      const uint32_t tmem_o = tmem_base + 256u + (uint32_t)(g * kHd);
+      const uint32_t tmem_o = tmem_base + kOColumn + (uint32_t)(g * kHd);
       // S[g][i & 1] = Q_g K_i^T over the two 64-dim halves, 4 steps of 16 dims (32 bytes) in each
       auto issue_qk = [&](int i) {
         const uint32_t ks = k_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
@@ -258,7 +267,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int quad = warp & 3;                 // the tensor-memory lanes this warp may touch
     const int row = quad * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t tmem_o = tmem_base + 256u + (uint32_t)(g * kHd) + lane_base;
+    const uint32_t tmem_o = tmem_base + kOColumn + (uint32_t)(g * kHd) + lane_base;
     const int rg = row0 + g * tile_rows + row;
     const bool mine = row < rows_q[g];
     const int kv_end = mine ? base + rg / G + 1 : 0;
@@ -360,7 +369,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const float nan = __int_as_float(0x7fc00000);
       const float inv = parts == 1 ? 1.f / l : 1.f;
       __nv_bfloat16* dst = prm.out + out_row * kHd;
-      float* partial = prm.scratch + (out_row * prm.splits + part) * (kHd + 4);      // (reference, sum), then the sums of values
+      float* partial = prm.scratch + (out_row * prm.splits + part) * (kHd + 8);      // (reference, sum), then the sums of values
 #pragma unroll 1
       for (int ch = 0; ch < kHd / 32; ++ch) {
         uint32_t o[32];
@@ -380,10 +389,12 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            __stcg(reinterpret_cast<float4*>(partial + 4 + ch * 32 + j),
-                   make_float4(__uint_as_float(o[j]) * f, __uint_as_float(o[j + 1]) * f, __uint_as_float(o[j + 2]) * f,
-                               __uint_as_float(o[j + 3]) * f));
+          for (int j = 0; j < 32; j += 8) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[j + e]) * f;
+            store_sector(partial + 8 + ch * 32 + j, v);
+          }
         }
       }
       if (mine && parts > 1) __stcg(reinterpret_cast<float2*>(partial), make_float2(m_used, l));
@@ -542,17 +553,17 @@ attn_quant_join_kernel(const float* scratch, __nv_bfloat16* out, const int* seq_
   const int rg = (t - t0) * G + head % G, block_rows = kQTiles * tile_rows;
   const int parts = min(splits, key_tiles(base_len[b], q_len, rg / block_rows * block_rows, G, tile_rows, seq_tiles[2 * b + 1]));
   if (parts < 2) return;
-  const float* part = scratch + (size_t)row * splits * (D + 4);
+  const float* part = scratch + (size_t)row * splits * (D + 8);
   float m = -INFINITY, l = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int p = 0; p < parts; ++p, part += D + 4) {
+  for (int p = 0; p < parts; ++p, part += D + 8) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(part));
     const float mx = fmaxf(m, ml.x), fa = m == mx ? 1.f : ex2(m - mx), fb = ml.x == mx ? 1.f : ex2(ml.x - mx);
     m = mx;
     l = l * fa + ml.y * fb;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * fa + __ldcg(part + 4 + i * 32 + lane) * fb;
+    for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * fa + __ldcg(part + 8 + i * 32 + lane) * fb;
   }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) out[(size_t)row * D + i * 32 + lane] = __float2bfloat16_rn(acc[i] / l);
@@ -628,7 +639,7 @@ extern "C" int siar_widen_tiles(int bits, const void* k_pool, const void* v_pool
   return D == 64 ? go(widen_tiles_kernel<64, 4>) : go(widen_tiles_kernel<128, 4>);
 }
 
-// q [N, Hq, D] float16 with q_factor [N, Hq]; out [N, Hq * D] bfloat16; scratch: with splits > 1 N * Hq * splits * (D + 4)
+// q [N, Hq, D] float16 with q_factor [N, Hq]; out [N, Hq * D] bfloat16; scratch: with splits > 1 N * Hq * splits * (D + 8)
 // floats.  splits: parts into which the keys of a block of rows are cut.
 extern "C" int siar_attn_quant_tc(const void* q, const float* q_factor, const void* k_tiles, const void* v_tiles, const void* tiles,
                                   const int* seq_tiles, const int* q_start, const int* base_len, void* out, float* scratch, int N, int B,
@@ -645,7 +656,9 @@ extern "C" int siar_attn_quant_tc(const void* q, const float* q_factor, const vo
   const QuantTcParams prm = {(__nv_bfloat16*)out, scratch, (const TileInfo*)tiles, seq_tiles, q_factor, q_start, base_len, status, Hq,
                              Hkv, splits, scale * 1.4426950408889634f};
   const int G = Hq / Hkv, block_rows = kQTiles * (kRows / G) * G;
-  const dim3 grid((max_q_len * G + block_rows - 1) / block_rows * splits, Hkv, B);
+  const long long across = (long long)splits * Hkv * B, down = (max_q_len * (long long)G + block_rows - 1) / block_rows;
+  if (across >= (1ll << 31) || down > 65535) return (int)cudaErrorInvalidValue;
+  const dim3 grid((unsigned)across, (unsigned)down);
   return D == 64 ? launch_tc<64>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream)
                  : launch_tc<128>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream);
 }

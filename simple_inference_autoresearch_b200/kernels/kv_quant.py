@@ -67,7 +67,12 @@ def check_window(window: Optional[int]) -> None:
 
 
 def _batch(meta):
-    return ops._ptr(meta.slot_ids), ops._ptr(meta.q_start), ops._ptr(meta.base_len)
+    return meta.slot_ids.data_ptr(), meta.q_start.data_ptr(), meta.base_len.data_ptr()
+
+
+def _entry(kv):
+    """What every kernel takes of a cache entry first."""
+    return (kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.block_table.data_ptr())
 
 
 def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -84,8 +89,7 @@ def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads:
     ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
     with ops._on_device(qkv):
         ops._launch("kv_quant", "siar_rope_quantize", ops._is_bf16(qkv.dtype), kv.bits, ops._ptr(qkv), ops._ptr(q_out),
-                    ops._ptr(inv_freq), ops._ptr(kv.k), ops._ptr(kv.v), ops._ptr(kv.k_scale), ops._ptr(kv.v_scale),
-                    ops._ptr(kv.block_table), *_batch(meta), qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
+                    ops._ptr(inv_freq), *_entry(kv), *_batch(meta), qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
                     kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], int(write_kv),
                     ops._ptr(ops.status_word(qkv.device)), ops._stream(), rotary_dim, int(interleaved))
 
@@ -109,9 +113,8 @@ def _read(kv, meta, dtype: torch.dtype, window: Optional[int]):
     cells = meta.n_seqs * kv.block_table.shape[1]
     table, slots = ints[:cells].view(meta.n_seqs, -1), ints[cells:]
     with ops._on_device(kv.k):
-        ops._launch("kv_quant", "siar_read_kv", ops._is_bf16(dtype), kv.bits, ops._ptr(kv.k), ops._ptr(kv.v),
-                    ops._ptr(kv.k_scale), ops._ptr(kv.v_scale), ops._ptr(kv.block_table), *_batch(meta), ops._ptr(k),
-                    ops._ptr(v), ops._ptr(table), ops._ptr(slots), meta.n_seqs, n_kv_heads, head_dim, page,
+        ops._launch("kv_quant", "siar_read_kv", ops._is_bf16(dtype), kv.bits, *_entry(kv), *_batch(meta), k.data_ptr(),
+                    v.data_ptr(), table.data_ptr(), slots.data_ptr(), meta.n_seqs, n_kv_heads, head_dim, page,
                     kv.block_table.shape[1], kv.k.shape[0], pages, meta.max_kv_len, int(window or 0),
                     ops._ptr(ops.status_word(device)), ops._stream())
     return KVEntry(k, v, table, page), slots
@@ -128,8 +131,10 @@ def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options:
     return _read(kv, meta, dtype, window)[0]
 
 
-#: query rows (new tokens x heads of a group) a sequence may bring to the kernel that works on the codes; a
-#: longer run reads the cache back once for the prompt kernel instead of walking the codes for every 16 rows
+#: query rows (new tokens x heads of a group) a sequence may bring to the kernel that works on the codes; a longer run
+#: widens the cache once for the tensor-core kernel instead of walking the codes for every 16 rows.  Measured on B200,
+#: four sequences of 4,000 held positions (8 bits, 32 heads on 8, 128 dims): 64 rows 33 us against 40, 256 rows 83
+#: against 54; one sequence of 500: 64 rows 19 us against 18
 MOST_ROWS = 64
 
 
@@ -179,20 +184,33 @@ def _new_workspace(index: int):
     return counters.data_ptr(), scratch.data_ptr(), counters, scratch
 
 
+def _queries16(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, write_kv):
+    """Rotates the queries into float16 rows with a factor each, and stores the new keys and values (``write_kv``)."""
+    n, table, device = qkv.shape[0], kv.block_table, qkv.device
+    q16 = torch.empty((n, n_heads, head_dim), dtype=torch.float16, device=device)
+    factor = torch.empty((n, n_heads), dtype=torch.float32, device=device)
+    ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, qkv.data_ptr(), q16.data_ptr(), factor.data_ptr(),
+                ops._ptr(inv_freq), *_entry(kv), *_batch(meta), n, meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens,
+                table.shape[1], kv.k.shape[0], int(write_kv), ops.status_word(device).data_ptr(), ops._stream())
+    return q16, factor
+
+
 def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
-    device = qkv.device
-    index = device.index
-    k, table = kv.k, kv.block_table
+    """``fused``: one token a sequence, rotated (``inv_freq``) and stored (``write_kv``) by the attention kernel itself;
+    else, where ``write_kv`` is not None, by a kernel in front."""
+    device, index, table = qkv.device, qkv.device.index, kv.block_table
     with ops._on_device(qkv):
+        q16 = factor = None
+        if not fused and write_kv is not None:
+            q16, factor = _queries16(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, write_kv)
         out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
-        stream = torch._C._cuda_getCurrentRawStream(index)
+        stream = ops._stream()
         counters, scratch = _workspace(index, stream)
-        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), k.data_ptr(), kv.v.data_ptr(),
-                    kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), table.data_ptr(), meta.slot_ids.data_ptr(),
-                    meta.q_start.data_ptr(), meta.base_len.data_ptr(), ops._ptr(inv_freq), out.data_ptr(), counters, scratch,
-                    meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], meta.max_q_len,
-                    meta.max_kv_len, ops._sm_count(index), int(fused), int(write_kv), float(scale),
-                    ops.status_word(device).data_ptr(), stream)
+        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), ops._ptr(q16), ops._ptr(factor), *_entry(kv),
+                    *_batch(meta), ops._ptr(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads,
+                    head_dim, kv.page_tokens, table.shape[1], kv.k.shape[0], meta.max_q_len, meta.max_kv_len,
+                    ops._sm_count(index), int(fused), int(bool(write_kv)), float(scale), ops.status_word(device).data_ptr(),
+                    stream)
     return out
 
 
@@ -206,16 +224,17 @@ def works_on_tiles(kv, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_d
 
 
 def key_parts(blocks: int, longest: int, average: float, row_floats: int, sms: int) -> int:
-    """Into how many parts the keys of a block of 256 rows are cut, for ``blocks`` of them of up to ``longest`` key
-    tiles: a tile takes a block 1.3 us and a block 6 us besides (B200, 128 dims); blocks run one to an SM; parts are
-    written and read once more as float32 (``row_floats`` of them a part) by a kernel of its own."""
+    """Into how many parts the keys of a block of 128 rows are cut, for ``blocks`` of them of up to ``longest``
+    (on average ``average``) key tiles.  Measured on B200 at 128 dims: a block alone on its SM takes 7 us and 0.95 us
+    a tile, two on every SM 0.66 us a tile and SM, a last round a third of a block more; parts (``row_floats`` floats each)
+    are written and read again at 3.6 TB/s by a kernel of its own.  A chunk of 128 tokens on 8,000 held (32 heads on 8): one
+    part 139 us, 8 parts 54; a prompt of 2,048: one part 69 us, two 109."""
     best, best_cost = 1, None
     for parts in range(1, min(16, longest) + 1):
-        one, mean = 6.0 + 1.3 * -(-longest // parts), 6.0 + 1.3 * average / parts
-        total = blocks * parts * mean / sms
-        cost = max(one, min(-(-blocks * parts // sms) * one, total + 0.5 * mean))
+        tiles = -(-longest // parts)
+        cost = max(7 + 0.95 * tiles, blocks * average * 0.66 / sms + 0.35 * (7 + 1.3 * tiles))
         if parts > 1:
-            cost += 3.0 + parts * row_floats * 8 / 4e6
+            cost += 4 + parts * row_floats * 8 / 3.6e6
         if best_cost is None or cost < best_cost:
             best, best_cost = parts, cost
     return best
@@ -233,28 +252,24 @@ def _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, wri
     else:
         tiles, q_lens = meta.n_seqs * most, [meta.max_q_len] * meta.n_seqs
     sms, group = ops._sm_count(index), n_heads // n_kv_heads
-    block_rows = 2 * (128 // group * group)
+    block_rows = 128 // group * group
     blocks = n_kv_heads * sum(-(-m * group // block_rows) for m in q_lens)
-    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 4), sms)
+    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 8), sms)
     empty = lambda shape, dt: torch.empty(shape, dtype=dt, device=device)  # noqa: E731
     with ops._on_device(qkv):
-        stream, status = ops._stream(), ops._ptr(ops.status_word(device))
+        stream, status = ops._stream(), ops.status_word(device).data_ptr()
+        q16, factor = _queries16(qkv, inv_freq, kv, meta, *heads, write_kv)
         out = empty((n, n_heads * head_dim), torch.bfloat16)
-        q16, factor = empty((n, n_heads, head_dim), torch.float16), empty((n, n_heads), torch.float32)
         wide = empty((2, tiles, n_kv_heads, 64, head_dim), torch.float16)
         k16, v16 = wide.data_ptr(), wide.data_ptr() + wide.numel()
         info = empty(tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), torch.uint8)
         seq = empty((meta.n_seqs, 2), torch.int32)
-        scratch = empty(n * n_heads * splits * (head_dim + 4), torch.float32) if splits > 1 else None
-        pools = (ops._ptr(k), ops._ptr(kv.v), ops._ptr(kv.k_scale), ops._ptr(kv.v_scale), ops._ptr(table), *_batch(meta))
-        ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, ops._ptr(qkv), ops._ptr(q16), ops._ptr(factor),
-                    ops._ptr(inv_freq), *pools, n, meta.n_seqs, *heads, kv.page_tokens, table.shape[1], k.shape[0],
-                    int(write_kv), status, stream)
-        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, k16, v16, ops._ptr(info), ops._ptr(seq),
-                    meta.n_seqs, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], tiles, meta.max_kv_len,
-                    status, stream)
-        ops._launch("attention_quant_tc", "siar_attn_quant_tc", ops._ptr(q16), ops._ptr(factor), k16, v16, ops._ptr(info),
-                    ops._ptr(seq), ops._ptr(meta.q_start), ops._ptr(meta.base_len), ops._ptr(out), ops._ptr(scratch), n,
+        scratch = empty(n * n_heads * splits * (head_dim + 8), torch.float32) if splits > 1 else None
+        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *_entry(kv), *_batch(meta), k16, v16, info.data_ptr(),
+                    seq.data_ptr(), meta.n_seqs, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], tiles,
+                    meta.max_kv_len, status, stream)
+        ops._launch("attention_quant_tc", "siar_attn_quant_tc", q16.data_ptr(), factor.data_ptr(), k16, v16, info.data_ptr(),
+                    seq.data_ptr(), meta.q_start.data_ptr(), meta.base_len.data_ptr(), out.data_ptr(), ops._ptr(scratch), n,
                     meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
                     kernels=2 if splits > 1 else 1)
     return out
@@ -268,7 +283,7 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], False, window)
     if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
-        return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, False)
+        return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, None)
     if not meta.is_decode and works_on_tiles(kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
         return _on_tiles(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False)
     pages, slots = _read(kv, meta, qkv.dtype, window)
@@ -290,9 +305,10 @@ def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_h
     check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
     codes = works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options)
     whole = None                            # a path that rotates and stores as well
-    if plain_layout and meta.is_decode and codes and options.fuse_decode_rope:
-        whole = lambda: _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, True, write_kv)  # noqa: E731
-    elif plain_layout and not meta.is_decode and not codes and works_on_tiles(
+    if plain_layout and codes:
+        fused = meta.is_decode and options.fuse_decode_rope
+        whole = lambda: _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv)  # noqa: E731
+    elif plain_layout and not meta.is_decode and works_on_tiles(
             kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
         whole = lambda: _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv)  # noqa: E731
     if whole is not None:

@@ -90,10 +90,10 @@ _signatures = {
                          c_int, c_int, c_void_p, c_void_p],
     },
     "attention_quant": {
-        # bits, qkv, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
+        # bits, qkv, q16, q_factor, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
         # B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, max_kv_len, sm_count, fused, write_kv, scale, status,
         # stream
-        "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
         "siar_attn_quant_counters": [c_int],

@@ -296,7 +296,7 @@ def test_a_chunk_against_a_long_cache_is_cut_into_parts(bits, heads, kv_heads, d
     from simple_inference_autoresearch_b200.kernels import kv_quant
     held, new = ([1700, 3], [70, 90]) if heads < 100 else ([700], [9])
     b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=7)
-    assert kv_quant.key_parts(kv_heads, 28, 20.0, b.tokens * heads * (dim + 4), 148) > 1
+    assert kv_quant.key_parts(kv_heads, 28, 20.0, b.tokens * heads * (dim + 8), 148) > 1
     kv, inv = b.entry(DEV), freqs(dim)
     out = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV), *b.sizes(), dim ** -0.5)
     ops.check_status(DEV)
