@@ -126,6 +126,13 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t off) {
   return off ^ (((off >> 7) & (ROW / 16 - 1)) << 4);
 }
 
+// ceil(steps / chunk) for steps below 2^24: the float quotient is off by at most one.
+__device__ __forceinline__ int chunks_of(int steps, int chunk) {
+  int q = (int)__fdividef((float)(steps + chunk - 1), (float)chunk);
+  q -= q * chunk > steps + chunk - 1;
+  return q + ((q + 1) * chunk <= steps + chunk - 1);
+}
+
 // One sequence's units: (row tile, kv head), all of T block steps.
 struct QuantSeq {
   int b, base, t0, q_len, slot, len, T, row_tiles;
@@ -172,24 +179,27 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     s.slot = P.slot_ids[b];
     s.len = min(s.base + s.q_len, cap);
     past_table |= s.base + s.q_len > cap;
-    s.T = (s.len + C::kBlockKeys - 1) / C::kBlockKeys;
-    s.row_tiles = (s.q_len * G + C::kRows - 1) / C::kRows;
+    s.T = max(0, (s.len + C::kBlockKeys - 1) / C::kBlockKeys);
+    s.row_tiles = max(0, (s.q_len * G + C::kRows - 1) / C::kRows);
     return s;
   };
   // ---- this block's share of all block steps
-  // Sums over all sequences, 32 a time; a sum beyond 2^31 is refused below, so a lane's part may stop at 2^26.
+  // Sums over all sequences, 32 a time (a lane keeps its first one); a sum of 2^26 or more is refused, so a lane's
+  // part may stop there.
+  QuantSeq own = {};
+  if (lane < P.B) own = load_seq(lane);
   auto total_of = [&](auto weight) {
-    long long mine = 0;
-    for (int b = lane; b < P.B; b += 32) mine += weight(load_seq(b));
+    long long mine = weight(own);
+    for (int b = lane + 32; b < P.B; b += 32) mine += weight(load_seq(b));
     return __reduce_add_sync(0xffffffffu, (unsigned)min(mine, 1ll << 26));
   };
-  const unsigned sum = total_of([&](const QuantSeq& s) { return (long long)s.T * s.row_tiles * P.Hkv; });
+  const unsigned sum = total_of([&](const QuantSeq& s) { return (long long)s.T * (s.row_tiles * P.Hkv); });
   if (sum >= 1u << 26) {
     if (threadIdx.x == 0) atomicOr(P.status, kStatusLengthPastGrid);
     return;
   }
   const int total = (int)sum;
-  const unsigned units = total_of([&](const QuantSeq& s) { return s.T > 0 ? (long long)s.row_tiles * P.Hkv : 0ll; });
+  const unsigned units = total_of([&](const QuantSeq& s) { return s.T > 0 ? (long long)(s.row_tiles * P.Hkv) : 0ll; });
   // at least one step a block: a block without one would be waited for by the join of a unit around it
   int nb = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= nb) return;
@@ -201,7 +211,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   int chunk = each + (odd > 0);
   bool by_unit = false;
   for (const int most = chunk + kCrossing; chunk <= most && units <= gridDim.x; ++chunk) {
-    const unsigned need = total_of([&](const QuantSeq& s) { return (long long)((s.T + chunk - 1) / chunk) * s.row_tiles * P.Hkv; });
+    const unsigned need = total_of([&](const QuantSeq& s) { return (long long)chunks_of(s.T, chunk) * (s.row_tiles * P.Hkv); });
     by_unit = need <= gridDim.x;
     if (by_unit) {
       nb = (int)need;
@@ -209,7 +219,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     }
   }
   if ((int)blockIdx.x >= nb) return;
-  auto parts_of = [&](const QuantSeq& s) { return by_unit ? (s.T + chunk - 1) / chunk : s.T; };   // blocks, or steps, of a unit
+  auto parts_of = [&](const QuantSeq& s) { return by_unit ? chunks_of(s.T, chunk) : s.T; };   // blocks, or steps, of a unit
   auto begin_of = [&](int i) { return i * each + min(i, odd); };
   auto block_of = [&](int step) { return step < odd * (each + 1) ? step / (each + 1) : odd + (step - odd * (each + 1)) / each; };
   const int start = by_unit ? blockIdx.x : begin_of(blockIdx.x);
@@ -222,7 +232,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     while (true) {                                // 32 sequences at a time
       int mine = 0;
       if (b0 + lane < P.B) {
-        const QuantSeq s = load_seq(b0 + lane);
+        const QuantSeq s = b0 == 0 ? own : load_seq(b0 + lane);
         mine = parts_of(s) * s.row_tiles * P.Hkv;
       }
       int incl = mine;
