@@ -326,7 +326,7 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
 // ------------------------------------------------------------------ read back
 // Sequence b's pages go, in order, behind those of the sequences before it: page p of sequence b is
 // page first(b) + p of the output pools [pages][Hkv][page_tokens][D]; row b of `out_table` names them
-// (-1 beyond), `out_slots[b]` = b.  Rows behind a sequence's last token are zeros.  Pages that lie
+// (-1 beyond), `out_slots[b]` = b (nullptr: not written).  Rows behind a sequence's last token are zeros.  Pages that lie
 // wholly in front of every query's window (first_key of the batch's first new token) are not read.
 // grid (pages of the longest sequence, Hkv, B), 256 threads, 16 codes a thread and step.
 template <typename T, int BITS>
@@ -358,7 +358,7 @@ read_kv_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale
     for (int i = threadIdx.x; i < max_pages; i += blockDim.x)
       out_table[(size_t)b * max_pages + i] = i >= unseen && i < mine && first + i < pages_out ? first + i : -1;
     if (threadIdx.x == 0) {
-      out_slots[b] = b;
+      if (out_slots != nullptr) out_slots[b] = b;
       if ((total + page_tokens - 1) / page_tokens > most) atomicOr(status, kStatusLengthPastGrid);
     }
   }

@@ -94,8 +94,8 @@ def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads:
                     ops._ptr(ops.status_word(qkv.device)), ops._stream(), rotary_dim, int(interleaved))
 
 
-def _read(kv, meta, dtype: torch.dtype, window: Optional[int]):
-    """(KVEntry of the batch's keys and values, the batch's row of its block table per sequence)."""
+def _read(kv, meta, dtype: torch.dtype, window: Optional[int], with_slots: bool = False):
+    """(KVEntry of the batch's keys and values, the row of its block table per sequence)."""
     from ..cache.sequence_cache import KVEntry
 
     device = kv.k.device
@@ -109,12 +109,11 @@ def _read(kv, meta, dtype: torch.dtype, window: Optional[int]):
         pages = meta.n_seqs * most
     k = torch.empty((pages, n_kv_heads, page, head_dim), dtype=dtype, device=device)
     v = torch.empty_like(k)
-    ints = torch.empty((meta.n_seqs, kv.block_table.shape[1] + 1), dtype=torch.int32, device=device).view(-1)
-    cells = meta.n_seqs * kv.block_table.shape[1]
-    table, slots = ints[:cells].view(meta.n_seqs, -1), ints[cells:]
+    table = torch.empty((meta.n_seqs, kv.block_table.shape[1]), dtype=torch.int32, device=device)
+    slots = torch.empty(meta.n_seqs, dtype=torch.int32, device=device) if with_slots else None
     with ops._on_device(kv.k):
         ops._launch("kv_quant", "siar_read_kv", ops._is_bf16(dtype), kv.bits, *_entry(kv), *_batch(meta), k.data_ptr(),
-                    v.data_ptr(), table.data_ptr(), slots.data_ptr(), meta.n_seqs, n_kv_heads, head_dim, page,
+                    v.data_ptr(), table.data_ptr(), ops._ptr(slots), meta.n_seqs, n_kv_heads, head_dim, page,
                     kv.block_table.shape[1], kv.k.shape[0], pages, meta.max_kv_len, int(window or 0),
                     ops._ptr(ops.status_word(device)), ops._stream())
     return KVEntry(k, v, table, page), slots
@@ -138,15 +137,16 @@ def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options:
 MOST_ROWS = 64
 
 
-def works_on_codes(kv, meta, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int,
+def works_on_codes(kv, meta, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                    window: Optional[int] = None, options: KernelOptions = DEFAULT) -> bool:
     """True when attention over this entry runs on the codes themselves (bfloat16, head_dim 64 or 128, pages of
-    a multiple of 64, no window, single tokens or short runs); else the cache is read back first."""
+    a multiple of 64, no window): single tokens, short runs, and whatever ``works_on_tiles`` does not take."""
     if dtype != torch.bfloat16 or window is not None or head_dim not in (64, 128) or not options.use_mma_attention:
         return False
-    if not meta.is_decode and meta.max_q_len * (n_heads // n_kv_heads) > MOST_ROWS:
+    if kv.page_tokens % 64 or kv.k.shape[0] * n_kv_heads * kv.page_tokens >= 1 << 31:
         return False
-    return kv.page_tokens % 64 == 0 and kv.k.shape[0] * n_kv_heads * kv.page_tokens < 1 << 31
+    return meta.is_decode or meta.max_q_len * (n_heads // n_kv_heads) <= MOST_ROWS or not works_on_tiles(
+        kv, dtype, n_heads, n_kv_heads, head_dim, scale, window, options)
 
 
 _workspaces, _captured_workspaces = {}, {}
@@ -282,11 +282,11 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     check_entry(kv, n_kv_heads, head_dim, qkv.device)
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], False, window)
-    if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options):
+    if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
         return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, None)
     if not meta.is_decode and works_on_tiles(kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
         return _on_tiles(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False)
-    pages, slots = _read(kv, meta, qkv.dtype, window)
+    pages, slots = _read(kv, meta, qkv.dtype, window, with_slots=True)
     of_batch = copy.copy(meta)
     of_batch.slot_ids = slots
     if meta.is_decode and not ops._fn("attention", "siar_attn_decode_fits")(
@@ -303,7 +303,7 @@ def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_h
     inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
     plain_layout = inv_freq is None or (rotary_dim == head_dim and not interleaved)
     check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
-    codes = works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, window, options)
+    codes = works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options)
     whole = None                            # a path that rotates and stores as well
     if plain_layout and codes:
         fused = meta.is_decode and options.fuse_decode_rope

@@ -213,7 +213,7 @@ def attention_bounds(batch, q, kv, scale, window=None):
             terms = q[t0 + i].double()[None] * kk
             s = terms.sum(-1) * scale                                   # [keys, heads]
             p = torch.softmax(s, 0)
-            dmax = (2 * u * scale * terms.abs().sum(-1)).amax(0)        # [heads]
+            dmax = (2 * u * abs(scale) * terms.abs().sum(-1)).amax(0)        # [heads]
             o = (p[..., None] * vv).sum(0)
             pv = (p[..., None] * vv.abs()).sum(0)
             small = 2.0 ** -12 if batch.qkv.dtype == torch.float32 else 0.0

@@ -352,3 +352,250 @@ def test_numbers_that_are_none_reach_only_the_rows_that_see_them(bits, heads, kv
     hidden[bad_v:new[0], :group] = False
     hidden[bad_k, heads - group:] = False
     assert bool(((out.double() - ref).abs() <= bound)[hidden].all())
+
+
+def attend(b, device_kv, *, scale, meta=None, **kw):
+    return ops.rope_and_attention(b.qkv.to(DEV), None, device_kv, meta or b.meta(DEV), *b.sizes(), scale, **kw)
+
+
+def plain_of(b):
+    """The entry with the batch's new tokens stored, and the queries, for a batch without rotation."""
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), None, want, b.meta(), *b.sizes())
+    return want, b.qkv.view(b.tokens, -1, b.dim)[:, :b.heads].float()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("page", [128, 192])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 1], [90, 5, 200]])
+def test_pages_of_other_sizes(bits, page, new):
+    b = eq.Batch(bits, 8, 2, 64, [0, 300, 191], new, seed=page, page=page)
+    out = attend(b, b.entry(DEV), scale=0.125)
+    ops.check_status(DEV)
+    want, q = plain_of(b)
+    check_attention(b, out, q, want, 0.125)
+    got = ops.read_kv(b.entry(DEV), b.meta(DEV), torch.float32)
+    assert got.page_tokens == page and got.k.shape[2] == page
+    ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (4, 2, 128), (3, 1, 32)])
+@pytest.mark.parametrize("kind", ["decode", "run", "chunk"])
+def test_more_sequences_than_a_warp_has_lanes(bits, heads, kv_heads, dim, kind):
+    g = torch.Generator().manual_seed(11)
+    held = torch.randint(0, 200, (75,), generator=g).tolist()
+    new = [1] * 75 if kind == "decode" else torch.randint(1, 4 if kind == "run" else 12, (75,), generator=g).tolist()
+    if kind == "chunk":
+        new[40] = 130
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=1, stale="random")
+    out = attend(b, b.entry(DEV), scale=dim ** -0.5)
+    ops.check_status(DEV)
+    want, q = plain_of(b)
+    check_attention(b, out, q, want, dim ** -0.5)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 3, 70])
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_any_scale(bits, new, scale):
+    b = eq.Batch(bits, 8, 2, 64, [130, 7], [new, 1], seed=8)
+    out = attend(b, b.entry(DEV), scale=scale)
+    want, q = plain_of(b)
+    check_attention(b, out, q, want, scale)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 40])
+@pytest.mark.parametrize("tall", [3, 200])
+def test_a_dominant_key_without_a_value(bits, new, tall):
+    """Scores of 30 (base e) for key ``tall`` with a value of zeros, 0 for all others with values of 1: the result is
+    n e^-30 / (1 + n e^-30), far below the reference that the scores alone would set.  Every number is its code times a
+    power of two, so only p (16 bits of the largest of a step, all equal here), the exponential (2^-21 at 30 log2 e,
+    whose own rounding is 2^-19 there) and the result (2^-9) round.  Runs of more than 64 rows go over float16 tiles,
+    where p is a float16 that starts 2^8 below the largest score's: what is under 2^-24 of that, 2^-32 of the largest,
+    is lost, at most 2^-32 a key of values of 1."""
+    dim, held = 64, 300
+    b = eq.Batch(bits, 2, 1, dim, [held], [new], seed=0, stale="random")
+    x = b.qkv.view(new, 4, dim)
+    x.zero_()
+    x[:, :2, 0] = 1.0
+    x[:, 3] = 1.0                                             # new values; new keys are zeros
+    k = torch.zeros(b.kv.k.shape[0], 1, 64, dim)
+    v = torch.ones_like(k)
+    page, at = int(b.kv.block_table[int(b.slot_ids[0]), tall // 64]), tall % 64
+    k[page, 0, at, 0] = 15.0 * 16
+    k[page, 0, at, 1] = -15.0 * 16                            # (4 bits: the run's range is a multiple of 15)
+    v[page, 0, at] = 0.0
+    b.kv.k, b.kv.k_scale = eq.quantise(k, bits)
+    b.kv.v, b.kv.v_scale = eq.quantise(v, bits)
+    top = float(eq.values(b.kv.k, b.kv.k_scale)[page, 0, at, 0])
+    scale = 30.0 / top
+    out = attend(b, b.entry(DEV), scale=scale).cpu().double().view(new, 2, dim)
+    ops.check_status(DEV)
+    for i in range(new):
+        n = held + i
+        want = n * math.exp(-30.0) / (1 + n * math.exp(-30.0))
+        lost = n * 2.0 ** -32 if new * 2 > 64 else 0.0
+        assert bool(((out[i] - want).abs() <= want * (2 ** -9 + 2 ** -15 + 2 ** -18) + lost).all()), out[i, 0, :3]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 40])
+def test_values_of_very_unequal_rows(bits, new):
+    """Rows of values from 2^-40 to 2^40 of one another and rows of zeros; where every value is zero the result is."""
+    b = eq.Batch(bits, 4, 2, 128, [200, 66], [new, 1], seed=6)
+    powers = torch.randint(-40, 41, b.kv.v_scale.shape[:3], generator=torch.Generator().manual_seed(1)).float().exp2()
+    powers[powers < 2.0 ** -30] = 0.0
+    s = b.kv.v_scale
+    b.kv.v_scale = (s.float() * (powers if bits == 8 else powers[..., None, None])).to(s.dtype)
+    out = attend(b, b.entry(DEV), scale=0.05)
+    want, q = plain_of(b)
+    check_attention(b, out, q, want, 0.05)
+    b.kv.v_scale = torch.zeros_like(s)
+    b.qkv.view(b.tokens, 8, 128)[:, 6:] = 0.0
+    assert not attend(b, b.entry(DEV), scale=0.05).any()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_results_are_the_same_every_time_on_any_stream(bits, new):
+    b = eq.Batch(bits, 8, 2, 128, [3000, 17, 900], [new, 1, 2 if new > 1 else 1], seed=4)
+    kv = b.entry(DEV)
+    first = attend(b, kv, scale=0.09)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(12):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            again = attend(b, kv, scale=0.09)
+            assert torch.equal(again, first)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_two_captured_graphs_run_side_by_side(bits, new):
+    """Captured on one stream, replayed on two at once, an eager call beside them: no workspace is shared."""
+    batches = [eq.Batch(bits, 8, 2, 128, [4000 + 600 * i, 70], [new, 1], seed=20 + i) for i in range(3)]
+    state = [(b.qkv.to(DEV), b.entry(DEV), b.meta(DEV), b.sizes()) for b in batches]
+    call = lambda s: ops.rope_and_attention(s[0], None, s[1], s[2], *s[3], 0.09)  # noqa: E731
+    want = [call(s) for s in state]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in state[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([call(s) for _ in range(3)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = call(state[2])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[2])
+        for got, w in zip(outs, want):
+            assert all(torch.equal(o, w) for o in got)
+    ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dim", [128, 48])
+def test_a_captured_step_replayed_while_the_sequences_grow(bits, dim):
+    """One capture, lengths advanced on the device by the graph itself, over page and step borders; as eager steps."""
+    steps = 9
+    b = eq.Batch(bits, 4, 2, dim, [60, 250, 0], [steps, steps, steps], seed=2, stale="nan")
+    g = torch.Generator().manual_seed(9)
+    rows = torch.randn(steps, 3, 8 * dim, generator=g).to(torch.bfloat16).to(DEV)
+    inv = freqs(dim).to(DEV)
+    from simple_inference_autoresearch_b200.engine.batch import BatchMeta
+    starts = torch.arange(4, dtype=torch.int32, device=DEV)
+
+    def meta(base):
+        return BatchMeta(b.slot_ids.to(DEV), starts, base, None, None, 3, 3, 0, 1, 512, False)
+
+    kv, want = b.entry(DEV), []
+    for i in range(steps):
+        want.append(ops.rope_and_attention(rows[i], inv, kv, meta((b.base_len + i).to(DEV)), 4, 2, dim, 0.1))
+    kv2, base, qkv = b.entry(DEV), b.base_len.to(DEV), rows[0].clone()
+    m = meta(base)
+    ops.rope_and_attention(qkv, inv, kv2, m, 4, 2, dim, 0.1)               # loads the kernels
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.rope_and_attention(qkv, inv, kv2, m, 4, 2, dim, 0.1)
+        ops.advance_lengths(base, starts, 3)
+    for i in range(steps):
+        qkv.copy_(rows[i])
+        graph.replay()
+        assert torch.equal(out, want[i]), i
+    ops.check_status(DEV)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).float(), getattr(kv2, name).float())
+
+
+def test_offsets_past_32_bits():
+    """A pool of 70,000 pages (4.6 GB of codes): the batch's pages are its last ones."""
+    pages, heads, dim = 70000, 8, 128
+    from simple_inference_autoresearch_b200.cache import QuantizedKVEntry
+    b = eq.Batch(8, 8, heads, dim, [100, 63], [1, 1], seed=3)
+    small = b.entry(DEV)
+    n = small.k.shape[0]
+    k, v = (torch.empty(pages, heads, 64, dim, dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.empty(pages, heads, 64, device=DEV) for _ in range(2))
+    for big, few in ((k, small.k), (v, small.v), (ks, small.k_scale), (vs, small.v_scale)):
+        big[pages - n:] = few
+    table = torch.where(small.block_table >= 0, small.block_table + (pages - n), small.block_table)
+    big = QuantizedKVEntry(k, v, ks, vs, table, 64)
+    assert k.numel() > 1 << 32
+    for new in ([1, 1], [2, 1], [27, 1]):
+        b.new, b.tokens = new, sum(new)
+        b.q_start = torch.tensor([0, new[0], sum(new)], dtype=torch.int32)
+        b.qkv = torch.randn(b.tokens, 24 * dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+        assert torch.equal(attend(b, big, scale=0.09), attend(b, small, scale=0.09))
+        a, c = (ops.read_kv(e, b.meta(DEV), torch.bfloat16) for e in (big, small))
+        assert torch.equal(a.k, c.k) and torch.equal(a.v, c.v)
+        assert torch.equal(k[pages - n:], small.k) and same(vs[pages - n:], small.v_scale)
+    ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+def test_layers_with_a_window_over_a_quantised_cache(tmp_path, monkeypatch, kv_format):
+    """Layer 0 keeps all keys, the others the last 37: prompt and single tokens far past the window, against the
+    restated kernels on the CPU."""
+    import simple_inference_autoresearch_b200 as siar
+    from simple_inference_autoresearch_b200.architectures.llama import llama_model_spec
+    from simple_inference_autoresearch_b200.config.llama import LlamaConfig
+    from simple_inference_autoresearch_b200.engine.model import DecoderModel, ModelSpec
+    from simple_inference_autoresearch_b200.parts.base import PartSpec
+    from tests import tiny_configs
+    raw, w = tiny_configs.read_folder(tiny_configs.make_folder(tmp_path, "B", seed=5))
+    base = llama_model_spec(LlamaConfig.from_dict(raw))
+    layers = list(base.layers)
+    for i in (1, 2):
+        p = dict(layers[i].params)
+        p["mixer"] = PartSpec("gqa_attention", {**p["mixer"].params, "window": 37})
+        layers[i] = PartSpec(layers[i].kind, p)
+    toks = torch.randint(0, raw["vocab_size"], (150,), generator=torch.Generator().manual_seed(4)).tolist()
+
+    def run(device):
+        model = DecoderModel(ModelSpec(**{**base.__dict__, "layers": tuple(layers)}), torch.float32, device)
+        model.load({k: v.float().to(device) for k, v in w.items()})
+        eng = siar.Engine(model, max_batch=2, max_seq_len=256, use_cuda_graph=False, kv_cache=kv_format)
+        a = eng.open()
+        outs = [eng.step([siar.StepEntry(a, toks[:90], range(90))])]
+        outs += [eng.step([siar.StepEntry(a, [t], [0])]) for t in toks[90:]]
+        assert eng.cache.groups[1].held_pages(a) <= 2
+        eng.close(a)
+        assert all(len(g.pages) == g.pages.n for g in eng.cache.groups)
+        return torch.cat(outs).cpu().double()
+
+    got = run(DEV)
+    ops.check_status(DEV)
+    with monkeypatch.context() as m:
+        eq.install(m)
+        want = run("cpu")
+    off = float((got - want).abs().max() / want.abs().max())
+    assert off <= 2e-4 * (1 if kv_format == "int8" else 127 / 15), off      # as in the engine test above
