@@ -1,13 +1,15 @@
 """The functions of ``ops`` for a cache entry held in 8 or 4 bits (``cache.QuantizedKVEntry``).
 
 ``ops.rope_kv_write``, ``ops.attention`` and ``ops.rope_and_attention`` come here when their cache entry is
-such a one; ``ops.read_kv`` is the read-back.  The formats stand at the top of ``csrc/kv_quant.cu``.
+such a one; ``ops.read_kv`` is the read-back.  The formats stand at the top of ``csrc/kv_quant.cu``.  A decode step over
+a short cache is shorter than its own call, so arguments are looked at once and their pointers taken with that, and
+what a call needs besides its result is one allocation.
 """
 
 from __future__ import annotations
 
 import copy
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -19,34 +21,40 @@ def is_quantized(kv) -> bool:
     return getattr(kv, "k_scale", None) is not None
 
 
-def check_entry(kv, n_kv_heads: int, head_dim: int, device) -> None:
-    """Raises ``ValueError`` unless the entry's tensors are what the kernels index: shapes, types,
-    contiguity, one device."""
+# ------------------------------------------------------------------ arguments
+def check_entry(kv, n_kv_heads: int, head_dim: int, index: int) -> Tuple[int, ...]:
+    """Raises ``ValueError`` unless the entry's tensors are what the kernels index: shapes, types, contiguity, all
+    on GPU ``index`` (-1: the CPU).  Returns what every kernel takes of an entry first: pointers to codes, scales and
+    block table."""
     if head_dim % 16 or not 0 < head_dim <= 256:
         raise ValueError(f"a quantised cache takes head_dim in steps of 16 up to 256, got {head_dim}")
     k, page = kv.k, int(kv.page_tokens)
     code = k.dtype
     rows = (k.shape[0], n_kv_heads, page)
-    if code == torch.int8:
+    if code is torch.int8:
         want, scale, scale_dtype = rows + (head_dim,), rows, torch.float32
-    elif code == torch.uint8:
+    elif code is torch.uint8:
         want, scale, scale_dtype = rows + (head_dim // 2,), rows + (-(-head_dim // 64), 2), torch.bfloat16
     else:
         raise ValueError(f"a quantised cache holds int8 (8 bits) or uint8 (4 bits), got {code}")
+    pointers = []
     for name, t, shape, dtype in (("k", k, want, code), ("v", kv.v, want, code),
                                   ("k_scale", kv.k_scale, scale, scale_dtype), ("v_scale", kv.v_scale, scale, scale_dtype)):
-        if t.shape != shape or t.dtype != dtype:
+        if t.shape != shape or t.dtype is not dtype:
             raise ValueError(f"{name} of a cache entry in {kv.bits} bits must be {dtype} of shape {shape}, "
                              f"got {t.dtype} {tuple(t.shape)}")
-        if not t.is_contiguous() or t.data_ptr() % 16:
+        at = t.data_ptr()
+        if at % 16 or not t.is_contiguous():
             raise ValueError(f"{name} of a cache entry must be contiguous and 16-byte aligned")
-        if t.device != device:
-            raise ValueError(f"{name} of the cache entry is on {t.device}, the activations are on {device}")
+        if t.get_device() != index:
+            raise ValueError(f"{name} of the cache entry is on {t.device}, not where the call's other tensors are")
+        pointers.append(at)
     table = kv.block_table
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+    if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise ValueError("block_table must be a contiguous int32 tensor [slots, pages per sequence]")
-    if table.device != device:
-        raise ValueError(f"block_table is on {table.device}, the activations are on {device}")
+    if table.get_device() != index:
+        raise ValueError(f"block_table is on {table.device}, not where the call's other tensors are")
+    return (*pointers, table.data_ptr())
 
 
 def check_rows(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, meta) -> None:
@@ -55,10 +63,33 @@ def check_rows(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, 
     if qkv.shape != (meta.n_tokens, (n_heads + 2 * n_kv_heads) * head_dim):
         raise ValueError(f"qkv must be [{meta.n_tokens}, {(n_heads + 2 * n_kv_heads) * head_dim}] for these heads, "
                          f"got {tuple(qkv.shape)}")
-    if qkv.dtype not in (torch.bfloat16, torch.float32):
+    if qkv.dtype is not torch.bfloat16 and qkv.dtype is not torch.float32:
         raise TypeError(f"compute dtype must be bfloat16 or float32, got {qkv.dtype}")
     if not qkv.is_contiguous() or qkv.data_ptr() % 16:
         raise ValueError("qkv must be contiguous and 16-byte aligned")
+
+
+def check_batch_tensors(meta, index: int) -> Tuple[int, ...]:
+    """Pointers to the batch's slot ids, row starts and lengths, which have to be int32 on GPU ``index``."""
+    pointers = []
+    for name, n in (("slot_ids", meta.n_seqs), ("q_start", meta.n_seqs + 1), ("base_len", meta.n_seqs)):
+        t = getattr(meta, name)
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < n or t.get_device() != index:
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {n} where the call's other tensors are, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        pointers.append(t.data_ptr())
+    return tuple(pointers)
+
+
+def check_rotary(rotary, head_dim: int, index: int):
+    """``ops.rotary_layout``, with the frequencies where the call's other tensors are."""
+    if isinstance(rotary, torch.Tensor) and rotary.dtype is torch.float32 and 2 * rotary.numel() == head_dim:
+        inv_freq, rotary_dim, interleaved = rotary, head_dim, False       # the common one, without attribute look-ups that fail
+    else:
+        inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
+    if inv_freq is not None and (inv_freq.get_device() != index or not inv_freq.is_contiguous()):
+        raise ValueError(f"inv_freq must be contiguous and where the call's other tensors are, got a tensor on {inv_freq.device}")
+    return inv_freq, rotary_dim, interleaved
 
 
 def check_window(window: Optional[int]) -> None:
@@ -66,57 +97,62 @@ def check_window(window: Optional[int]) -> None:
         raise ValueError(f"an attention window must be positive, got {window}")
 
 
-def _batch(meta):
-    return meta.slot_ids.data_ptr(), meta.q_start.data_ptr(), meta.base_len.data_ptr()
+def _carve(device, *sizes: int):
+    """One allocation for pieces of so many bytes: the tensor to keep while they are in use, and their pointers."""
+    at, offsets = 0, []
+    for n in sizes:
+        offsets.append(at)
+        at += -(-n // 256) * 256
+    held = torch.empty(at, dtype=torch.uint8, device=device)
+    first = held.data_ptr()
+    return (held, *(first + o for o in offsets))
 
 
-def _entry(kv):
-    """What every kernel takes of a cache entry first."""
-    return (kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.block_table.data_ptr())
-
-
+# ------------------------------------------------------------------ store and read back
 def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads: int, head_dim: int,
                   write_kv: bool = True, options: KernelOptions = DEFAULT,
                   q_out: Optional[torch.Tensor] = None) -> None:
-    inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
+    index = qkv.get_device()
+    inv_freq, rotary_dim, interleaved = check_rotary(rotary, head_dim, index)
     check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
-    check_entry(kv, n_kv_heads, head_dim, qkv.device)
+    pools, batch = check_entry(kv, n_kv_heads, head_dim, index), check_batch_tensors(meta, index)
     if q_out is None:
         q_out = qkv
-    elif q_out.shape != qkv.shape or q_out.dtype != qkv.dtype or not q_out.is_contiguous() or q_out.device != qkv.device:
+    elif q_out.shape != qkv.shape or q_out.dtype is not qkv.dtype or not q_out.is_contiguous() or q_out.get_device() != index:
         raise ValueError(f"q_out must be a contiguous tensor like qkv, {qkv.dtype} {tuple(qkv.shape)}")
-    ops._need_cuda(qkv, inv_freq, kv.k)
+    ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
-    with ops._on_device(qkv):
-        ops._launch("kv_quant", "siar_rope_quantize", ops._is_bf16(qkv.dtype), kv.bits, ops._ptr(qkv), ops._ptr(q_out),
-                    ops._ptr(inv_freq), *_entry(kv), *_batch(meta), qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
+    with ops._on_device(index):
+        ops._launch("kv_quant", "siar_rope_quantize", int(qkv.dtype is torch.bfloat16), kv.bits, qkv.data_ptr(), q_out.data_ptr(),
+                    ops._ptr(inv_freq), *pools, *batch, qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
                     kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], int(write_kv),
-                    ops._ptr(ops.status_word(qkv.device)), ops._stream(), rotary_dim, int(interleaved))
+                    ops.status_word(qkv.device).data_ptr(), ops._stream(), rotary_dim, int(interleaved))
 
 
-def _read(kv, meta, dtype: torch.dtype, window: Optional[int], with_slots: bool = False):
+def _pages(kv, meta, page: int) -> Tuple[int, int]:
+    """(pages of ``page`` positions that the batch's sequences hold together, the most of one)."""
+    most = -(-min(meta.max_kv_len, kv.block_table.shape[1] * kv.page_tokens) // page)
+    if meta.base_lens is None or meta.q_lens is None:        # lengths live on the device only: room for the longest everywhere
+        return meta.n_seqs * most, most
+    return sum([min(-(-(n + m) // page), most) for n, m in zip(meta.base_lens, meta.q_lens)]), most
+
+
+def _read(kv, meta, dtype: torch.dtype, window: Optional[int], pools, batch, with_slots: bool = False):
     """(KVEntry of the batch's keys and values, the row of its block table per sequence)."""
-    from ..cache.sequence_cache import KVEntry
-
-    device = kv.k.device
+    device, index = kv.k.device, kv.k.get_device()
     n_kv_heads, head_dim, page = kv.k.shape[1], kv.head_dim, int(kv.page_tokens)
     if meta.max_kv_len <= 0:
         raise ValueError(f"max_kv_len must be positive, got {meta.max_kv_len}")
-    most = min(-(-meta.max_kv_len // page), kv.block_table.shape[1])
-    if meta.base_lens is not None and meta.q_lens is not None:
-        pages = sum(min(-(-(n + m) // page), most) for n, m in zip(meta.base_lens, meta.q_lens))
-    else:                                   # lengths live on the device only: room for the longest everywhere
-        pages = meta.n_seqs * most
-    k = torch.empty((pages, n_kv_heads, page, head_dim), dtype=dtype, device=device)
-    v = torch.empty_like(k)
+    pages, _ = _pages(kv, meta, page)
+    k, v = torch.empty((2, pages, n_kv_heads, page, head_dim), dtype=dtype, device=device).unbind(0)
     table = torch.empty((meta.n_seqs, kv.block_table.shape[1]), dtype=torch.int32, device=device)
     slots = torch.empty(meta.n_seqs, dtype=torch.int32, device=device) if with_slots else None
-    with ops._on_device(kv.k):
-        ops._launch("kv_quant", "siar_read_kv", ops._is_bf16(dtype), kv.bits, *_entry(kv), *_batch(meta), k.data_ptr(),
+    with ops._on_device(index):
+        ops._launch("kv_quant", "siar_read_kv", int(dtype is torch.bfloat16), kv.bits, *pools, *batch, k.data_ptr(),
                     v.data_ptr(), table.data_ptr(), ops._ptr(slots), meta.n_seqs, n_kv_heads, head_dim, page,
                     kv.block_table.shape[1], kv.k.shape[0], pages, meta.max_kv_len, int(window or 0),
-                    ops._ptr(ops.status_word(device)), ops._stream())
-    return KVEntry(k, v, table, page), slots
+                    ops.status_word(device).data_ptr(), ops._stream())
+    return ops.KVEntry(k, v, table, page), slots
 
 
 def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options: KernelOptions = DEFAULT):
@@ -124,12 +160,14 @@ def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options:
         raise TypeError("read_kv reads a quantised cache entry back; this one holds its values as they are")
     check_window(window)
     ops._is_bf16(dtype)                     # raises for anything but bfloat16 and float32
-    check_entry(kv, kv.k.shape[1], kv.head_dim, kv.k.device)
+    index = kv.k.get_device()
+    pools, batch = check_entry(kv, kv.k.shape[1], kv.head_dim, index), check_batch_tensors(meta, index)
     ops._need_cuda(kv.k)
     ops._check_if_asked(options, kv, meta, meta.n_tokens, False, window)
-    return _read(kv, meta, dtype, window)[0]
+    return _read(kv, meta, dtype, window, pools, batch)[0]
 
 
+# ------------------------------------------------------------------ attention
 #: query rows (new tokens x heads of a group) a sequence may bring to the kernel that works on the codes; a longer run
 #: widens the cache once for the tensor-core kernel instead of walking the codes for every 16 rows.  Measured on B200,
 #: four sequences of 4,000 held positions (8 bits, 32 heads on 8, 128 dims): 64 rows 33 us against 40, 256 rows 83
@@ -184,31 +222,28 @@ def _new_workspace(index: int):
     return counters.data_ptr(), scratch.data_ptr(), counters, scratch
 
 
-def _queries16(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, write_kv):
+def _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, write_kv, q16: int, factor: int) -> None:
     """Rotates the queries into float16 rows with a factor each, and stores the new keys and values (``write_kv``)."""
-    n, table, device = qkv.shape[0], kv.block_table, qkv.device
-    q16 = torch.empty((n, n_heads, head_dim), dtype=torch.float16, device=device)
-    factor = torch.empty((n, n_heads), dtype=torch.float32, device=device)
-    ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, qkv.data_ptr(), q16.data_ptr(), factor.data_ptr(),
-                ops._ptr(inv_freq), *_entry(kv), *_batch(meta), n, meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens,
-                table.shape[1], kv.k.shape[0], int(write_kv), ops.status_word(device).data_ptr(), ops._stream())
-    return q16, factor
+    ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, qkv.data_ptr(), q16, factor, ops._ptr(inv_freq), *pools, *batch,
+                qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1],
+                kv.k.shape[0], int(write_kv), ops.status_word(qkv.device).data_ptr(), ops._stream())
 
 
-def _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
+def _on_codes(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
     """``fused``: one token a sequence, rotated (``inv_freq``) and stored (``write_kv``) by the attention kernel itself;
     else, where ``write_kv`` is not None, by a kernel in front."""
-    device, index, table = qkv.device, qkv.device.index, kv.block_table
-    with ops._on_device(qkv):
-        q16 = factor = None
+    device, index, n = qkv.device, qkv.get_device(), qkv.shape[0]
+    with ops._on_device(index):
+        held = q16 = factor = None
         if not fused and write_kv is not None:
-            q16, factor = _queries16(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, write_kv)
-        out = torch.empty((qkv.shape[0], n_heads * head_dim), dtype=qkv.dtype, device=device)
+            held, q16, factor = _carve(device, n * n_heads * head_dim * 2, n * n_heads * 4)
+            _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, write_kv, q16, factor)
+        out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=device)
         stream = ops._stream()
         counters, scratch = _workspace(index, stream)
-        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), ops._ptr(q16), ops._ptr(factor), *_entry(kv),
-                    *_batch(meta), ops._ptr(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads,
-                    head_dim, kv.page_tokens, table.shape[1], kv.k.shape[0], meta.max_q_len, meta.max_kv_len,
+        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), q16, factor, *pools, *batch,
+                    ops._ptr(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads, head_dim,
+                    kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], meta.max_q_len, meta.max_kv_len,
                     ops._sm_count(index), int(fused), int(bool(write_kv)), float(scale), ops.status_word(device).data_ptr(),
                     stream)
     return out
@@ -224,53 +259,34 @@ def works_on_tiles(kv, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_d
 
 
 def key_parts(blocks: int, longest: int, average: float, row_floats: int, sms: int) -> int:
-    """Into how many parts the keys of a block of 128 rows are cut, for ``blocks`` of them of up to ``longest``
-    (on average ``average``) key tiles.  Measured on B200 at 128 dims: a block alone on its SM takes 7 us and 0.95 us
-    a tile, two on every SM 0.66 us a tile and SM, a last round a third of a block more; parts (``row_floats`` floats each)
-    are written and read again at 3.6 TB/s by a kernel of its own.  A chunk of 128 tokens on 8,000 held (32 heads on 8): one
-    part 139 us, 8 parts 54; a prompt of 2,048: one part 69 us, two 109."""
-    best, best_cost = 1, None
-    for parts in range(1, min(16, longest) + 1):
-        tiles = -(-longest // parts)
-        cost = max(7 + 0.95 * tiles, blocks * average * 0.66 / sms + 0.35 * (7 + 1.3 * tiles))
-        if parts > 1:
-            cost += 4 + parts * row_floats * 8 / 3.6e6
-        if best_cost is None or cost < best_cost:
-            best, best_cost = parts, cost
-    return best
+    """Into how many parts the keys of a block of 128 rows are cut (the rule stands at ``siar_attn_quant_tc_parts``)."""
+    return ops._fn("attention_quant_tc", "siar_attn_quant_tc_parts")(blocks, longest, average, row_floats, sms)
 
 
-def _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv) -> torch.Tensor:
+def _on_tiles(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, write_kv) -> torch.Tensor:
     """Rotates (``inv_freq``) and stores (``write_kv``) the new tokens, widens the batch's cache to float16 tiles and
     attends on those."""
-    device, index, n = qkv.device, qkv.device.index, qkv.shape[0]
-    k, table, heads = kv.k, kv.block_table, (n_heads, n_kv_heads, head_dim)
-    most = -(-min(meta.max_kv_len, table.shape[1] * kv.page_tokens) // 64)
-    if meta.base_lens is not None and meta.q_lens is not None:
-        tiles = sum(min(-(-(a + b) // 64), most) for a, b in zip(meta.base_lens, meta.q_lens))
-        q_lens = meta.q_lens
-    else:
-        tiles, q_lens = meta.n_seqs * most, [meta.max_q_len] * meta.n_seqs
-    sms, group = ops._sm_count(index), n_heads // n_kv_heads
+    device, index, n, heads = qkv.device, qkv.get_device(), qkv.shape[0], (n_heads, n_kv_heads, head_dim)
+    tiles, most = _pages(kv, meta, 64)
+    q_lens = meta.q_lens if meta.q_lens is not None else [meta.max_q_len] * meta.n_seqs
+    group = n_heads // n_kv_heads
     block_rows = 128 // group * group
-    blocks = n_kv_heads * sum(-(-m * group // block_rows) for m in q_lens)
-    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 8), sms)
-    empty = lambda shape, dt: torch.empty(shape, dtype=dt, device=device)  # noqa: E731
-    with ops._on_device(qkv):
+    blocks = n_kv_heads * sum([-(-m * group // block_rows) for m in q_lens])
+    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 8), ops._sm_count(index))
+    row_bytes, tile_bytes = n * n_heads * 4, tiles * n_kv_heads * 64 * head_dim * 2
+    with ops._on_device(index):
         stream, status = ops._stream(), ops.status_word(device).data_ptr()
-        q16, factor = _queries16(qkv, inv_freq, kv, meta, *heads, write_kv)
-        out = empty((n, n_heads * head_dim), torch.bfloat16)
-        wide = empty((2, tiles, n_kv_heads, 64, head_dim), torch.float16)
-        k16, v16 = wide.data_ptr(), wide.data_ptr() + wide.numel()
-        info = empty(tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), torch.uint8)
-        seq = empty((meta.n_seqs, 2), torch.int32)
-        scratch = empty(n * n_heads * splits * (head_dim + 8), torch.float32) if splits > 1 else None
-        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *_entry(kv), *_batch(meta), k16, v16, info.data_ptr(),
-                    seq.data_ptr(), meta.n_seqs, n_kv_heads, head_dim, kv.page_tokens, table.shape[1], k.shape[0], tiles,
-                    meta.max_kv_len, status, stream)
-        ops._launch("attention_quant_tc", "siar_attn_quant_tc", q16.data_ptr(), factor.data_ptr(), k16, v16, info.data_ptr(),
-                    seq.data_ptr(), meta.q_start.data_ptr(), meta.base_len.data_ptr(), out.data_ptr(), ops._ptr(scratch), n,
-                    meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
+        out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=device)
+        held, q16, factor, k16, v16, info, seq, scratch = _carve(
+            device, row_bytes // 2 * head_dim, row_bytes, tile_bytes, tile_bytes,
+            tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), meta.n_seqs * 8,
+            row_bytes * splits * (head_dim + 8) if splits > 1 else 0)
+        _queries16(qkv, inv_freq, kv, meta, pools, batch, *heads, write_kv, q16, factor)
+        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, *batch, k16, v16, info, seq, meta.n_seqs,
+                    n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], tiles, meta.max_kv_len,
+                    status, stream)
+        ops._launch("attention_quant_tc", "siar_attn_quant_tc", q16, factor, k16, v16, info, seq, batch[1], batch[2],
+                    out.data_ptr(), scratch, n, meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
                     kernels=2 if splits > 1 else 1)
     return out
 
@@ -279,43 +295,41 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
               window: Optional[int] = None, options: KernelOptions = DEFAULT) -> torch.Tensor:
     check_window(window)
     check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
-    check_entry(kv, n_kv_heads, head_dim, qkv.device)
+    index, heads = qkv.get_device(), (n_heads, n_kv_heads, head_dim)
+    pools, batch = check_entry(kv, n_kv_heads, head_dim, index), check_batch_tensors(meta, index)
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], False, window)
-    if works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
-        return _on_codes(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False, None)
-    if not meta.is_decode and works_on_tiles(kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
-        return _on_tiles(qkv, None, kv, meta, n_heads, n_kv_heads, head_dim, scale, False)
-    pages, slots = _read(kv, meta, qkv.dtype, window, with_slots=True)
+    if works_on_codes(kv, meta, qkv.dtype, *heads, scale, window, options):
+        return _on_codes(qkv, None, kv, meta, pools, batch, *heads, scale, False, None)
+    if not meta.is_decode and works_on_tiles(kv, qkv.dtype, *heads, scale, window, options):
+        return _on_tiles(qkv, None, kv, meta, pools, batch, *heads, scale, False)
+    pages, slots = _read(kv, meta, qkv.dtype, window, pools, batch, with_slots=True)
     of_batch = copy.copy(meta)
     of_batch.slot_ids = slots
-    if meta.is_decode and not ops._fn("attention", "siar_attn_decode_fits")(
-            ops._is_bf16(qkv.dtype), n_heads, n_kv_heads, head_dim):
+    if meta.is_decode and not ops._fn("attention", "siar_attn_decode_fits")(ops._is_bf16(qkv.dtype), *heads):
         of_batch.is_decode = False          # one row a sequence on the prompt kernel
-    return ops.attention(qkv, pages, of_batch, n_heads, n_kv_heads, head_dim, scale, window=window,
-                         options=options.but(check_arguments=False) if options.check_arguments else options)
+    with ops._on_device(index):
+        return ops.attention(qkv, pages, of_batch, *heads, scale, window=window,
+                             options=options.but(check_arguments=False) if options.check_arguments else options)
 
 
 def rope_and_attention(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                        write_kv: bool = True, window: Optional[int] = None,
                        options: KernelOptions = DEFAULT) -> torch.Tensor:
     check_window(window)
-    inv_freq, rotary_dim, interleaved = ops.rotary_layout(rotary, head_dim)
-    plain_layout = inv_freq is None or (rotary_dim == head_dim and not interleaved)
     check_rows(qkv, n_heads, n_kv_heads, head_dim, meta)
-    codes = works_on_codes(kv, meta, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options)
-    whole = None                            # a path that rotates and stores as well
-    if plain_layout and codes:
-        fused = meta.is_decode and options.fuse_decode_rope
-        whole = lambda: _on_codes(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, fused, write_kv)  # noqa: E731
-    elif plain_layout and not meta.is_decode and works_on_tiles(
-            kv, qkv.dtype, n_heads, n_kv_heads, head_dim, scale, window, options):
-        whole = lambda: _on_tiles(qkv, inv_freq, kv, meta, n_heads, n_kv_heads, head_dim, scale, write_kv)  # noqa: E731
-    if whole is not None:
-        check_entry(kv, n_kv_heads, head_dim, qkv.device)
-        ops._need_cuda(qkv, inv_freq)
-        ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
-        return whole()
+    index, heads = qkv.get_device(), (n_heads, n_kv_heads, head_dim)
+    inv_freq, rotary_dim, interleaved = check_rotary(rotary, head_dim, index)
+    if inv_freq is None or (rotary_dim == head_dim and not interleaved):      # paths that rotate and store as well
+        codes = works_on_codes(kv, meta, qkv.dtype, *heads, scale, window, options)
+        if codes or (not meta.is_decode and works_on_tiles(kv, qkv.dtype, *heads, scale, window, options)):
+            pools, batch = check_entry(kv, n_kv_heads, head_dim, index), check_batch_tensors(meta, index)
+            ops._need_cuda(qkv)
+            ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
+            if codes:
+                return _on_codes(qkv, inv_freq, kv, meta, pools, batch, *heads, scale,
+                                 meta.is_decode and options.fuse_decode_rope, write_kv)
+            return _on_tiles(qkv, inv_freq, kv, meta, pools, batch, *heads, scale, write_kv)
     q = torch.empty_like(qkv)               # the rotated queries; qkv stays as it is
-    rope_kv_write(qkv, rotary, kv, meta, n_heads, n_kv_heads, head_dim, write_kv=write_kv, options=options, q_out=q)
-    return attention(q, kv, meta, n_heads, n_kv_heads, head_dim, scale, window=window, options=options)
+    rope_kv_write(qkv, rotary, kv, meta, *heads, write_kv=write_kv, options=options, q_out=q)
+    return attention(q, kv, meta, *heads, scale, window=window, options=options)

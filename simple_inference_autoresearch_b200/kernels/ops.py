@@ -111,6 +111,7 @@ _signatures = {
         "siar_attn_quant_tc": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
         "siar_attn_quant_tc_tile_info_bytes": [],
+        "siar_attn_quant_tc_parts": [c_int, c_int, c_float, c_longlong, c_int],
     },
     "sampling": {
         "siar_sample": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -158,9 +159,9 @@ class _Here:
 _here = _Here()
 
 
-def _on_device(t: torch.Tensor):
-    """A context in which ``t``'s device is the current one (its stream and launches are then that device's)."""
-    return _here if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+def _on_device(index: int):
+    """A context in which GPU ``index`` is the current one (its stream and launches are then that device's)."""
+    return _here if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -695,4 +696,5 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     return out
 
 
+from ..cache.sequence_cache import KVEntry  # noqa: E402  (the cache's module calls this one)
 from . import kv_quant  # noqa: E402  (its functions call this module's)

@@ -23,7 +23,7 @@ def test_entries_and_bytes(kv_format, row):
     c = cache(kv_format)
     e = c.entry(0)
     assert isinstance(e, QuantizedKVEntry) and e.bits == int(kv_format[3:]) and e.head_dim == 80
-    kv_quant.check_entry(e, 2, 80, e.k.device)
+    kv_quant.check_entry(e, 2, 80, -1)
     assert c.entry(1).k.data_ptr() != e.k.data_ptr() and c.entry(2).state.shape == (4, 3)
     assert c.groups[0].bytes() == 2 * 2 * 10 * 2 * 64 * row          # entries, k and v, pages, heads, positions
     assert not eq.values(e.k, e.k_scale).any() or kv_format == "int4"
@@ -142,3 +142,22 @@ def test_unknown_kv_cache_is_refused(tmp_path):
     loaded = siar.load_model(folder, device="cpu", dtype=torch.float32)
     with pytest.raises(CacheError, match="int8, int4"):
         siar.build_engine(loaded, max_seq_len=64, kv_cache="int2")
+
+
+@pytest.mark.parametrize("name,wrong", [("slot_ids", lambda t: t.long()), ("q_start", lambda t: t[:-1]),
+                                        ("base_len", lambda t: torch.stack([t, t], 1)[:, 0])])
+def test_batch_tensors_of_another_type_or_shape(name, wrong):
+    b = eq.Batch(8, 4, 2, 64, [70, 3], [1, 1])
+    for call in (lambda m: ops.rope_and_attention(b.qkv, None, b.kv, m, 4, 2, 64, 0.125),
+                 lambda m: ops.rope_kv_write(b.qkv, None, b.kv, m, 4, 2, 64),
+                 lambda m: ops.attention(b.qkv, b.kv, m, 4, 2, 64, 0.125), lambda m: ops.read_kv(b.kv, m, torch.bfloat16)):
+        meta = b.meta()
+        setattr(meta, name, wrong(getattr(meta, name)))
+        with pytest.raises(ValueError, match=name):
+            call(meta)
+
+
+def test_frequencies_that_are_not_contiguous():
+    b = eq.Batch(8, 4, 2, 64, [70, 3], [1, 1])
+    with pytest.raises(ValueError, match="inv_freq"):
+        ops.rope_and_attention(b.qkv, torch.ones(64)[::2], b.kv, b.meta(), 4, 2, 64, 0.125)
