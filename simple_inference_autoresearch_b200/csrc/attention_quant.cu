@@ -23,10 +23,16 @@
 // latency: 64 sequences of up to 4,500 keys 101 us, of 9,000 in 4 bits 194 us.)  What should bound it is
 // memory: a key and value of a head are 264 bytes (8 bits, head_dim 128) or 144 (4 bits).
 //
-// Work is cut evenly: all (sequence, kv head) units' key tiles stand in one row that is shared out over two
-// blocks an SM, so unequal lengths leave no tail; a warp's loads (TMA, its own ring of stages, the scales
-// along with the codes) run on across the border between two units.  A unit that was cut is joined in
-// block order by the block that finishes it last.
+// Work is cut evenly: all (sequence, kv head) units' key tiles stand in one row that is shared out over two or
+// three blocks an SM, so unequal lengths leave no tail; a warp's loads (TMA, its own ring of stages, the scales
+// along with the codes) run on across the border between two units.  Where every unit can have blocks of its own for
+// at most two steps more a block, it gets them: a border costs about that much.  A unit that was cut is joined
+// in block order by the block that finishes it last.
+//
+// Measured (keys and values at the measured copy rate in brackets): 64 sequences of up to 4,500 keys, 8 bits, 32 heads on
+// 8, 80 us (71); 64 of up to 9,000 in 4 bits, 24 on 8, 93 (77); one of 131,072 in 8 bits 50 (42); one of 6 keys 6.2, the
+// latency of the chain batch -> block table -> keys -> softmax -> values.  Three blocks an SM for 8 bits 82 us, rings of
+// four stages there 83.
 #include "attention_mma.cuh"
 #include "kv_quant.cuh"
 #include "tcgen05.cuh"
@@ -646,8 +652,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
           return far;
         };
         if (__any_sync(0xffffffffu, exponentials())) {      // the unit's first step, and hardly ever after
-          // the reference moves to the largest s + log2 sv seen so far; a row of zeros (or of values below
-          // 127 x 2^-80) must not move it without end
+          // the reference moves to the largest s + log2 sv seen so far; a row of zeros (or of values below 127 x
+          // 2^-40) must not move it without end, or leave a sum of p that no float32 holds
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float m = m_r[nt];
@@ -658,12 +664,13 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
                 if (!MASKED || seen[k][nt][h])
 #pragma unroll
                   for (int gr = 0; gr < NG; ++gr)
-                    m = fmaxf(m, fmaf(x[k][nt][h], f_r[nt], __log2f(fmaxf(sv[k][h][gr], 8.3e-25f))));
+                    m = fmaxf(m, fmaf(x[k][nt][h], f_r[nt], __log2f(fmaxf(sv[k][h][gr], 9.1e-13f))));
 #pragma unroll
             for (int sh = 4; sh <= 16; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
-            const float alpha = m == m_r[nt] ? 1.f : fast_exp2(m_r[nt] - m);
+            // (the sum of p may be as far above 1 as the factor is below what a float32 holds: it takes its root twice)
+            const float root = m == m_r[nt] ? 1.f : fast_exp2(0.5f * (m_r[nt] - m)), alpha = root * root;
             m_r[nt] = m;
-            l_r[nt] *= alpha;
+            l_r[nt] = l_r[nt] * root * root;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) z[nt][gr] *= alpha;
 #pragma unroll
@@ -802,10 +809,11 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     // (m, l, o) of two parts of a row's keys as one
     auto factors = [](float& m, float& l, float m2, float l2, float& fa, float& fb) {
       const float mx = fmaxf(m, m2);
-      fa = m == mx ? 1.f : fast_exp2(m - mx);
-      fb = m2 == mx ? 1.f : fast_exp2(m2 - mx);
+      const float ra = m == mx ? 1.f : fast_exp2(0.5f * (m - mx)), rb = m2 == mx ? 1.f : fast_exp2(0.5f * (m2 - mx));
+      fa = ra * ra;
+      fb = rb * rb;
       m = mx;
-      l = l * fa + l2 * fb;
+      l = l * ra * ra + l2 * rb * rb;
     };
     auto add = [&](int buf) {
       const float2* j = reinterpret_cast<const float2*>(join + buf * C::kRegs * 32) + lane;

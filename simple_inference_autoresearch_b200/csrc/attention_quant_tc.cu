@@ -7,13 +7,17 @@
 //                   into the exponent;
 //   attn_quant_tc   the kernel of attention_tc.cu (its roles, rings and tensor-memory layout are described there)
 //                   on float16 operands: queries as float16 with a power of two of their own, P in float16 against a
-//                   reference that leaves it 32 binary orders of range;  where the rows are too few to fill the
-//                   GPU (a chunk of 512 tokens against a long cache: 56 blocks of 256 rows) the keys of a block of
-//                   rows are cut into parts;
+//                   reference that leaves it 32 binary orders of range.  A block has 128 rows of one kv head's queries,
+//                   so that two blocks share an SM: one's softmax runs under the other's products.  (Blocks of 256 rows,
+//                   one an SM: a prompt of 2,048 tokens 74 us, of 128 rows 67.)  Where the rows are too few to fill
+//                   the GPU the keys of a block of rows are cut into parts;
 //   attn_quant_join adds the parts up.
 //
-// Reading the cache back as bfloat16 pages for the bfloat16 kernel took 87 us for a prompt of 2,048 tokens (4 bits, 32
-// heads on 8) and 199 us for a chunk of 515 on 8,191 held (24 on 8), with 2.5 times the rounding error.
+// All of it, with the kernel that stores the tokens, takes 68 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
+// dims; its products at the measured matrix rate 21 us) and 109 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
+// us).  Beside the products stand their exponentials (67 million in the prompt, 15 us at 16 a clock and SM), whose
+// warps also move scores and P between tensor memory and registers; that, not the products, sets the pace.  Reading the
+// cache back as bfloat16 pages for the bfloat16 kernel took 87 and 199 us, with 2.5 times the rounding error.
 #include "kv_quant.cuh"
 #include "tcgen05.cuh"
 
@@ -21,16 +25,15 @@
 
 namespace siar {
 
-constexpr int kRows = 128;       // rows per query tile
-constexpr int kQTiles = 1;       // query tiles per block
+constexpr int kRows = 128;       // query rows per block
 constexpr int kKeys = 64;        // keys per tile
 constexpr int kStages = 2;       // K and V rings
-constexpr int smem_bytes(int hd) { return kQTiles * kRows * hd * 2 + kStages * 2 * kKeys * hd * 2; }
-constexpr uint32_t kTmemCols = 256 * kQTiles;       // S[q][buf]: 64 columns each from 0; O[q]: head_dim each from kOColumn
-constexpr uint32_t kOColumn = 128 * kQTiles;
+constexpr int smem_bytes(int hd) { return kRows * hd * 2 + kStages * 2 * kKeys * hd * 2; }
+constexpr uint32_t kTmemCols = 256;                 // S[buf]: 64 columns each from 0; O: head_dim from kOColumn
+constexpr uint32_t kOColumn = 128;
 constexpr float kHeadroom = 8.f, kRescaleGap = 7.f; // log2 of where p of the largest score starts, and of what it may grow by
-constexpr int kBlocksPerSM = 2 / kQTiles;
-constexpr int kThreads = 128 + kQTiles * 128;       // TMA warp, one MMA warp per query tile, a spare, the softmax warps
+constexpr int kBlocksPerSM = 2;
+constexpr int kThreads = 256;                       // TMA warp, MMA warp, two that only take part in barriers, four softmax warps
 
 // What the softmax has to know of a key tile and its value tile.
 struct TileInfo {
@@ -74,7 +77,7 @@ __host__ __device__ constexpr uint32_t instr_desc_f16(int n, bool b_mn_major = f
 }
 // Key tiles of the block of rows that begins at row0: up to the last key its last row sees, and what the sequence has.
 __host__ __device__ inline int key_tiles(int base, int q_len, int row0, int G, int tile_rows, int held) {
-  const int last = min(q_len * G, row0 + kQTiles * tile_rows) - 1;
+  const int last = min(q_len * G, row0 + tile_rows) - 1;
   return min((base + last / G + 1 + kKeys - 1) / kKeys, held);
 }
 #define SIAR_TMEM_ST_32(taddr, r)                                                                                  \
@@ -93,7 +96,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                      const __grid_constant__ CUtensorMap tmV, const QuantTcParams prm) {
   extern __shared__ unsigned char smem_dyn[];
   __shared__ __align__(8) uint64_t q_full;
-  __shared__ __align__(8) uint64_t s_full[kQTiles][2], p_full[kQTiles][2], pv_full[kQTiles][2];
+  __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_full[2];
   // keys and values have rings of their own: a key stage is free again as soon as the scores that
   // read it are done, a value stage only after P.V, a step later, so each is asked for as early as it can be
   __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -109,21 +112,13 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   // of short blocks
   const int part = blockIdx.x % prm.splits, kvh = blockIdx.x / prm.splits % prm.Hkv, b = blockIdx.x / prm.splits / prm.Hkv;
   const int G = prm.Hq / prm.Hkv;
-  const int tile_rows = (kRows / G) * G;             // rows of a query tile in use: whole tokens only
+  const int tile_rows = (kRows / G) * G;             // rows in use: whole tokens only
   const int t0 = prm.q_start[b];
   const int q_len = prm.q_start[b + 1] - t0;
   const int rows_total = q_len * G;
-  const int row0 = (gridDim.y - 1 - blockIdx.y) * (kQTiles * tile_rows);
+  const int row0 = (gridDim.y - 1 - blockIdx.y) * tile_rows;
   if (row0 >= rows_total) return;
   const int base = prm.base_len[b];
-  // both query tiles walk all the key tiles of the block (the first tile's last one may be masked entirely)
-  int rows_q[kQTiles];
-  int n_q = 0;
-#pragma unroll
-  for (int g = 0; g < kQTiles; ++g) {
-    rows_q[g] = max(0, min(tile_rows, rows_total - row0 - g * tile_rows));
-    if (rows_q[g] > 0) n_q = g + 1;
-  }
   const int all_tiles = key_tiles(base, q_len, row0, G, tile_rows, prm.seq_tiles[2 * b + 1]);
   const int parts = min(prm.splits, all_tiles);
   if (part >= parts) return;
@@ -132,26 +127,23 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   const uint32_t dyn = smem_u32(smem_dyn);
   unsigned char* sm = smem_dyn + ((1024u - (dyn & 1023u)) & 1023u);
-  unsigned char* q_s = sm;                                   // [q tile][half][128 rows][64 dims]
-  unsigned char* k_s = q_s + kQTiles * kQBytes;              // [stage][half][64 keys][64 dims]
+  unsigned char* q_s = sm;                                   // [half][128 rows][64 dims]
+  unsigned char* k_s = q_s + kQBytes;                        // [stage][half][64 keys][64 dims]
   unsigned char* v_s = k_s + kStages * kTileBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    for (int g = 0; g < kQTiles; ++g) {
-      mbar_init(&s_full[g][0], 1);
-      mbar_init(&s_full[g][1], 1);
-      mbar_init(&p_full[g][0], 1);
-      mbar_init(&p_full[g][1], 1);
-      mbar_init(&pv_full[g][0], 1);
-      mbar_init(&pv_full[g][1], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 1);
+      mbar_init(&pv_full[i], 1);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], n_q);
+      mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], n_q);
+      mbar_init(&v_empty[s], 1);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -177,13 +169,10 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       asm volatile("prefetch.tensormap [%0];" ::"l"(&tmQ) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV) : "memory");
-      mbar_expect_tx(&q_full, n_q * tile_rows * kHd * 2);      // a box is tile_rows packed rows (the rest of the tile stays as it was: masked rows)
-      for (int g = 0; g < n_q; ++g) {
-        const int tok = t0 + (row0 + g * tile_rows) / G;
+      mbar_expect_tx(&q_full, tile_rows * kHd * 2);      // a box is tile_rows packed rows (the rest of the tile stays as it was: masked rows)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-          tma_load_3d(q_s + g * kQBytes + h * (kQBytes / kHalves), &tmQ, &q_full, 64 * h, kvh * G, tok);
-      }
+      for (int h = 0; h < kHalves; ++h)
+        tma_load_3d(q_s + h * (kQBytes / kHalves), &tmQ, &q_full, 64 * h, kvh * G, t0 + row0 / G);
       int issued_k = 0, issued_v = 0;
       for (int i = 0; i < nt_max; ++i) {
         const int s = i % kStages;
@@ -208,29 +197,27 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
       }
     }
-  } else if (warp == 1 || warp == 2) {
-    // ---------------- MMA issue: one thread per query tile (the two tiles depend on nothing of
-    // each other but the K / V stages, and two issuing warps sit on two schedulers)
-    const int g = warp - 1;
-    if (lane == 0 && g < n_q) {
+  } else if (warp == 1) {
+    // ---------------- MMA issue: one thread
+    if (lane == 0) {
       constexpr uint32_t idesc_qk = instr_desc_f16(kKeys);
       constexpr uint32_t idesc_pv = instr_desc_f16(kHd, true);
       // descriptors differ in their low word only (the address field, in units of 16 bytes)
       const uint32_t hi_k = (uint32_t)(smem_desc_sw128(0) >> 32);
       const uint32_t hi_v = (uint32_t)(smem_desc_sw128_mn(0, kTileBytes / kHalves) >> 32);
-      const uint32_t q_lo = (uint32_t)smem_desc_sw128(smem_u32(q_s + g * kQBytes));
+      const uint32_t q_lo = (uint32_t)smem_desc_sw128(smem_u32(q_s));
       const uint32_t k_lo = (uint32_t)smem_desc_sw128(smem_u32(k_s));
       const uint32_t v_lo = (uint32_t)smem_desc_sw128_mn(smem_u32(v_s), kTileBytes / kHalves);
-      const uint32_t tmem_o = tmem_base + kOColumn + (uint32_t)(g * kHd);
-      // S[g][i & 1] = Q_g K_i^T over the two 64-dim halves, 4 steps of 16 dims (32 bytes) in each
+      const uint32_t tmem_o = tmem_base + kOColumn;
+      // S[i & 1] = Q K_i^T over the two 64-dim halves, 4 steps of 16 dims (32 bytes) in each
       auto issue_qk = [&](int i) {
         const uint32_t ks = k_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
-        const uint32_t tmem_s = tmem_base + (uint32_t)((g * 2 + (i & 1)) * kKeys);
+        const uint32_t tmem_s = tmem_base + (uint32_t)((i & 1) * kKeys);
 #pragma unroll
         for (int kk = 0; kk < kHd / kUmmaK; ++kk)
           umma_f16_words(tmem_s, q_lo + (uint32_t)((kk / 4) * (kQBytes / kHalves >> 4) + (kk % 4) * 2), hi_k,
                          ks + (uint32_t)((kk / 4) * (kTileBytes / kHalves >> 4) + (kk % 4) * 2), hi_k, idesc_qk, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[g][i & 1]);
+        umma_commit(&s_full[i & 1]);
         umma_commit(&k_empty[i % kStages]);       // the key stage is free once these scores are done
       };
       bool ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
@@ -244,32 +231,31 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           tc_fence_after();
           issue_qk(i + 1);
         }
-        if (!mbar_wait(&p_full[g][i & 1], (i >> 1) & 1) || !mbar_wait(&v_full[i % kStages], (i / kStages) & 1) ||
+        if (!mbar_wait(&p_full[i & 1], (i >> 1) & 1) || !mbar_wait(&v_full[i % kStages], (i / kStages) & 1) ||
             SIAR_ABORTED()) { ok = false; break; }
         tc_fence_after();
-        // O_g += P_g V_i: 4 steps of 16 keys; V rows (keys) are 128 bytes of one dim half,
+        // O += P V_i: 4 steps of 16 keys; V rows (keys) are 128 bytes of one dim half,
         // 8-row groups 1024 bytes apart, the two dim halves 8 KiB apart
         // P_i sits in tensor memory, in the first 32 columns of the scores it was made from
-        const uint32_t tmem_p = tmem_base + (uint32_t)((g * 2 + (i & 1)) * kKeys);
+        const uint32_t tmem_p = tmem_base + (uint32_t)((i & 1) * kKeys);
         const uint32_t vs = v_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
 #pragma unroll
         for (int t = 0; t < kKeys / kUmmaK; ++t)
           umma_f16_tmem_a(tmem_o, tmem_p + (uint32_t)(t * 8), vs + (uint32_t)(t * (2048 >> 4)), hi_v, idesc_pv,
                           (i > 0 || t > 0) ? 1u : 0u);
-        umma_commit(&pv_full[g][i & 1]);
+        umma_commit(&pv_full[i & 1]);
         umma_commit(&v_empty[i % kStages]);
       }
       if (!ok) SIAR_FAIL();
     }
-  } else if (warp >= 4 && (warp - 4) / 4 < n_q) {
-    // ---------------- softmax: one thread per row, one group of four warps per query tile
-    const int g = (warp - 4) / 4;
+  } else if (warp >= 4) {
+    // ---------------- softmax: one thread per row
     const int quad = warp & 3;                 // the tensor-memory lanes this warp may touch
     const int row = quad * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t tmem_o = tmem_base + kOColumn + (uint32_t)(g * kHd) + lane_base;
-    const int rg = row0 + g * tile_rows + row;
-    const bool mine = row < rows_q[g];
+    const uint32_t tmem_o = tmem_base + kOColumn + lane_base;
+    const int rg = row0 + row;
+    const bool mine = row < min(tile_rows, rows_total - row0);
     const int kv_end = mine ? base + rg / G + 1 : 0;
     const size_t out_row = (size_t)(t0 + (mine ? rg / G : 0)) * prm.Hq + kvh * G + (mine ? rg % G : 0);
     const float row_scale = prm.sl2 * prm.q_factor[out_row];       // of a raw score, times the tile's key factor
@@ -284,9 +270,9 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const TileInfo at = next;
       if (i + 1 < n_tiles) next = info[(size_t)(i + 1) * prm.Hkv];
       const float sl2 = row_scale * at.k_factor;
-      if (!mbar_wait(&s_full[g][i & 1], (i >> 1) & 1) || SIAR_ABORTED()) { ok = false; break; }
+      if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1) || SIAR_ABORTED()) { ok = false; break; }
       tc_fence_after();
-      const uint32_t tmem_s = tmem_base + (uint32_t)((g * 2 + (i & 1)) * kKeys) + lane_base;
+      const uint32_t tmem_s = tmem_base + (uint32_t)((i & 1) * kKeys) + lane_base;
       uint32_t sr[64];
       SIAR_TMEM_LD_32(tmem_s, sr);
       {
@@ -319,10 +305,11 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const bool need = m_new > m_used + kRescaleGap;      // also true for the first finite maximum
       if (i > 0 && __any_sync(0xffffffffu, need)) {
         // O may be touched once the previous tile's P.V has completed
-        if (!mbar_wait(&pv_full[g][(i - 1) & 1], ((i - 1) >> 1) & 1) || SIAR_ABORTED()) { ok = false; break; }
+        if (!mbar_wait(&pv_full[(i - 1) & 1], ((i - 1) >> 1) & 1) || SIAR_ABORTED()) { ok = false; break; }
         tc_fence_after();
-        const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - m_new)) : 1.f;
-        l *= alpha;
+        // (the sum of p may be as far above 1 as the factor is below what a float32 holds: it takes its root twice)
+        const float root = need ? (m_used == -INFINITY ? 0.f : ex2(0.5f * (m_used - m_new))) : 1.f, alpha = root * root;
+        l = l * root * root;
 #pragma unroll 1
         for (int ch = 0; ch < kHd / 32; ++ch) {
           uint32_t o[32];
@@ -336,7 +323,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       if (need) m_used = m_new;
       const float neg_m = m_used == -INFINITY ? 0.f : at.v_log2 - m_used;
-      // P = 2^(s c - m) as bf16 pairs, written over the first 32 columns of the scores in tensor
+      // P = 2^(s c - m) as float16 pairs, written over the first 32 columns of the scores in tensor
       // memory (this thread holds its whole row in registers by now).  The next scores for this
       // buffer are issued after the P.V that reads P, and the tensor pipe keeps that order.
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -355,13 +342,10 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) * at.v_inverse;
       tc_fence_before();
-      if (g == 0)
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      else
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-      if ((threadIdx.x & 127) == 0) mbar_arrive(&p_full[g][i & 1]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if ((threadIdx.x & 127) == 0) mbar_arrive(&p_full[i & 1]);
     }
-    if (ok) ok = mbar_wait(&pv_full[g][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
+    if (ok) ok = mbar_wait(&pv_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
     if (!ok) {
       SIAR_FAIL();
     } else {
@@ -474,12 +458,15 @@ widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_s
     if (first + mine > tiles_out) atomicOr(status, kStatusLengthPastGrid);      // host lengths that fall short
   }
   if (tile >= mine || first + tile >= tiles_out) return;
-  // the power of two that brings the bound to 2^9 .. 2^10 (a tile of zeros, or of next to nothing: 2^60)
+  // The power of two that brings the bound to 2^9 .. 2^10.  At most 2^40 (below a bound of 2^-31 a tile's values keep
+  // fewer bits), 2^20 for a tile of zeros: the softmax takes p against the largest p x value, so the sum of p of a tile of
+  // next to nothing beside one of very large values has to stand within the range of a float32.
   float up[2];
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    const int e = (int)(__float_as_uint(fmaxf(bound_s[2 * kv], bound_s[2 * kv + 1])) >> 23) - 127;
-    up[kv] = __uint_as_float((uint32_t)(max(-120, min(60, 9 - e)) + 127) << 23);
+    const float bound = fmaxf(bound_s[2 * kv], bound_s[2 * kv + 1]);
+    const int e = (int)(__float_as_uint(bound) >> 23) - 127;
+    up[kv] = __uint_as_float((uint32_t)(max(-120, min(bound > 0.f ? 40 : 20, 9 - e)) + 127) << 23);
   }
   const size_t out_row0 = ((size_t)(first + tile) * Hkv + kvh) * kKeys;
   if (threadIdx.x == 0) {
@@ -550,8 +537,8 @@ attn_quant_join_kernel(const float* scratch, __nv_bfloat16* out, const int* seq_
   }
   const int t0 = q_start[b], q_len = q_start[b + 1] - t0;
   if (t < t0 || t >= t0 + q_len) return;
-  const int rg = (t - t0) * G + head % G, block_rows = kQTiles * tile_rows;
-  const int parts = min(splits, key_tiles(base_len[b], q_len, rg / block_rows * block_rows, G, tile_rows, seq_tiles[2 * b + 1]));
+  const int rg = (t - t0) * G + head % G;
+  const int parts = min(splits, key_tiles(base_len[b], q_len, rg / tile_rows * tile_rows, G, tile_rows, seq_tiles[2 * b + 1]));
   if (parts < 2) return;
   const float* part = scratch + (size_t)row * splits * (D + 8);
   float m = -INFINITY, l = 0.f, acc[D / 32];
@@ -559,9 +546,10 @@ attn_quant_join_kernel(const float* scratch, __nv_bfloat16* out, const int* seq_
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
   for (int p = 0; p < parts; ++p, part += D + 8) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(part));
-    const float mx = fmaxf(m, ml.x), fa = m == mx ? 1.f : ex2(m - mx), fb = ml.x == mx ? 1.f : ex2(ml.x - mx);
+    const float mx = fmaxf(m, ml.x), ra = m == mx ? 1.f : ex2(0.5f * (m - mx)), rb = ml.x == mx ? 1.f : ex2(0.5f * (ml.x - mx));
+    const float fa = ra * ra, fb = rb * rb;
+    l = l * ra * ra + ml.y * rb * rb;
     m = mx;
-    l = l * fa + ml.y * fb;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * fa + __ldcg(part + 8 + i * 32 + lane) * fb;
   }
@@ -672,7 +660,7 @@ extern "C" int siar_attn_quant_tc(const void* q, const float* q_factor, const vo
     return (int)cudaErrorInvalidValue;
   const QuantTcParams prm = {(__nv_bfloat16*)out, scratch, (const TileInfo*)tiles, seq_tiles, q_factor, q_start, base_len, status, Hq,
                              Hkv, splits, scale * 1.4426950408889634f};
-  const int G = Hq / Hkv, block_rows = kQTiles * (kRows / G) * G;
+  const int G = Hq / Hkv, block_rows = (kRows / G) * G;
   const long long across = (long long)splits * Hkv * B, down = (max_q_len * (long long)G + block_rows - 1) / block_rows;
   if (across >= (1ll << 31) || down > 65535) return (int)cudaErrorInvalidValue;
   const dim3 grid((unsigned)across, (unsigned)down);

@@ -53,6 +53,7 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x;
+  if (t >= q_start[B]) return;           // a row behind the last sequence stays as it is
   const int b = sequence_of(q_start, B, t);
   const int pos = base_len[b] + (t - q_start[b]);
   const int half = rotary_dim >> 1;
@@ -115,8 +116,9 @@ rope_quantize_kernel(const T* qkv, T* q_out, const float* __restrict__ inv_freq,
 // lanes share a head, a lane holds dims 8j .. 8j + 7 and D/2 + 8j .. + 7, so the pairs of a rotation are its own
 // and a row's statistics take two or three shuffles.  A block walks a run of tokens, kTokens of them at a time:
 // their sequences, pages and angles are formed together, and a token's heads are asked for while the token in
-// front is worked on.  Instructions bound it before memory does: with 8 bytes an access and a division for every
-// code 200 warp instructions for two heads, 59 us for 9,500 tokens of the 8B heads where their bytes take 34.
+// front is worked on.  9,500 tokens of the 8B heads (8 bits): 43 us where their bytes take 34.  Instructions come next to
+// memory as its bound: 8 bytes an access and a division for every code took 59 us (200 warp instructions for two
+// heads), one token a block 61.
 // F16: queries leave as float16 [tokens, Hq, D], each row times a power of two that brings its largest element to
 // 2^9 .. 2^10, and that power's inverse as the row's factor (what the prompt attention on float16 tiles takes: 11 bits
 // of a query where bfloat16 keeps 8).
@@ -133,7 +135,8 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
   __shared__ int pos_s[kTokens], page_s[kTokens];
   const float freq = inv_freq != nullptr ? inv_freq[threadIdx.x % (D / 2)] : 0.f;
   pdl_wait();
-  const int t_begin = (int)((long long)N * blockIdx.x / gridDim.x), t_end = (int)((long long)N * (blockIdx.x + 1) / gridDim.x);
+  const int t_begin = (int)((long long)N * blockIdx.x / gridDim.x);
+  int t_end = (int)((long long)N * (blockIdx.x + 1) / gridDim.x);
   const int lane = threadIdx.x & 31, j = threadIdx.x % LANES, h0 = threadIdx.x / LANES;
   const unsigned mates = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));       // the lanes that share the head
   const int heads = Hq + 2 * Hkv, stride = gridDim.y * HEADS;
@@ -150,6 +153,7 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
       }
   };
   load(t_begin, blockIdx.y * HEADS);
+  const int used = q_start[B];                      // rows behind the last sequence stay as they are
   for (int t0 = t_begin; t0 < t_end; t0 += kTokens) {
     __syncthreads();                                // the angles of the tokens in front have been used
     if (threadIdx.x < 32) {
@@ -165,12 +169,12 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
           const int at = __shfl_sync(0xffffffffu, base - first, b), sl = __shfl_sync(0xffffffffu, own, b);
           if (lane == i) { pos = at + t; slot = sl; }
         }
-      } else if (lane < kTokens && t < t_end) {
+      } else if (lane < kTokens && t < min(t_end, used)) {
         const int b = sequence_of(q_start, B, t);
         pos = base_len[b] + (t - q_start[b]);
         slot = slot_ids[b];
       }
-      if (lane < kTokens && t < t_end) {
+      if (lane < kTokens && t < min(t_end, used)) {
         int page = -1;
         if (write_kv) {
           const int cell = pos / page_tokens;
@@ -185,6 +189,7 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
       }
     }
     __syncthreads();
+    t_end = min(t_end, used);                       // (here, where its load has come back)
     if (inv_freq != nullptr) {
       const int f = threadIdx.x % (D / 2);
       for (int i = threadIdx.x / (D / 2); i < kTokens && t0 + i < t_end; i += 128 / (D / 2))
@@ -328,7 +333,8 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
 // page first(b) + p of the output pools [pages][Hkv][page_tokens][D]; row b of `out_table` names them
 // (-1 beyond), `out_slots[b]` = b (nullptr: not written).  Rows behind a sequence's last token are zeros.  Pages that lie
 // wholly in front of every query's window (first_key of the batch's first new token) are not read.
-// grid (pages of the longest sequence, Hkv, B), 256 threads, 16 codes a thread and step.
+// grid (pages of the longest sequence, Hkv, B), 256 threads, 16 codes a thread and step.  Memory bounds it: 9,500 tokens of
+// the 8B heads in 8 bits 16 us where the bytes take 9 (four steps asked for together: 19, fewer blocks fit an SM).
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
 read_kv_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale, const void* v_scale,
@@ -373,71 +379,46 @@ read_kv_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale
   const size_t out0 = ((size_t)(first + p) * Hkv + kvh) * page_tokens;
   const int rows_held = absent ? 0 : min(page_tokens, total - p * page_tokens);
   const int per_row = D / 16, groups = (D + kQuantGroup - 1) / kQuantGroup;
-  // 16 codes a thread and turn, kTurns turns asked for together
-  constexpr int kTurns = 1;
-  for (int first_idx = threadIdx.x; first_idx < 2 * page_tokens * per_row; first_idx += kTurns * blockDim.x) {
-    uint4 code[kTurns];
-    uint32_t scale[kTurns];
+  for (int idx = threadIdx.x; idx < 2 * page_tokens * per_row; idx += blockDim.x) {
+    const bool is_k = idx < page_tokens * per_row;
+    const int i = is_k ? idx : idx - page_tokens * per_row;
+    const int r = i / per_row, d = (i % per_row) * 16;
+    // a code as a float: its bits in the mantissa of 2^23, the constant taken off again (both exact); 4-bit codes stand for
+    // code - 8
+    float x[16];
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int idx = first_idx + u * blockDim.x;
-      const bool is_k = idx < page_tokens * per_row;
-      const int i = is_k ? idx : idx - page_tokens * per_row;
-      const int r = i / per_row, d = (i % per_row) * 16;
-      code[u] = make_uint4(0u, 0u, 0u, 0u);
-      scale[u] = 0u;
-      if (idx >= 2 * page_tokens * per_row || r >= rows_held) continue;
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+    if (r < rows_held) {
       const uint8_t* src = (is_k ? k_pool : v_pool) + ((row0 + r) * D + d) * BITS / 8;
       const uint32_t* sc = reinterpret_cast<const uint32_t*>(is_k ? k_scale : v_scale);
       if (BITS == 8) {
-        code[u] = *reinterpret_cast<const uint4*>(src);
-        scale[u] = sc[row0 + r];
-      } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(src);
-        code[u].x = c.x;
-        code[u].y = c.y;
-        scale[u] = sc[(row0 + r) * groups + d / kQuantGroup];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int idx = first_idx + u * blockDim.x;
-      if (idx >= 2 * page_tokens * per_row) break;
-      const bool is_k = idx < page_tokens * per_row;
-      const int i = is_k ? idx : idx - page_tokens * per_row;
-      const int r = i / per_row, d = (i % per_row) * 16;
-      // a code as a float: its bits in the mantissa of 2^23, the constant taken off again (both exact).  Rows behind
-      // the last token have codes and scales of zero here; 4-bit codes stand for code - 8, so they are set apart
-      const uint32_t w[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
-      float x[16];
-      if (BITS == 8) {
-        const float s = __uint_as_float(scale[u]);
+        const uint4 code = *reinterpret_cast<const uint4*>(src);
+        const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+        const float s = __uint_as_float(sc[row0 + r]);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           x[e] = (__uint_as_float(__byte_perm(w[e >> 2] ^ 0x80808080u, 0x4b000000u, 0x7440 + (e & 3))) - 8388736.f) * s;
       } else {
-        const float s = __uint_as_float(scale[u] << 16), m = __uint_as_float(scale[u] & 0xffff0000u);
+        const uint2 code = *reinterpret_cast<const uint2*>(src);
+        const uint32_t w[2] = {code.x, code.y}, at = sc[(row0 + r) * groups + d / kQuantGroup];
+        const float s = __uint_as_float(at << 16), m = __uint_as_float(at & 0xffff0000u);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           x[e] = __fadd_rn(__fmul_rn(__uint_as_float(((w[e >> 3] >> (4 * (e & 7))) & 15u) | 0x4b000000u) - 8388616.f, s), m);
       }
-      if (r >= rows_held) {
+    }
+    T* dst = (is_k ? k_out : v_out) + (out0 + r) * D + d;
+    if (sizeof(T) == 2) {
+      uint4 pk[2];
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(pk);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-      }
-      T* dst = (is_k ? k_out : v_out) + (out0 + r) * D + d;
-      if (sizeof(T) == 2) {
-        uint4 pk[2];
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(pk);
+      for (int e = 0; e < 8; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+      reinterpret_cast<uint4*>(dst)[0] = pk[0];
+      reinterpret_cast<uint4*>(dst)[1] = pk[1];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        reinterpret_cast<uint4*>(dst)[0] = pk[0];
-        reinterpret_cast<uint4*>(dst)[1] = pk[1];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          reinterpret_cast<float4*>(dst)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-      }
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<float4*>(dst)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
     }
   }
 }

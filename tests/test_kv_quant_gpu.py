@@ -599,3 +599,52 @@ def test_layers_with_a_window_over_a_quantised_cache(tmp_path, monkeypatch, kv_f
         want = run("cpu")
     off = float((got - want).abs().max() / want.abs().max())
     assert off <= 2e-4 * (1 if kv_format == "int8" else 127 / 15), off      # as in the engine test above
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 40, 300])
+@pytest.mark.parametrize("power", [60, 100])
+@pytest.mark.parametrize("tall", [2, 290, 4000])
+def test_one_very_large_value_among_zeros(bits, new, power, tall):
+    """All scores are equal, all values are zeros but those of key ``tall``, 15 x 2^power: the result is that over the number
+    of keys.  Every number is its code times a power of two (8 bits: a scale off by 2^-24), the sum of equal p by at most
+    2^-23 a key, an exponential and a quotient by 2^-21 each; the result rounds by 2^-9."""
+    dim, held = 64, 4100
+    b = eq.Batch(bits, 2, 1, dim, [held], [new], seed=0, stale="random")
+    x = b.qkv.view(new, 4, dim)
+    x.zero_()
+    x[:, :2, 0] = 1.0                                         # keys are zeros
+    k = torch.zeros(b.kv.k.shape[0], 1, 64, dim)
+    v = torch.zeros_like(k)
+    page = int(b.kv.block_table[int(b.slot_ids[0]), tall // 64])
+    v[page, 0, tall % 64, :] = 15.0 * 2.0 ** power
+    v[page, 0, tall % 64, 1::2] *= -1.0                       # (4 bits: a scale that is not zero)
+    b.kv.k, b.kv.k_scale = eq.quantise(k, bits)
+    b.kv.v, b.kv.v_scale = eq.quantise(v, bits)
+    value = eq.values(b.kv.v, b.kv.v_scale)[page, 0, tall % 64]
+    out = attend(b, b.entry(DEV), scale=1.0).cpu().double().view(new, 2, dim)
+    ops.check_status(DEV)
+    for i in range(new):
+        n = held + i + 1
+        assert bool(((out[i] - value / n).abs() <= (value / n).abs() * (2 ** -9 + n * 2 ** -23 + 2 ** -19)).all()), (i, out[i, 0, :3], value[:3] / n)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.bfloat16, 48), (torch.float32, 64)])
+@pytest.mark.parametrize("new", [[1, 1], [3, 2], [70, 0, 9]])
+def test_rows_behind_the_last_sequence_stay_as_they_are(bits, dtype, dim, new):
+    b = eq.Batch(bits, 4, 2, dim, [65] * len(new), new, seed=9, dtype=dtype)
+    want = b.entry()
+    q = b.qkv.clone()
+    eq.rope_kv_write(q, freqs(dim), want, b.meta(), *b.sizes())
+    pad = torch.randn(37, b.qkv.shape[1], generator=torch.Generator().manual_seed(1)).to(dtype)
+    padded, kv, meta = torch.cat([b.qkv, pad]).to(DEV), b.entry(DEV), b.meta(DEV)
+    meta.n_tokens += 37
+    out = ops.rope_and_attention(padded.clone(), freqs(dim).to(DEV), kv, meta, *b.sizes(), 0.1)
+    ops.rope_kv_write(padded, freqs(dim).to(DEV), kv, meta, *b.sizes())
+    ops.check_status(DEV)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    assert torch.equal(padded[b.tokens:].cpu(), pad) and torch.equal(padded[:b.tokens].cpu(), q)
+    alone = ops.rope_and_attention(b.qkv.to(DEV), freqs(dim).to(DEV), kv, b.meta(DEV), *b.sizes(), 0.1)
+    assert torch.equal(out[:b.tokens], alone)
