@@ -136,7 +136,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     mbar_init(&q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 1);
+      mbar_init(&p_full[i], 4);                      // the softmax warps (no barrier among them: one that gave up would hold the rest)
       mbar_init(&pv_full[i], 1);
     }
     for (int s = 0; s < kStages; ++s) {
@@ -342,8 +342,8 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) * at.v_inverse;
       tc_fence_before();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if ((threadIdx.x & 127) == 0) mbar_arrive(&p_full[i & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[i & 1]);
     }
     if (ok) ok = mbar_wait(&pv_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
     if (!ok) {
