@@ -61,6 +61,27 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two float32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves_of(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // 32 bytes, a whole sector, in one store (a thread owns a row: narrower stores leave sectors half written).
 __device__ __forceinline__ void store_sector(float* p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
@@ -326,21 +347,23 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       // P = 2^(s c - m) as float16 pairs, written over the first 32 columns of the scores in tensor
       // memory (this thread holds its whole row in registers by now).  The next scores for this
       // buffer are issued after the P.V that reads P, and the tensor pipe keeps that order.
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
+      const unsigned long long by = pair_of(sl2, sl2), off = pair_of(neg_m, neg_m);
       uint32_t pw[32];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p0 = ex2(fmaf(__uint_as_float(sr[c * 8 + 2 * e]), sl2, neg_m));
-          const float p1 = ex2(fmaf(__uint_as_float(sr[c * 8 + 2 * e + 1]), sl2, neg_m));
-          sum[e] += p0 + p1;
+          const float2 x = halves_of(fma_pair(pair_of(__uint_as_float(sr[c * 8 + 2 * e]), __uint_as_float(sr[c * 8 + 2 * e + 1])), by, off));
+          const float p0 = ex2(x.x), p1 = ex2(x.y);
+          sum[e] = add_pair(sum[e], pair_of(p0, p1));
           pw[c * 4 + e] = pack_f16x2(p0, p1);
         }
       }
       SIAR_TMEM_ST_32(tmem_s, pw);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) * at.v_inverse;
+      const float2 both = halves_of(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
+      l += (both.x + both.y) * at.v_inverse;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
