@@ -30,7 +30,7 @@
 // in block order by the block that finishes it last.
 //
 // Measured (keys and values at the measured copy rate in brackets): 64 sequences of up to 4,500 keys, 8 bits, 32 heads on
-// 8, 80 us (71); 64 of up to 9,000 in 4 bits, 24 on 8, 93 (77); one of 131,072 in 8 bits 50 (42); one of 6 keys 6.2, the
+// 8, 80 us (71); 64 of up to 9,000 in 4 bits 93 (77); one of 130,018 in 8 bits 50 (42); one of 34 keys 6.2, the
 // latency of the chain batch -> block table -> keys -> softmax -> values.  Three blocks an SM for 8 bits 82 us, rings of
 // four stages there 83.
 #include "attention_mma.cuh"

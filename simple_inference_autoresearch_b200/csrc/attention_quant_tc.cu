@@ -13,11 +13,14 @@
 //                   the GPU the keys of a block of rows are cut into parts;
 //   attn_quant_join adds the parts up.
 //
-// All of it, with the kernel that stores the tokens, takes 68 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
-// dims; its products at the measured matrix rate 21 us) and 109 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
-// us).  Beside the products stand their exponentials (67 million in the prompt, 15 us at 16 a clock and SM), whose
-// warps also move scores and P between tensor memory and registers; that, not the products, sets the pace.  Reading the
-// cache back as bfloat16 pages for the bfloat16 kernel took 87 and 199 us, with 2.5 times the rounding error.
+// All of it, with the kernel that stores the tokens, takes 67 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
+// dims; its products at the measured matrix rate 21 us) and 105 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
+// us).  The chunk's kernels one by one: 9 us storing, 16 widening, 80 the products, 10 joining (they overlap at their
+// ends).  In the products' kernel neither the tensor pipe (37 %) nor the exponentials (37 %) are busy all the time: a
+// tile is a chain scores -> largest -> exponentials -> P -> O, 1,700 cycles for a block alone and 2,000 with two on an
+// SM, at 1.7 GHz.  Tried and no faster: two threads a row (131 us), all key tiles shared out evenly over two blocks an
+// SM (104 to 111, the prompt 68 to 73), four-stage rings.  Reading the cache back as bfloat16 pages for the bfloat16
+// kernel took 87 and 199 us, with 2.5 times the rounding error.
 #include "kv_quant.cuh"
 #include "tcgen05.cuh"
 
