@@ -1019,7 +1019,7 @@ extern "C" unsigned long long siar_capture_id(void* stream) {
 // query and key are rotated here (inv_freq; nullptr: not rotated) and whose key and value are stored
 // (write_kv) and attended to; else the tokens' rows are in the cache and the queries are as they are to be
 // used, in qkv or (q16 not nullptr; qkv is not read then) as siar_rope_quantize_q16 leaves them.  counters: siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
-extern "C" int siar_attn_quant(int bits, const void* qkv, const void* q16, const float* q_factor, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+static int siar_attn_quant_of(int bits, const void* qkv, const void* q16, const float* q_factor, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
                                const int* block_table, const int* slot_ids, const int* q_start, const int* base_len,
                                const float* inv_freq, void* out, int* counters, float* scratch, int B, int Hq, int Hkv, int D,
                                int page_tokens, int max_pages, int n_pages, int max_q_len, int max_kv_len, int sm_count,
@@ -1047,3 +1047,4 @@ extern "C" int siar_attn_quant(int bits, const void* qkv, const void* q16, const
   SIAR_GO(4, 128);
 #undef SIAR_GO
 }
+SIAR_TAKES_WORDS(siar_attn_quant)

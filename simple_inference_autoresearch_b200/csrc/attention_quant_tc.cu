@@ -652,7 +652,7 @@ extern "C" int siar_attn_quant_tc_tile_info_bytes(void) { return (int)sizeof(Til
 
 // The batch's keys and values as float16 tiles of 64 positions, sequence after sequence: k_out, v_out
 // [tiles_out, Hkv, 64, D], tiles [tiles_out, Hkv] (siar_attn_quant_tc_tile_info_bytes each), seq_tiles [B, 2].
-extern "C" int siar_widen_tiles(int bits, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+static int siar_widen_tiles_of(int bits, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                                 const int* block_table, const int* slot_ids, const int* q_start, const int* base_len, void* k_out,
                                 void* v_out, void* tiles, int* seq_tiles, int B, int Hkv, int D, int page_tokens, int max_pages,
                                 int n_pages, int tiles_out, int max_kv_len, int* status, void* stream) {
@@ -669,10 +669,11 @@ extern "C" int siar_widen_tiles(int bits, const void* k_pool, const void* v_pool
   if (bits == 8) return D == 64 ? go(widen_tiles_kernel<64, 8>) : go(widen_tiles_kernel<128, 8>);
   return D == 64 ? go(widen_tiles_kernel<64, 4>) : go(widen_tiles_kernel<128, 4>);
 }
+SIAR_TAKES_WORDS(siar_widen_tiles)
 
 // q [N, Hq, D] float16 with q_factor [N, Hq]; out [N, Hq * D] bfloat16; scratch: with splits > 1 N * Hq * splits * (D + 8)
 // floats.  splits: parts into which the keys of a block of rows are cut.
-extern "C" int siar_attn_quant_tc(const void* q, const float* q_factor, const void* k_tiles, const void* v_tiles, const void* tiles,
+static int siar_attn_quant_tc_of(const void* q, const float* q_factor, const void* k_tiles, const void* v_tiles, const void* tiles,
                                   const int* seq_tiles, const int* q_start, const int* base_len, void* out, float* scratch, int N, int B,
                                   int Hq, int Hkv, int D, int tiles_out, int max_q_len, int splits, float scale, int* status,
                                   void* stream) {
@@ -693,3 +694,4 @@ extern "C" int siar_attn_quant_tc(const void* q, const float* q_factor, const vo
   return D == 64 ? launch_tc<64>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream)
                  : launch_tc<128>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream);
 }
+SIAR_TAKES_WORDS(siar_attn_quant_tc)

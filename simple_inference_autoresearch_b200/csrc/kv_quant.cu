@@ -454,7 +454,7 @@ static int launch_wide(int bits, const void* qkv, void* q_to, float* q_factor, c
 
 // qkv [N, (Hq + 2 Hkv) D] (not changed unless q_out == qkv); q_out: the same layout, its query part is
 // written (rotated).  Pools and scales as at the top of the file.
-extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* q_out, const float* inv_freq,
+static int siar_rope_quantize_of(int is_bf16, int bits, const void* qkv, void* q_out, const float* inv_freq,
                                   void* k_pool, void* v_pool, void* k_scale, void* v_scale, const int* block_table,
                                   const int* slot_ids, const int* q_start, const int* base_len, int N, int B, int Hq,
                                   int Hkv, int D, int page_tokens, int max_pages, int n_pages, int write_kv,
@@ -482,10 +482,11 @@ extern "C" int siar_rope_quantize(int is_bf16, int bits, const void* qkv, void* 
   return bits == 8 ? go(rope_quantize_kernel<float, 8>, (float*)nullptr)
                    : go(rope_quantize_kernel<float, 4>, (float*)nullptr);
 }
+SIAR_TAKES_WORDS(siar_rope_quantize)
 
 // The same for bfloat16, head_dim 64 or 128 and whole-head rotation (or none), with the queries as float16:
 // q16 [N, Hq, D], q_factor [N, Hq].
-extern "C" int siar_rope_quantize_q16(int bits, const void* qkv, void* q16, float* q_factor, const float* inv_freq, void* k_pool,
+static int siar_rope_quantize_q16_of(int bits, const void* qkv, void* q16, float* q_factor, const float* inv_freq, void* k_pool,
                                       void* v_pool, void* k_scale, void* v_scale, const int* block_table, const int* slot_ids,
                                       const int* q_start, const int* base_len, int N, int B, int Hq, int Hkv, int D, int page_tokens,
                                       int max_pages, int n_pages, int write_kv, int* status, void* stream) {
@@ -496,11 +497,12 @@ extern "C" int siar_rope_quantize_q16(int bits, const void* qkv, void* q16, floa
   return launch_wide<true>(bits, qkv, q16, q_factor, inv_freq, k_pool, v_pool, k_scale, v_scale, block_table, slot_ids, q_start,
                            base_len, N, B, Hq, Hkv, D, page_tokens, max_pages, n_pages, write_kv, status, stream);
 }
+SIAR_TAKES_WORDS(siar_rope_quantize_q16)
 
 // The keys and values of a batch as pages of the compute type; see read_kv_kernel.  out_table
 // [B, max_pages], out_slots [B]; pages_out: pages the output pools have (host lengths that fall short of
 // the device's leave the pages beyond unread, with cell -1).
-extern "C" int siar_read_kv(int is_bf16, int bits, const void* k_pool, const void* v_pool, const void* k_scale,
+static int siar_read_kv_of(int is_bf16, int bits, const void* k_pool, const void* v_pool, const void* k_scale,
                             const void* v_scale, const int* block_table, const int* slot_ids, const int* q_start,
                             const int* base_len, void* k_out, void* v_out, int* out_table, int* out_slots, int B,
                             int Hkv, int D, int page_tokens, int max_pages, int n_pages, int pages_out, int max_kv_len,
@@ -522,3 +524,4 @@ extern "C" int siar_read_kv(int is_bf16, int bits, const void* k_pool, const voi
                      : go(read_kv_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr);
   return bits == 8 ? go(read_kv_kernel<float, 8>, (float*)nullptr) : go(read_kv_kernel<float, 4>, (float*)nullptr);
 }
+SIAR_TAKES_WORDS(siar_read_kv)

@@ -97,6 +97,10 @@ def check_window(window: Optional[int]) -> None:
         raise ValueError(f"an attention window must be positive, got {window}")
 
 
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _carve(device, *sizes: int):
     """One allocation for pieces of so many bytes: the tensor to keep while they are in use, and their pointers."""
     at, offsets = 0, []
@@ -123,8 +127,8 @@ def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads:
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
     with ops._on_device(index):
-        ops._launch("kv_quant", "siar_rope_quantize", int(qkv.dtype is torch.bfloat16), kv.bits, qkv.data_ptr(), q_out.data_ptr(),
-                    ops._ptr(inv_freq), *pools, *batch, qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
+        ops._launch_words("kv_quant", "siar_rope_quantize", int(qkv.dtype is torch.bfloat16), kv.bits, qkv.data_ptr(), q_out.data_ptr(),
+                    _at(inv_freq), *pools, *batch, qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim,
                     kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], int(write_kv),
                     ops.status_word(qkv.device).data_ptr(), ops._stream(), rotary_dim, int(interleaved))
 
@@ -148,8 +152,8 @@ def _read(kv, meta, dtype: torch.dtype, window: Optional[int], pools, batch, wit
     table = torch.empty((meta.n_seqs, kv.block_table.shape[1]), dtype=torch.int32, device=device)
     slots = torch.empty(meta.n_seqs, dtype=torch.int32, device=device) if with_slots else None
     with ops._on_device(index):
-        ops._launch("kv_quant", "siar_read_kv", int(dtype is torch.bfloat16), kv.bits, *pools, *batch, k.data_ptr(),
-                    v.data_ptr(), table.data_ptr(), ops._ptr(slots), meta.n_seqs, n_kv_heads, head_dim, page,
+        ops._launch_words("kv_quant", "siar_read_kv", int(dtype is torch.bfloat16), kv.bits, *pools, *batch, k.data_ptr(),
+                    v.data_ptr(), table.data_ptr(), _at(slots), meta.n_seqs, n_kv_heads, head_dim, page,
                     kv.block_table.shape[1], kv.k.shape[0], pages, meta.max_kv_len, int(window or 0),
                     ops.status_word(device).data_ptr(), ops._stream())
     return ops.KVEntry(k, v, table, page), slots
@@ -224,7 +228,7 @@ def _new_workspace(index: int):
 
 def _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, write_kv, q16: int, factor: int) -> None:
     """Rotates the queries into float16 rows with a factor each, and stores the new keys and values (``write_kv``)."""
-    ops._launch("kv_quant", "siar_rope_quantize_q16", kv.bits, qkv.data_ptr(), q16, factor, ops._ptr(inv_freq), *pools, *batch,
+    ops._launch_words("kv_quant", "siar_rope_quantize_q16", kv.bits, qkv.data_ptr(), q16, factor, _at(inv_freq), *pools, *batch,
                 qkv.shape[0], meta.n_seqs, n_heads, n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1],
                 kv.k.shape[0], int(write_kv), ops.status_word(qkv.device).data_ptr(), ops._stream())
 
@@ -234,15 +238,15 @@ def _on_codes(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_d
     else, where ``write_kv`` is not None, by a kernel in front."""
     device, index, n = qkv.device, qkv.get_device(), qkv.shape[0]
     with ops._on_device(index):
-        held = q16 = factor = None
+        held, q16, factor = None, 0, 0
         if not fused and write_kv is not None:
             held, q16, factor = _carve(device, n * n_heads * head_dim * 2, n * n_heads * 4)
             _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, write_kv, q16, factor)
         out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=device)
         stream = ops._stream()
         counters, scratch = _workspace(index, stream)
-        ops._launch("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), q16, factor, *pools, *batch,
-                    ops._ptr(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads, head_dim,
+        ops._launch_words("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), q16, factor, *pools, *batch,
+                    _at(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads, head_dim,
                     kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], meta.max_q_len, meta.max_kv_len,
                     ops._sm_count(index), int(fused), int(bool(write_kv)), float(scale), ops.status_word(device).data_ptr(),
                     stream)
@@ -282,10 +286,10 @@ def _on_tiles(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_d
             tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), meta.n_seqs * 8,
             row_bytes * splits * (head_dim + 8) if splits > 1 else 0)
         _queries16(qkv, inv_freq, kv, meta, pools, batch, *heads, write_kv, q16, factor)
-        ops._launch("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, *batch, k16, v16, info, seq, meta.n_seqs,
+        ops._launch_words("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, *batch, k16, v16, info, seq, meta.n_seqs,
                     n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], tiles, meta.max_kv_len,
                     status, stream)
-        ops._launch("attention_quant_tc", "siar_attn_quant_tc", q16, factor, k16, v16, info, seq, batch[1], batch[2],
+        ops._launch_words("attention_quant_tc", "siar_attn_quant_tc", q16, factor, k16, v16, info, seq, batch[1], batch[2],
                     out.data_ptr(), scratch, n, meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
                     kernels=2 if splits > 1 else 1)
     return out

@@ -12,6 +12,7 @@ The parts call these functions through the module (``ops.linear(...)``).
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -90,7 +91,7 @@ _signatures = {
                          c_int, c_int, c_void_p, c_void_p],
     },
     "attention_quant": {
-        # bits, qkv, q16, q_factor, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
+        # (taken as words) bits, qkv, q16, q_factor, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
         # B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, max_kv_len, sm_count, fused, write_kv, scale, status,
         # stream
         "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -136,6 +137,21 @@ def _fn(unit: str, name: str):
 def _launch(unit: str, name: str, *args, kernels: int = 1) -> None:
     global launch_count
     err = _fn(unit, name)(*args)
+    if err != 0:
+        raise RuntimeError(f"{name} failed to launch: CUDA error {err} (see cudaError_t); "
+                           "sizes the kernel refuses are reported as cudaErrorInvalidValue (1)")
+    launch_count += kernels
+
+
+def _launch_words(unit: str, name: str, *args, kernels: int = 1) -> None:
+    """``_launch`` for a function that takes its arguments as one buffer of 64-bit words (floats as doubles; no pointer: 0)."""
+    global launch_count
+    f = _bound.get(name)
+    if f is None:
+        entry = getattr(build.load_unit(unit), name)
+        entry.argtypes, entry.restype = [ctypes.c_char_p], c_int
+        f = _bound[name] = entry, struct.Struct("".join("d" if t is c_float else "q" for t in _signatures[unit][name])).pack
+    err = f[0](f[1](*args))
     if err != 0:
         raise RuntimeError(f"{name} failed to launch: CUDA error {err} (see cudaError_t); "
                            "sizes the kernel refuses are reported as cudaErrorInvalidValue (1)")
