@@ -256,8 +256,7 @@ def _on_codes(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_d
 def works_on_tiles(kv, dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                    window: Optional[int] = None, options: KernelOptions = DEFAULT) -> bool:
     """True when prompts' attention over this entry runs on float16 tiles on the tensor cores (bfloat16, head_dim 64
-    or 128, at most 128 query heads per kv head, pages of a multiple of 64, no window); else the cache is read back
-    for the kernels of an ordinary cache."""
+    or 128, at most 128 query heads per kv head, pages of a multiple of 64, no window, a positive scale)."""
     return (dtype == torch.bfloat16 and window is None and head_dim in (64, 128) and n_heads // n_kv_heads <= 128
             and kv.page_tokens % 64 == 0 and scale > 0 and options.use_tc_attention and options.use_mma_attention)
 

@@ -21,10 +21,12 @@ class KernelOptions:
     #: the products of a decode step add into the residual stream and make the next product's
     #: normed input themselves (no norm kernel between them); False: separate norm kernels
     fuse_residual_stream: bool = True
-    #: prompts' attention on the tcgen05 kernel where its sizes allow; False: the warp-level kernel
+    #: prompts' attention on the tcgen05 kernel where its sizes allow; False: the warp-level kernel (over a cache
+    #: in 8 or 4 bits: the kernel that works on the codes)
     use_tc_attention: bool = True
     #: bfloat16 attention on the warp-level tensor-core kernels where their sizes allow; False:
-    #: the CUDA-core kernels (this also rules out the tcgen05 kernel)
+    #: the CUDA-core kernels (this also rules out the tcgen05 kernel, and over a cache in 8 or 4 bits every kernel
+    #: but the read-back in front of the CUDA-core ones)
     use_mma_attention: bool = True
     #: a decode step's rotary encoding and cache write inside its attention kernel
     fuse_decode_rope: bool = True
