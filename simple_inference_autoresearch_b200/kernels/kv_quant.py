@@ -124,6 +124,8 @@ def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads:
         q_out = qkv
     elif q_out.shape != qkv.shape or q_out.dtype is not qkv.dtype or not q_out.is_contiguous() or q_out.get_device() != index:
         raise ValueError(f"q_out must be a contiguous tensor like qkv, {qkv.dtype} {tuple(qkv.shape)}")
+    elif 0 < abs(q_out.data_ptr() - qkv.data_ptr()) < qkv.numel() * qkv.element_size():
+        raise ValueError("q_out must be qkv itself or lie apart from it")
     ops._need_cuda(qkv)
     ops._check_if_asked(options, kv, meta, qkv.shape[0], write_kv)
     with ops._on_device(index):
@@ -203,7 +205,7 @@ def _workspace(index: int, stream: int):
     if not torch._C._cuda_isCurrentStreamCapturing():
         held = _workspaces.get(key)
         if held is None:
-            held = _workspaces[key] = _new_workspace(index)
+            held = _workspaces.setdefault(key, _new_workspace(index))      # (one of two threads' is kept)
         return held[:2]
     fn = ops._fn("attention_quant", "siar_capture_id")
     fn.restype = ops.c_ulonglong

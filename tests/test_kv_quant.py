@@ -161,3 +161,10 @@ def test_frequencies_that_are_not_contiguous():
     b = eq.Batch(8, 4, 2, 64, [70, 3], [1, 1])
     with pytest.raises(ValueError, match="inv_freq"):
         ops.rope_and_attention(b.qkv, torch.ones(64)[::2], b.kv, b.meta(), 4, 2, 64, 0.125)
+
+
+def test_queries_that_would_go_over_other_rows():
+    b = eq.Batch(8, 4, 2, 64, [70, 3], [1, 1])
+    room = torch.zeros(3, 512, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_kv_write(room[:2], None, b.kv, b.meta(), 4, 2, 64, q_out=room[1:])

@@ -648,3 +648,38 @@ def test_rows_behind_the_last_sequence_stay_as_they_are(bits, dtype, dim, new):
     assert torch.equal(padded[b.tokens:].cpu(), pad) and torch.equal(padded[:b.tokens].cpu(), q)
     alone = ops.rope_and_attention(b.qkv.to(DEV), freqs(dim).to(DEV), kv, b.meta(DEV), *b.sizes(), 0.1)
     assert torch.equal(out[:b.tokens], alone)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_threads_that_call_on_one_stream_and_on_their_own(bits, new):
+    import threading
+    batches = [eq.Batch(bits, 8, 2, 64, [700, 1500, 20 + i], [new] * 3, seed=i) for i in range(4)]
+    entries, inv = [b.entry(DEV) for b in batches], freqs(64).to(DEV)
+    call = lambda i: ops.rope_and_attention(  # noqa: E731
+        batches[i].qkv.to(DEV), inv, entries[i], batches[i].meta(DEV), 8, 2, 64, 0.125)
+    want = [call(i) for i in range(4)]
+    torch.cuda.synchronize()
+    for shared in (True, False):
+        stream = torch.cuda.Stream()
+        got, errors = [None] * 4, []
+
+        def work(i):
+            try:
+                with torch.cuda.stream(stream if shared else torch.cuda.Stream()):
+                    for _ in range(20):
+                        got[i] = call(i)
+                    torch.cuda.current_stream().synchronize()
+            except Exception as e:  # noqa: BLE001 - reported below
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not errors
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    ops.check_status(DEV)
