@@ -13,12 +13,13 @@
 //                   the GPU the keys of a block of rows are cut into parts;
 //   attn_quant_join adds the parts up.
 //
-// All of it, with the kernel that stores the tokens, takes 67 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
-// dims; its products at the measured matrix rate 21 us) and 105 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
-// us).  The chunk's kernels one by one: 9 us storing, 16 widening, 80 the products, 10 joining (they overlap at their
+// All of it, with the kernel that stores the tokens, takes 64 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
+// dims; its products at the measured matrix rate 21 us) and 99 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
+// us).  The chunk's kernels one by one: 9 us storing, 16 widening, 75 the products, 10 joining (they overlap at their
 // ends).  In the products' kernel neither the tensor pipe (37 %) nor the exponentials (37 %) are busy all the time: a
-// tile is a chain scores -> largest -> exponentials -> P -> O, 1,700 cycles for a block alone and 2,000 with two on an
-// SM, at 1.7 GHz.  Tried and no faster: two threads a row (131 us), all key tiles shared out evenly over two blocks an
+// tile is a chain scores -> largest -> exponentials -> P -> O, some 1,700 cycles for a block alone and 1,900 with two on an
+// SM, at 1.7 GHz.  (With scores and P.V issued by one thread of a warp, and a load a tile for its factors, the two took
+// 66 and 104 us.)  Tried and no faster: two threads a row (131 us), all key tiles shared out evenly over two blocks an
 // SM (104 to 111, the prompt 68 to 73), four-stage rings.  Reading the cache back as bfloat16 pages for the bfloat16
 // kernel took 87 and 199 us, with 2.5 times the rounding error.
 #include "kv_quant.cuh"
@@ -36,13 +37,12 @@ constexpr uint32_t kTmemCols = 256;                 // S[buf]: 64 columns each f
 constexpr uint32_t kOColumn = 128;
 constexpr float kHeadroom = 8.f, kRescaleGap = 7.f; // log2 of where p of the largest score starts, and of what it may grow by
 constexpr int kBlocksPerSM = 2;
-constexpr int kThreads = 256;                       // TMA warp, MMA warp, two that only take part in barriers, four softmax warps
+constexpr int kThreads = 256;                       // TMA warp, scores, a spare, P.V, four softmax warps
 
 // What the softmax has to know of a key tile and its value tile.
 struct TileInfo {
   float k_factor;                // a key is the tile's float16 times this power of two
-  float v_log2, v_inverse;       // a value is the tile's float16 times 2^v_log2; 2^-v_log2
-  float unused;
+  float v_log2;                  // a value is the tile's float16 times 2^v_log2
   unsigned long long bad[2];     // bit r: the value of position r is not a number (in its first, second run of 64 dims)
 };
 
@@ -63,6 +63,12 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 // Two float32 operations in one instruction.
 __device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
@@ -154,7 +160,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   unsigned char* q_s = sm;                                   // [half][128 rows][64 dims]
   unsigned char* k_s = q_s + kQBytes;                        // [stage][half][64 keys][64 dims]
   unsigned char* v_s = k_s + kStages * kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
@@ -176,7 +182,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = tmem_base_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
   const bool dead = (*(volatile int*)prm.status & kStatusWaitExpired) != 0;
 
 #define SIAR_FAIL()                                   \
@@ -221,57 +227,61 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
       }
     }
-  } else if (warp == 1) {
-    // ---------------- MMA issue: one thread
-    if (lane == 0) {
-      constexpr uint32_t idesc_qk = instr_desc_f16(kKeys);
-      constexpr uint32_t idesc_pv = instr_desc_f16(kHd, true);
-      // descriptors differ in their low word only (the address field, in units of 16 bytes)
-      const uint32_t hi_k = (uint32_t)(smem_desc_sw128(0) >> 32);
-      const uint32_t hi_v = (uint32_t)(smem_desc_sw128_mn(0, kTileBytes / kHalves) >> 32);
-      const uint32_t q_lo = (uint32_t)smem_desc_sw128(smem_u32(q_s));
-      const uint32_t k_lo = (uint32_t)smem_desc_sw128(smem_u32(k_s));
-      const uint32_t v_lo = (uint32_t)smem_desc_sw128_mn(smem_u32(v_s), kTileBytes / kHalves);
-      const uint32_t tmem_o = tmem_base + kOColumn;
-      // S[i & 1] = Q K_i^T over the two 64-dim halves, 4 steps of 16 dims (32 bytes) in each
-      auto issue_qk = [&](int i) {
-        const uint32_t ks = k_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
-        const uint32_t tmem_s = tmem_base + (uint32_t)((i & 1) * kKeys);
-#pragma unroll
-        for (int kk = 0; kk < kHd / kUmmaK; ++kk)
-          umma_f16_words(tmem_s, q_lo + (uint32_t)((kk / 4) * (kQBytes / kHalves >> 4) + (kk % 4) * 2), hi_k,
-                         ks + (uint32_t)((kk / 4) * (kTileBytes / kHalves >> 4) + (kk % 4) * 2), hi_k, idesc_qk, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[i & 1]);
-        umma_commit(&k_empty[i % kStages]);       // the key stage is free once these scores are done
-      };
-      bool ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        issue_qk(0);
-      }
+  } else if (warp == 1 || warp == 3) {
+    // ---------------- MMA issue: warp 1 the scores, warp 3 P.V.  One thread issues; the whole warp walks along, so that all it
+    // computes is the same in every lane and stays in uniform registers, where the products take their operands
+    // from (issue under lane == 0: 75 cycles a product more).
+    auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+    const bool chosen = elect_one();
+    // descriptors differ in their low word only (the address field, in units of 16 bytes)
+    const uint32_t hi_k = (uint32_t)(smem_desc_sw128(0) >> 32);
+    const uint32_t hi_v = (uint32_t)(smem_desc_sw128_mn(0, kTileBytes / kHalves) >> 32);
+    const uint32_t q_lo = (uint32_t)smem_desc_sw128(smem_u32(q_s));
+    const uint32_t k_lo = (uint32_t)smem_desc_sw128(smem_u32(k_s));
+    const uint32_t v_lo = (uint32_t)smem_desc_sw128_mn(smem_u32(v_s), kTileBytes / kHalves);
+    bool ok = true;
+    if (warp == 1) {
+      ok = wait(&q_full, 0);
       for (int i = 0; i < nt_max && ok; ++i) {
-        if (i + 1 < nt_max) {
-          if (!mbar_wait(&k_full[(i + 1) % kStages], ((i + 1) / kStages) & 1) || SIAR_ABORTED()) { ok = false; break; }
-          tc_fence_after();
-          issue_qk(i + 1);
-        }
-        if (!mbar_wait(&p_full[i & 1], (i >> 1) & 1) || !mbar_wait(&v_full[i % kStages], (i / kStages) & 1) ||
-            SIAR_ABORTED()) { ok = false; break; }
+        // the buffer is free when the P.V that read P from it is done
+        ok = wait(&k_full[i % kStages], (i / kStages) & 1) && (i < 2 || wait(&pv_full[i & 1], ((i - 2) >> 1) & 1));
+        if (!ok) break;
         tc_fence_after();
-        // O += P V_i: 4 steps of 16 keys; V rows (keys) are 128 bytes of one dim half,
-        // 8-row groups 1024 bytes apart, the two dim halves 8 KiB apart
-        // P_i sits in tensor memory, in the first 32 columns of the scores it was made from
-        const uint32_t tmem_p = tmem_base + (uint32_t)((i & 1) * kKeys);
-        const uint32_t vs = v_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
+        if (chosen) {
+          // S[i & 1] = Q K_i^T over the 64-dim halves, 4 steps of 16 dims (32 bytes) in each
+          constexpr uint32_t idesc = instr_desc_f16(kKeys);
+          const uint32_t ks = k_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
 #pragma unroll
-        for (int t = 0; t < kKeys / kUmmaK; ++t)
-          umma_f16_tmem_a(tmem_o, tmem_p + (uint32_t)(t * 8), vs + (uint32_t)(t * (2048 >> 4)), hi_v, idesc_pv,
-                          (i > 0 || t > 0) ? 1u : 0u);
-        umma_commit(&pv_full[i & 1]);
-        umma_commit(&v_empty[i % kStages]);
+          for (int kk = 0; kk < kHd / kUmmaK; ++kk)
+            umma_f16_words(tmem_base + (uint32_t)((i & 1) * kKeys), q_lo + (uint32_t)((kk / 4) * (kQBytes / kHalves >> 4) + (kk % 4) * 2), hi_k,
+                           ks + (uint32_t)((kk / 4) * (kTileBytes / kHalves >> 4) + (kk % 4) * 2), hi_k, idesc, kk > 0 ? 1u : 0u);
+          umma_commit(&s_full[i & 1]);
+          umma_commit(&k_empty[i % kStages]);       // the key stage is free once these scores are done
+        }
+        __syncwarp();
       }
-      if (!ok) SIAR_FAIL();
+    } else {
+      for (int i = 0; i < nt_max && ok; ++i) {
+        ok = wait(&v_full[i % kStages], (i / kStages) & 1) && wait(&p_full[i & 1], (i >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (chosen) {
+          // O += P V: 4 steps of 16 keys; V rows (keys) are 128 bytes of one dim half, 8-row groups 1024 bytes apart,
+          // the two dim halves 8 KiB apart.  P sits in tensor memory, in the first 32 columns of the scores it was made
+          // from.
+          constexpr uint32_t idesc = instr_desc_f16(kHd, true);
+          const uint32_t vs = v_lo + (uint32_t)((i % kStages) * (kTileBytes >> 4));
+#pragma unroll
+          for (int t = 0; t < kKeys / kUmmaK; ++t)
+            umma_f16_tmem_a(tmem_base + kOColumn, tmem_base + (uint32_t)((i & 1) * kKeys + t * 8), vs + (uint32_t)(t * (2048 >> 4)),
+                            hi_v, idesc, (i > 0 || t > 0) ? 1u : 0u);
+          umma_commit(&pv_full[i & 1]);
+          umma_commit(&v_empty[i % kStages]);
+        }
+        __syncwarp();
+      }
     }
+    if (!ok && chosen) SIAR_FAIL();
   } else if (warp >= 4) {
     // ---------------- softmax: one thread per row
     const int quad = warp & 3;                 // the tensor-memory lanes this warp may touch
@@ -284,16 +294,22 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const size_t out_row = (size_t)(t0 + (mine ? rg / G : 0)) * prm.Hq + kvh * G + (mine ? rg % G : 0);
     const float row_scale = prm.sl2 * prm.q_factor[out_row];       // of a raw score, times the tile's key factor
     const TileInfo* info = prm.tiles + ((size_t)seq_first + tile0) * prm.Hkv + kvh;
-    TileInfo next = info[0];
+    float k_factors = 0.f, v_logs = 0.f;        // lane l: of tile l of 32
+    unsigned bad_tiles = 0;
     const int n_tiles = nt_max;
     float m_used = -INFINITY, l = 0.f;
     unsigned poisoned = 0;                      // runs of 64 dims in which the row sees a value that is not a number
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
       const int j0 = (tile0 + i) * kKeys;
-      const TileInfo at = next;
-      if (i + 1 < n_tiles) next = info[(size_t)(i + 1) * prm.Hkv];
-      const float sl2 = row_scale * at.k_factor;
+      if (i % 32 == 0) {
+        const TileInfo* t = info + (size_t)min(i + lane, n_tiles - 1) * prm.Hkv;
+        k_factors = t->k_factor;
+        v_logs = t->v_log2;
+        bad_tiles = __ballot_sync(0xffffffffu, (t->bad[0] | t->bad[1]) != 0);
+      }
+      const float sl2 = row_scale * __shfl_sync(0xffffffffu, k_factors, i % 32);
+      const float v_log2 = __shfl_sync(0xffffffffu, v_logs, i % 32);
       if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1) || SIAR_ABORTED()) { ok = false; break; }
       tc_fence_after();
       const uint32_t tmem_s = tmem_base + (uint32_t)((i & 1) * kKeys) + lane_base;
@@ -309,11 +325,12 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int j = 0; j < 64; ++j)
           if (j0 + j >= kv_end) sr[j] = 0xff800000u;      // -inf
       }
-      if (at.bad[0] | at.bad[1]) {
+      if ((bad_tiles >> (i % 32)) & 1) {
         // values that are not numbers stand as zeros in the tile (0 x NaN would reach rows that do not see them)
+        const TileInfo* t = info + (size_t)i * prm.Hkv;
         const int n = kv_end - j0;
         const unsigned long long seen = n >= kKeys ? ~0ull : n > 0 ? (1ull << n) - 1ull : 0ull;
-        poisoned |= (at.bad[0] & seen ? 1u : 0u) | (at.bad[1] & seen ? 2u : 0u);
+        poisoned |= (t->bad[0] & seen ? 1u : 0u) | (t->bad[1] & seen ? 2u : 0u);
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -325,7 +342,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       // The reference is kHeadroom below the largest s + log2(value factor) so far, so that p is at most
       // 2^(kHeadroom + kRescaleGap) and float16 holds it down to 2^-32 of the largest.  A row whose raw scores are
       // all hidden (or NaN) has no maximum yet.
-      const float m_new = fmaxf(m_used, raw * sl2 + at.v_log2 - kHeadroom);
+      const float m_new = fmaxf(m_used, raw * sl2 + v_log2 - kHeadroom);
       const bool need = m_new > m_used + kRescaleGap;      // also true for the first finite maximum
       if (i > 0 && __any_sync(0xffffffffu, need)) {
         // O may be touched once the previous tile's P.V has completed
@@ -346,10 +363,10 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
       if (need) m_used = m_new;
-      const float neg_m = m_used == -INFINITY ? 0.f : at.v_log2 - m_used;
+      const float neg_m = m_used == -INFINITY ? 0.f : v_log2 - m_used;
       // P = 2^(s c - m) as float16 pairs, written over the first 32 columns of the scores in tensor
       // memory (this thread holds its whole row in registers by now).  The next scores for this
-      // buffer are issued after the P.V that reads P, and the tensor pipe keeps that order.
+      // buffer are issued after the P.V that reads P is done.
       unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
       const unsigned long long by = pair_of(sl2, sl2), off = pair_of(neg_m, neg_m);
       uint32_t pw[32];
@@ -366,7 +383,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       SIAR_TMEM_ST_32(tmem_s, pw);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       const float2 both = halves_of(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
-      l += (both.x + both.y) * at.v_inverse;
+      l += (both.x + both.y) * __int_as_float((127 - (int)v_log2) << 23);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
@@ -499,8 +516,6 @@ widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_s
     TileInfo t;
     t.k_factor = 1.f / up[0];
     t.v_log2 = -(float)((int)(__float_as_uint(up[1]) >> 23) - 127);
-    t.v_inverse = up[1];
-    t.unused = 0.f;
     t.bad[0] = bad_s[0][2] | (unsigned long long)bad_s[0][3] << 32;
     t.bad[1] = NG == 2 ? bad_s[NG - 1][2] | (unsigned long long)bad_s[NG - 1][3] << 32 : D == 128 ? t.bad[0] : 0ull;
     tiles[(size_t)(first + tile) * Hkv + kvh] = t;
