@@ -19,7 +19,8 @@
 // ends).  In the products' kernel neither the tensor pipe (37 %) nor the exponentials (37 %) are busy all the time: a
 // tile is a chain scores -> largest -> exponentials -> P -> O, some 1,700 cycles for a block alone and 1,900 with two on an
 // SM, at 1.7 GHz.  (With scores and P.V issued by one thread of a warp, and a load a tile for its factors, the two took
-// 66 and 104 us.)  Tried and no faster: two threads a row (131 us), all key tiles shared out evenly over two blocks an
+// 66 and 104 us.)  Products are fed from shared memory at 128 bytes a clock and read Q again for every 64 keys, 512
+// clocks a tile.  Tried and no faster: two threads a row (131 us), all key tiles shared out evenly over two blocks an
 // SM (104 to 111, the prompt 68 to 73), four-stage rings.  Reading the cache back as bfloat16 pages for the bfloat16
 // kernel took 87 and 199 us, with 2.5 times the rounding error.
 #include "kv_quant.cuh"
@@ -650,7 +651,8 @@ SIAR_DEFINE_PDL_SWITCH()
 // `average`) key tiles.  Measured on B200 at 128 dims: a block alone on its SM takes 7 us and 0.95 us a tile, two on
 // every SM 0.66 us a tile and SM, the last round a third of a block more; parts (`row_floats` floats each) are written and
 // read again at 3.6 TB/s by a kernel of its own.  A chunk of 128 tokens on 8,000 held (32 heads on 8): one part 139 us, 8
-// parts 54; a prompt of 2,048: one part 69 us, two 109.
+// parts 54; a chunk of 515 on 8,191 (24 on 8): parts 1, 2, 3, 4, 5, 6, 8 take 134, 101, 114, 99, 97, 109, 109 us (the rule
+// takes 4); a prompt of 2,048: one part 64 us, two over 100.
 extern "C" int siar_attn_quant_tc_parts(int blocks, int longest, float average, long long row_floats, int sms) {
   int best = 1;
   float best_cost = 1e30f;
