@@ -3,11 +3,11 @@
 //
 // Formats (a row is one position of one kv head, D values x_0 .. x_{D-1}; keys are held rotated):
 //   8 bits  codes int8 [pages][Hkv][page_tokens][D], scales float32 [pages][Hkv][page_tokens]
-//           s = max|x| / 127,  c_d = rint(x_d / s),  value c_d * s.   The reference's int8 cache has
+//           s = max|x| (1/127),  c_d = rint(x_d / s),  value c_d * s.   The reference's int8 cache has
 //           the same row scale (model/kv_cache.py:58-67), rounded to 16 bits there, 32 here.
 //   4 bits  codes uint8 [pages][Hkv][page_tokens][D/2] (dim 2i in the low half of byte i, 2i+1 in the
 //           high half), scales bfloat16 [pages][Hkv][page_tokens][ceil(D/64)][2]: for every run of 64
-//           dims s = bf16(max(x)/15 - min(x)/15), m = bf16(min(x) + 8 s), c_d = rint((x_d - m) / s) + 8
+//           dims s = bf16(max(x) (1/15) - min(x) (1/15)), m = bf16(min(x) + 8 s), c_d = rint((x_d - m) / s) + 8
 //           within 0..15, value (c_d - 8) * s + m.  s and m are rounded to 16 bits because they are a
 //           ninth of the format's bytes; the codes are taken against the rounded ones, so that costs
 //           at most 15 * 2^-9 steps at the ends of the range.
@@ -294,7 +294,7 @@ rope_quantize_wide_kernel(const __nv_bfloat16* qkv, void* q_to, float* q_factor,
             }
             uint32_t c[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) c[e] = whole_bits(corrected(x[e], by));       // |x| <= 127 s: no code leaves its byte
+            for (int e = 0; e < 16; ++e) c[e] = whole_bits(corrected(x[e], by));       // |x| <= 127 s (1 + 2^-23): no code leaves its byte
             uint32_t b[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)

@@ -117,14 +117,16 @@ __device__ __forceinline__ float quotient(float x, const Divisor& by) { return c
 // rint(y) for |y| < 2^22, in the low bits (two's complement): adding 1.5 x 2^23 rounds to a whole number.
 __device__ __forceinline__ uint32_t whole_bits(float y) { return __float_as_uint(__fadd_rn(y, 12582912.f)); }
 
-// The scale of a row in 8 bits, and a code against it in the low byte (0 without a scale).
-__device__ __forceinline__ float scale8(float amax) { return __fdiv_rn(amax, 127.f); }
+// The scale of a row in 8 bits, and a code against it in the low byte (0 without a scale).  127 and 15 divide by a product
+// with the float32 reciprocal, as torch divides a tensor on the GPU by a number: where a scale is rounded to 16 bits, the
+// last bit of the quotient decides about one run in 500,000.
+__device__ __forceinline__ float scale8(float amax) { return __fmul_rn(amax, 1.f / 127.f); }
 __device__ __forceinline__ uint32_t code8(float x, const Divisor& by, bool bad) {
   return bad ? 0u : whole_bits(fmaxf(-127.f, fminf(127.f, quotient(x, by))));
 }
 // Scale and mid of a run in 4 bits, and a code against them in the low four bits.
 __device__ __forceinline__ __nv_bfloat162 scale4(float lo, float hi, bool bad) {
-  const __nv_bfloat16 s = __float2bfloat16_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)));
+  const __nv_bfloat16 s = __float2bfloat16_rn(__fsub_rn(__fmul_rn(hi, 1.f / 15.f), __fmul_rn(lo, 1.f / 15.f)));
   const __nv_bfloat16 m = __float2bfloat16_rn(__fadd_rn(lo, 8.f * __bfloat162float(s)));
   const float nan = __int_as_float(0x7fc00000);
   return bad ? __floats2bfloat162_rn(nan, nan) : __halves2bfloat162(s, m);

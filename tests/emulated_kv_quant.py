@@ -21,7 +21,7 @@ def quantise(x, bits):
     """float32 [..., D] -> (codes, scales) as the cache holds them."""
     finite = torch.isfinite(x)
     if bits == 8:
-        s = x.abs().amax(-1) / 127.0
+        s = x.abs().amax(-1) * (1 / 127)                  # the float32 reciprocal, as the kernels
         c = torch.round(x / torch.where(s > 0, s, 1.0)[..., None]).clamp(-127, 127)
         bad = ~finite.all(-1)
         c = torch.where(bad[..., None] | (s <= 0)[..., None], torch.zeros_like(c), c)
@@ -30,7 +30,7 @@ def quantise(x, bits):
     for at in range(0, x.shape[-1], GROUP):
         g = x[..., at:at + GROUP]
         lo, hi = g.amin(-1), g.amax(-1)
-        s = (hi / 15.0 - lo / 15.0).to(torch.bfloat16).float()
+        s = (hi * (1 / 15) - lo * (1 / 15)).to(torch.bfloat16).float()
         m = (lo + 8.0 * s).to(torch.bfloat16).float()
         c = (torch.round((g - m[..., None]) / torch.where(s > 0, s, 1.0)[..., None]) + 8.0).clamp(0, 15)
         bad = ~finite[..., at:at + GROUP].all(-1)
