@@ -6,9 +6,9 @@
 //   8 bits  s_j = sk_j (q . ck_j),                            out = sum_j (p_j sv_j) cv_j / sum_j p_j
 //   4 bits  s_j = sum_g sk_jg (q_g . (ck_jg - 8)) + mk_jg sum(q_g),
 //           out_g = (sum_j (p_j sv_jg) cv_jg + sum_j p_j (mv_jg - 8 sv_jg)) / sum_j p_j
-// A query row becomes whole numbers of 16 bits (largest element 32512; a step is 2^-16 of it, where
-// bfloat16 keeps 8 bits of every element), split into two bytes that take two columns of the product;
-// the integer scores are exact.  For the value product the p_j sv_j of one step of keys become
+// A query row becomes whole numbers of 16 bits in both formats (largest element 32512: a step is 1 / 32512 of it, also
+// for the small elements of a row in which one stands out, where bfloat16 would keep 8 bits of each), split into two
+// bytes that take two columns of the product; the integer scores are exact.  For the value product the p_j sv_j of one step of keys become
 // whole numbers of 16 bits too, against the largest of the step, again two bytes in two columns: within a
 // step 2^-17 of the largest is lost, and a step's integer sum goes into the 32-bit accumulators with the
 // step's own factor, so nothing is lost between steps.  Statistics and sums are 32 bits.
@@ -30,7 +30,7 @@
 // in block order by the block that finishes it last.
 //
 // Measured (keys and values at the measured copy rate in brackets): 64 sequences of up to 4,500 keys, 8 bits, 32 heads on
-// 8, 80 us (71); 64 of up to 9,000 in 4 bits 93 (77); one of 130,018 in 8 bits 50 (42); one of 34 keys 6.2, the
+// 8, 80 us (71); 64 of up to 9,000 in 4 bits 96 (77); one of 130,018 in 8 bits 50 (42); one of 34 keys 6.2, the
 // latency of the chain batch -> block table -> keys -> softmax -> values.  Three blocks an SM for 8 bits 82 us, rings of
 // four stages there 83.
 #include "attention_mma.cuh"
@@ -93,10 +93,7 @@ struct QuantAttn {
   static_assert(kBlocksPerSM * (kSmem + 1024 + 1024 + (NT == 1 ? 1500 : NT == 2 ? 2100 : 3300)) <= 228 * 1024, "blocks an SM");
 };
 constexpr float kFixedP = 65500.f;                // p sv of a step's largest term, as a whole number
-// A query row's largest element as a whole number.  8 bits: 127 x 256.  4 bits: 2032; the even dims' numbers are
-// taken 16 times, because their codes are read from the low halves of the cache's bytes and the odd dims' from
-// the high halves, where they stand for 16 times as much: both sums are 16 times q . code, with no shift.
-template <int BITS> constexpr float kFixedQ = BITS == 8 ? 32512.f : 2032.f;
+constexpr float kFixedQ = 32512.f;                // a query row's largest element, as a whole number: 127 x 256
 
 // D (int32) = C + A B for bytes; ASIGN / BSIGN: signed operands, FIRST: C is zero.
 template <bool ASIGN, bool BSIGN, bool FIRST>
@@ -447,15 +444,14 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
 #pragma unroll
       for (int sh = 16; sh > 0; sh >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
       const bool fine = isfinite(amax) && amax > 1e-30f;       // else zeros; NaN through the factor where not finite
-      const float up = fine ? kFixedQ<BITS> / amax : 0.f;
+      const float up = fine ? kFixedQ / amax : 0.f;
       int sum[NG];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) sum[gr] = 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        int v = fine ? __float2int_rn(a[i] * up) : 0;
+        const int v = fine ? __float2int_rn(a[i] * up) : 0;
         sum[BITS == 8 ? 0 : 32 * i / kQuantGroup] += v;
-        if (BITS == 4 && !(lane & 1)) v *= 16;
         const int hi = (v + 128) >> 8;             // v = 256 hi + lo, lo in -128 .. 127
         // 4 bits: a word holds eight dims, the even ones in its low halves, the odd ones in its high halves
         const int d = 32 * i + lane, at = BITS == 8 ? d : (d & ~7) + ((d & 1) << 2) + ((d & 7) >> 1);
@@ -467,7 +463,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
         sum[gr] = __reduce_add_sync(0xffffffffu, sum[gr]);
         if (lane == 0) qsum_s[r][gr] = sum[gr];
       }
-      if (lane == 0) f_s[r] = fine ? P.sl2 * (amax / (kFixedQ<BITS> * (BITS == 8 ? 1.f : 16.f))) : amax - amax;
+      if (lane == 0) f_s[r] = fine ? P.sl2 * (amax / kFixedQ) : amax - amax;
     }
     __syncthreads();
 #pragma unroll
@@ -489,7 +485,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       l_r[nt] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        qs[nt][gr] = 16 * qsum_s[4 * nt + q4][gr];      // (4 bits only)
+        qs[nt][gr] = qsum_s[4 * nt + q4][gr];           // (4 bits only)
         qsf[nt][gr] = (float)qs[nt][gr];
         z[nt][gr] = 0.f;
       }
@@ -563,13 +559,13 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
             }
             uint32_t w[4];                         // 64 dims: chunks 2 gr and 2 gr + 1
             ldmatrix_x4(w, k_addr + at16[gr] + k * 16 * RB);
-            constexpr uint32_t LO = 0x0f0f0f0fu, HI = 0xf0f0f0f0u;
+            constexpr uint32_t LO = 0x0f0f0f0fu;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma_bytes<false, true, false>(acc[nt], w[2 * h] & LO, w[2 * h + 1] & LO, w[2 * h] & HI, w[2 * h + 1] & HI,
-                                              qb[2 * gr + h][nt][0], qb[2 * gr + h][nt][1]);
+                mma_bytes<false, true, false>(acc[nt], w[2 * h] & LO, w[2 * h + 1] & LO, (w[2 * h] >> 4) & LO,
+                                              (w[2 * h + 1] >> 4) & LO, qb[2 * gr + h][nt][0], qb[2 * gr + h][nt][1]);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {

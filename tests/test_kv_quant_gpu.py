@@ -683,3 +683,59 @@ def test_threads_that_call_on_one_stream_and_on_their_own(bits, new):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new", [[1, 1], [3, 2]])
+@pytest.mark.parametrize("dim,channel", [(128, 6), (128, 77), (64, 37)])
+@pytest.mark.parametrize("ratio", [30.0, 100.0, 1000.0])
+def test_queries_with_one_large_channel(bits, new, dim, channel, ratio):
+    """One channel of every query is ``ratio`` times the others, as some channels of real models are; the cache's
+    keys are zero there, so the scores are ordinary ones and what counts is how the other channels are held beside the
+    large one.  On the codes a query row becomes whole numbers of 16 bits: its largest element a is 32512 of them, so
+    each element is off by at most a / 65024, evenly within that (these queries are bfloat16 and not rotated:
+    nothing else rounds them).  With d = that rounding of the row, o the result and p the probabilities, to first order
+
+        o' - o = scale sum_i d_i sum_j p_j k_ji (v_j - o),
+
+    so its variance is scale^2 (a / 32512)^2 / 12 sum_i (sum_j p_j k_ji (v_j - o))^2.  The codes' sum p_j s_j is rounded to
+    1 / 65500 of a step's largest (variance P^2 / 12 a key, P = p_max / 65500 times a code times its scale: at most
+    max|v| in 8 bits, twice that in 4), the result to bfloat16 (at most u^2 / 3 of its square, u = 2^-8).  The rms
+    over all results has to be that to half as much again (some 1,000 independent roundings, so a few percent by chance; second
+    order: scores move by at most scale sum |k| a / 65024 < 0.2)."""
+    heads, kv_heads, held = 8, 2, [700, 320]
+    scale, g = dim ** -0.5, heads // kv_heads
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=dim + channel, stale="random")
+    gen = torch.Generator().manual_seed(int(ratio) + channel)
+    if bits == 8:
+        b.kv.k = torch.randint(-127, 128, b.kv.k.shape, generator=gen).to(torch.int8)
+        b.kv.k[..., channel] = 0
+        b.kv.k_scale = torch.full_like(b.kv.k_scale, 1 / 64)
+    else:
+        code = torch.randint(0, 16, b.kv.k.shape[:-1] + (dim,), generator=gen).to(torch.uint8)
+        code[..., channel] = 8
+        b.kv.k = code[..., 0::2] | (code[..., 1::2] << 4)
+        b.kv.k_scale[..., 0], b.kv.k_scale[..., 1] = 0.25, 0.0
+    x = b.qkv.view(b.tokens, -1, dim)
+    x[:, heads:heads + kv_heads] = 0.0                        # the new tokens' keys
+    x[:, :heads, channel] = ratio * x[:, :heads, channel].sign()
+    out = attend(b, b.entry(DEV), scale=scale).cpu().double().view(b.tokens, heads, dim)
+    ops.check_status(DEV)
+    want, q = plain_of(b)
+    k_all, v_all = eq.values(want.k, want.k_scale), eq.values(want.v, want.v_scale)
+    square, expected = [], []
+    for i, (c, m) in enumerate(zip(held, new)):
+        rows = want.block_table[int(b.slot_ids[i]), :-(-(c + m) // 64)].long()
+        k, v = (t[rows].transpose(1, 2).reshape(-1, kv_heads, dim) for t in (k_all, v_all))
+        for t in range(m):
+            for h in range(heads):
+                kk, vv, row = k[:c + t + 1, h // g], v[:c + t + 1, h // g], q[int(b.q_start[i]) + t, h].double()
+                p = torch.softmax(scale * (kk @ row), 0)
+                o = p @ vv
+                step = scale * float(row.abs().max()) / 32512
+                by_query = step ** 2 / 12 * ((p[:, None] * kk).T @ (vv - o)).square().sum(0)
+                top = float(p.max() * vv.abs().max()) * (1 if bits == 8 else 2) / 65500
+                expected.append(by_query + len(kk) * top ** 2 / 12 + 2.0 ** -16 / 3 * o.square())
+                square.append((out[int(b.q_start[i]) + t, h] - o).square())
+    rms, most = (float(torch.cat(s).mean().sqrt()) for s in (square, expected))
+    assert rms <= 1.5 * most, (rms, most)
