@@ -35,6 +35,7 @@
 // four stages there 83.
 #include "attention_mma.cuh"
 #include "kv_quant.cuh"
+#include "load_ring.h"
 #include "tcgen05.cuh"
 
 #include <cuda_fp16.h>
@@ -311,7 +312,9 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   // ---- this warp's loads: the same walk, ahead of the computation
   QuantSeq lu = cu;
   int l_rt = c_rt, l_kvh = c_kvh, l_t = c_t, l_left = n_steps;
-  int issued = 0, consumed = 0;
+  LoadRing<C::kStages> ring;
+  // the same answer in every lane: what follows is work of the whole warp
+  auto arrived = [&](int stage, int parity) { return __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], parity)) != 0; };
   bool absent_page = false;
   auto next_seq = [&](const QuantSeq& s) {        // the next sequence that has steps (there is one)
     int b = s.b + 1;
@@ -330,14 +333,14 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   ask_pages();
   fetch(cu, c_rt, c_kvh, c_t, n_steps);
   auto issue_next = [&]() {
-    while (l_left > 0) {
+    while (l_left > 0 && ring.room()) {
       const int w0 = l_t * C::kBlockKeys + warp * WK;
       const bool has = w0 < lu.len;
       if (has) {
         int page = __shfl_sync(0xffffffffu, l_pages, l_t - l_page0);
         if (page < 0 || page >= P.n_pages) { absent_page = true; page = 0; }
+        const int s = ring.next();
         if (lane == 0) {
-          const int s = issued % C::kStages;
           const int row = (page * P.Hkv + l_kvh) * P.page_tokens + w0 - page_index(w0) * P.page_tokens;
           unsigned char* kt = smem + C::kTiles + (s * 4 + warp) * 2 * C::kTileBytes;
           unsigned char* sc = smem + C::kScales + (s * 4 + warp) * 2 * C::kScaleBytes;
@@ -348,7 +351,6 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
           tma_load_2d(kt + C::kTileBytes, &v_map, bar, 0, row);
           bulk_load(sc + C::kScaleBytes, (const unsigned char*)P.v_scale + (size_t)row * (4 * NG), C::kScaleBytes, bar);
         }
-        ++issued;
       }
       --l_left;
       if (++l_t == lu.T) {
@@ -374,7 +376,6 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
   int qs[NT][NG];
   float qsf[NT][NG];
   uint32_t qb[D / 32][NT][2];
-  bool expired = false;
   // where the lane's row of an ldmatrix stands: (keys 0-7 | 8-15) x (chunk 2c, 2c + 1) of a tile's first 16 keys; 16
   // keys on is 16 rows on, whole periods of the swizzle
   uint32_t at16[RB / 32];
@@ -497,8 +498,8 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     for (int st = 0; st < seg; ++st) {
       const int w0 = (c_t + st) * C::kBlockKeys + warp * WK;
       if (w0 >= cu.len) break;
-      const int stage = consumed % C::kStages;
-      if (!expired && !mbar_wait(&bars[warp][stage], (consumed / C::kStages) & 1)) expired = true;
+      if (!ring.take(arrived)) break;              // the result is reported as lost; the joins still take place
+      const int stage = ring.stage();
       unsigned char* kt = smem + C::kTiles + (stage * 4 + warp) * 2 * C::kTileBytes;
       unsigned char* vt = kt + C::kTileBytes;
       unsigned char* sc = smem + C::kScales + (stage * 4 + warp) * 2 * C::kScaleBytes;
@@ -751,7 +752,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
             }
           }
       }
-      ++consumed;
+      ring.release();
       __syncwarp();                                          // every lane has read the stage
       issue_next();
     }
@@ -934,8 +935,9 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
       }
     }
   }
+  ring.drain(arrived);                            // (empty unless a wait ran out)
   if (absent_page || past_table) atomicOr(P.status, kStatusBadPage);
-  if (lane == 0 && expired) atomicOr(P.status, kStatusWaitExpired);
+  if (lane == 0 && ring.expired) atomicOr(P.status, kStatusWaitExpired);
 }
 
 // ------------------------------------------------------------------ host
