@@ -139,6 +139,7 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr int kTileBytes = kKeys * kHd * 2;        // 8 KiB per half
   pdl_launch_dependents();
   pdl_wait();
+  asm volatile("fence.proxy.async.global;" ::: "memory");      // queries and tiles that the kernels in front stored, for the TMA
   // blocks with the most keys (the last rows, of all sequences and heads) start first: the tail of the grid is made
   // of short blocks
   const int part = blockIdx.x % prm.splits, kvh = blockIdx.x / prm.splits % prm.Hkv, b = blockIdx.x / prm.splits / prm.Hkv;

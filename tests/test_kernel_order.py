@@ -1,0 +1,26 @@
+"""Orders that kernels have to keep and no run shows: read off the sources."""
+
+import pytest
+
+from simple_inference_autoresearch_b200.kernels import build
+
+
+def body_of(unit, kernel):
+    """The text of a kernel from its name to the end of its braces."""
+    text = (build.CSRC / f"{unit}.cu").read_text()
+    at = text.index("{", text.index(f"\n{kernel}("))
+    depth, i = 1, at + 1
+    while depth:
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        i += 1
+    return text[at:i]
+
+
+@pytest.mark.parametrize("unit,kernel", [("attention_quant", "attn_quant_kernel"), ("attention_quant_tc", "attn_quant_tc_kernel")])
+def test_loads_of_what_kernels_in_front_stored_follow_a_fence(unit, kernel):
+    """Rows, queries and tiles are written by ordinary stores of the kernel in front and read here through the asynchronous
+    proxy: behind the wait for that kernel, in front of the first load, the two have to be ordered."""
+    body = body_of(unit, kernel)
+    wait, fence = body.index("pdl_wait();"), body.index("fence.proxy.async.global;")
+    loads = [body.index(w) for w in ("tma_load_2d(", "tma_load_3d(", "bulk_load(") if w in body]
+    assert wait < fence < min(loads)
