@@ -137,7 +137,6 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr int kHalves = kHd / 64;                  // 64-dim (128-byte) column blocks of a row
   constexpr int kQBytes = kRows * kHd * 2;           // 16 KiB per half
   constexpr int kTileBytes = kKeys * kHd * 2;        // 8 KiB per half
-  pdl_launch_dependents();
   pdl_wait();
   asm volatile("fence.proxy.async.global;" ::: "memory");      // queries and tiles that the kernels in front stored, for the TMA
   // blocks with the most keys (the last rows, of all sequences and heads) start first: the tail of the grid is made
@@ -184,6 +183,10 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Tensor memory is taken behind the wait (all kernels in front have given theirs back) and in front of this, so the next
+  // kernel starts only when every block here has its columns: a product takes its own in front of its wait, and holding them
+  // beside a block that still asks for columns it would wait for that block without end.
+  pdl_launch_dependents();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
   const bool dead = (*(volatile int*)prm.status & kStatusWaitExpired) != 0;
 

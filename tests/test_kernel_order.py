@@ -24,3 +24,12 @@ def test_loads_of_what_kernels_in_front_stored_follow_a_fence(unit, kernel):
     wait, fence = body.index("pdl_wait();"), body.index("fence.proxy.async.global;")
     loads = [body.index(w) for w in ("tma_load_2d(", "tma_load_3d(", "bulk_load(") if w in body]
     assert wait < fence < min(loads)
+
+
+def test_tensor_memory_is_taken_between_the_wait_and_the_next_kernels_start():
+    """Two blocks of 256 columns fill an SM's 512.  Products take columns in front of their wait for the kernel in front;
+    one that starts beside a block of this kernel that has none yet would leave the two waiting for each other.  And in
+    front of this kernel's own wait a product may still be about to take its columns."""
+    body = body_of("attention_quant_tc", "attn_quant_tc_kernel")
+    assert body.index("pdl_wait();") < body.index("tmem_alloc(") < body.index("__syncthreads();") < body.index("pdl_launch_dependents();")
+    assert body.count("pdl_launch_dependents();") == 1 and body.count("tmem_alloc(") == 1
