@@ -65,6 +65,7 @@ struct QuantAttnParams {
   int page_shift;                // log2(page_tokens), or -1
   int fused;                     // rotate and (write_kv) store the new token here; one token a sequence
   int write_kv;
+  int most_new;                  // sequences with more new tokens than this are left to another kernel
   float sl2;                     // scale * log2(e)
 };
 
@@ -184,7 +185,7 @@ attn_quant_kernel(const __grid_constant__ QuantAttnParams P, const __grid_consta
     s.len = min(s.base + s.q_len, cap);
     past_table |= s.base + s.q_len > cap;
     s.T = max(0, (s.len + C::kBlockKeys - 1) / C::kBlockKeys);
-    s.row_tiles = max(0, (s.q_len * G + C::kRows - 1) / C::kRows);
+    s.row_tiles = s.q_len <= P.most_new ? max(0, (s.q_len * G + C::kRows - 1) / C::kRows) : 0;
     return s;
   };
   // ---- this block's share of all block steps
@@ -1016,12 +1017,14 @@ extern "C" unsigned long long siar_capture_id(void* stream) {
 // Attention of the batch's new tokens over the quantised cache.  fused: one new token a sequence, whose
 // query and key are rotated here (inv_freq; nullptr: not rotated) and whose key and value are stored
 // (write_kv) and attended to; else the tokens' rows are in the cache and the queries are as they are to be
-// used, in qkv or (q16 not nullptr; qkv is not read then) as siar_rope_quantize_q16 leaves them.  counters: siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
+// used, in qkv or (q16 not nullptr; qkv is not read then) as siar_rope_quantize_q16 leaves them.  Sequences with more than
+// most_new new tokens are passed over (max_q_len and max_kv_len are those of the others).  counters:
+// siar_attn_quant_counters int32 zeros, left zero; scratch: siar_attn_quant_scratch_floats floats.
 static int siar_attn_quant_of(int bits, const void* qkv, const void* q16, const float* q_factor, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
                                const int* block_table, const int* slot_ids, const int* q_start, const int* base_len,
                                const float* inv_freq, void* out, int* counters, float* scratch, int B, int Hq, int Hkv, int D,
                                int page_tokens, int max_pages, int n_pages, int max_q_len, int max_kv_len, int sm_count,
-                               int fused, int write_kv, float scale, int* status, void* stream) {
+                               int fused, int write_kv, int most_new, float scale, int* status, void* stream) {
   if (B == 0 || max_q_len == 0) return 0;
   if (Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || page_tokens <= 0 || page_tokens % 64 != 0 || (bits != 8 && bits != 4) ||
       n_pages <= 0 || max_pages <= 0 || max_kv_len <= 0 || sm_count <= 0 || (fused && (max_q_len != 1 || q16 != nullptr)) ||
@@ -1030,7 +1033,7 @@ static int siar_attn_quant_of(int bits, const void* qkv, const void* q16, const 
   QuantAttnParams p = {(const __nv_bfloat16*)qkv, (const __half*)q16, q_factor, (uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids,
                        q_start, base_len, inv_freq, (__nv_bfloat16*)out, scratch, counters, status, B, Hq, Hkv, page_tokens,
                        max_pages, n_pages, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, fused,
-                       write_kv, scale * 1.4426950408889634f};
+                       write_kv, most_new, scale * 1.4426950408889634f};
   cudaStream_t s = (cudaStream_t)stream;
   const int blocks = blocks_of(bits, B, Hkv, D, max_q_len * (Hq / Hkv), max_kv_len, sm_count);
   const int nt = column_tiles_of(max_q_len * (Hq / Hkv));

@@ -47,11 +47,17 @@ struct TileInfo {
   unsigned long long bad[2];     // bit r: the value of position r is not a number (in its first, second run of 64 dims)
 };
 
+// The sequences of a launch, by their places in the batch.
+constexpr int kMostSeqs = 64;
+struct SeqList {
+  unsigned short b[kMostSeqs];
+};
+
 struct QuantTcParams {
   __nv_bfloat16* out;
   float* scratch;                // parts of rows: [tokens x heads][splits][head_dim + 8]
   const TileInfo* tiles;         // [tiles][Hkv]
-  const int* seq_tiles;          // [B]: the sequence's first tile, and how many it has
+  const int* seq_tiles;          // [listed sequences]: the sequence's first tile, and how many it has
   const float* q_factor;         // [tokens][Hq]
   const int* q_start;
   const int* base_len;
@@ -124,7 +130,7 @@ __host__ __device__ inline int key_tiles(int base, int q_len, int row0, int G, i
 template <int kHd>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM)
 attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const QuantTcParams prm) {
+                     const __grid_constant__ CUtensorMap tmV, const QuantTcParams prm, const __grid_constant__ SeqList seqs) {
   extern __shared__ unsigned char smem_dyn[];
   __shared__ __align__(8) uint64_t q_full;
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_full[2];
@@ -141,7 +147,8 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   asm volatile("fence.proxy.async.global;" ::: "memory");      // queries and tiles that the kernels in front stored, for the TMA
   // blocks with the most keys (the last rows, of all sequences and heads) start first: the tail of the grid is made
   // of short blocks
-  const int part = blockIdx.x % prm.splits, kvh = blockIdx.x / prm.splits % prm.Hkv, b = blockIdx.x / prm.splits / prm.Hkv;
+  const int part = blockIdx.x % prm.splits, kvh = blockIdx.x / prm.splits % prm.Hkv, at = blockIdx.x / prm.splits / prm.Hkv;
+  const int b = seqs.b[at];
   const int G = prm.Hq / prm.Hkv;
   const int tile_rows = (kRows / G) * G;             // rows in use: whole tokens only
   const int t0 = prm.q_start[b];
@@ -150,11 +157,11 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int row0 = (gridDim.y - 1 - blockIdx.y) * tile_rows;
   if (row0 >= rows_total) return;
   const int base = prm.base_len[b];
-  const int all_tiles = key_tiles(base, q_len, row0, G, tile_rows, prm.seq_tiles[2 * b + 1]);
+  const int all_tiles = key_tiles(base, q_len, row0, G, tile_rows, prm.seq_tiles[2 * at + 1]);
   const int parts = min(prm.splits, all_tiles);
   if (part >= parts) return;
   const int tile0 = all_tiles * part / parts, nt_max = all_tiles * (part + 1) / parts - tile0;
-  const int seq_first = prm.seq_tiles[2 * b];        // the sequence's first tile of the widened cache
+  const int seq_first = prm.seq_tiles[2 * at];        // the sequence's first tile of the widened cache
 
   const uint32_t dyn = smem_u32(smem_dyn);
   unsigned char* sm = smem_dyn + ((1024u - (dyn & 1023u)) & 1023u);
@@ -444,20 +451,20 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
 
 // ------------------------------------------------------------------ widening
-// grid (tiles of the longest sequence, Hkv, B), 256 threads.  Rows behind a sequence's last token are zeros.
+// grid (tiles of the longest sequence, Hkv, listed sequences), 256 threads.  Rows behind a sequence's last token are zeros.
 template <int D, int BITS>
 __global__ void __launch_bounds__(256)
 widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_scale, const void* v_scale,
                    const int* block_table, const int* slot_ids, const int* q_start, const int* base_len, __half* k_out,
-                   __half* v_out, TileInfo* tiles, int* seq_tiles, int B, int Hkv, int page_tokens, int max_pages,
-                   int n_pages, int tiles_out, int* __restrict__ status) {
+                   __half* v_out, TileInfo* tiles, int* seq_tiles, const __grid_constant__ SeqList seqs, int Hkv, int page_tokens,
+                   int max_pages, int n_pages, int tiles_out, int* __restrict__ status) {
   constexpr int NG = BITS == 8 ? 1 : D / kQuantGroup;
   pdl_launch_dependents();
   __shared__ float bound_s[4];
   __shared__ unsigned bad_s[2][4];                   // [run][32 rows of K, K, V, V]
   __shared__ int first_s;
   pdl_wait();
-  const int tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int tile = blockIdx.x, kvh = blockIdx.y, at = blockIdx.z, b = seqs.b[at];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cap = max_pages * page_tokens;
   auto length_of = [&](int i) { return max(0, min(base_len[i] + q_start[i + 1] - q_start[i], min(cap, (int)gridDim.x * kKeys))); };
@@ -468,7 +475,7 @@ widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_s
   int page = tile < mine ? block_table[(size_t)slot * max_pages + pos / page_tokens] : 0;
   if (warp == 7) {
     int sum = 0;
-    for (int i = lane; i < b; i += 32) sum += (length_of(i) + kKeys - 1) / kKeys;
+    for (int i = lane; i < at; i += 32) sum += (length_of(seqs.b[i]) + kKeys - 1) / kKeys;
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) first_s = sum;
   }
@@ -501,8 +508,8 @@ widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_s
   __syncthreads();
   const int first = first_s;
   if (tile == 0 && kvh == 0 && threadIdx.x == 0) {
-    seq_tiles[2 * b] = first;
-    seq_tiles[2 * b + 1] = max(0, min(mine, tiles_out - first));
+    seq_tiles[2 * at] = first;
+    seq_tiles[2 * at + 1] = max(0, min(mine, tiles_out - first));
     if (first + mine > tiles_out) atomicOr(status, kStatusLengthPastGrid);      // host lengths that fall short
   }
   if (tile >= mine || first + tile >= tiles_out) return;
@@ -565,11 +572,11 @@ widen_tiles_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const void* k_s
 }
 
 // ------------------------------------------------------------------ parts of rows
-// One warp a row (token, head).
+// One warp a row (token, head); rows of sequences that are not listed are passed over.
 template <int D>
 __global__ void __launch_bounds__(256)
 attn_quant_join_kernel(const float* scratch, __nv_bfloat16* out, const int* seq_tiles, const int* q_start, const int* base_len,
-                       int N, int B, int Hq, int Hkv, int splits) {
+                       const __grid_constant__ SeqList seqs, int listed, int N, int B, int Hq, int Hkv, int splits) {
   pdl_launch_dependents();
   pdl_wait();
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -583,8 +590,15 @@ attn_quant_join_kernel(const float* scratch, __nv_bfloat16* out, const int* seq_
   }
   const int t0 = q_start[b], q_len = q_start[b + 1] - t0;
   if (t < t0 || t >= t0 + q_len) return;
+  int at = -1;
+#pragma unroll
+  for (int i = 0; i < kMostSeqs; i += 32) {
+    const unsigned hit = __ballot_sync(0xffffffffu, i + lane < listed && seqs.b[i + lane] == b);
+    if (hit != 0) at = i + __ffs(hit) - 1;
+  }
+  if (at < 0) return;
   const int rg = (t - t0) * G + head % G;
-  const int parts = min(splits, key_tiles(base_len[b], q_len, rg / tile_rows * tile_rows, G, tile_rows, seq_tiles[2 * b + 1]));
+  const int parts = min(splits, key_tiles(base_len[b], q_len, rg / tile_rows * tile_rows, G, tile_rows, seq_tiles[2 * at + 1]));
   if (parts < 2) return;
   const float* part = scratch + (size_t)row * splits * (D + 8);
   float m = -INFINITY, l = 0.f, acc[D / 32];
@@ -629,7 +643,7 @@ static bool query_map(const void* q, int n_tokens, int Hq, int Hkv, int hd, CUte
 
 template <int D>
 static int launch_tc(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const QuantTcParams& prm, dim3 grid,
-                     int N, int B, cudaStream_t s) {
+                     const SeqList& seqs, int listed, int N, int B, cudaStream_t s) {
   constexpr int smem = smem_bytes(D) + 1024;
   static bool attr[64] = {};                       // a property of the device's copy of the kernel
   int dev = 0;
@@ -639,10 +653,21 @@ static int launch_tc(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUten
     if (e != cudaSuccess) return (int)e;
     attr[dev] = true;
   }
-  const cudaError_t e = launch_kernel(attn_quant_tc_kernel<D>, grid, dim3(kThreads), smem, s, tmQ, tmK, tmV, prm);
+  const cudaError_t e = launch_kernel(attn_quant_tc_kernel<D>, grid, dim3(kThreads), smem, s, tmQ, tmK, tmV, prm, seqs);
   if (e != cudaSuccess || prm.splits == 1) return (int)e;
   return (int)launch_kernel(attn_quant_join_kernel<D>, dim3((unsigned)(((long long)N * prm.Hq + 7) / 8)), dim3(256), 0, s,
-                            (const float*)prm.scratch, prm.out, prm.seq_tiles, prm.q_start, prm.base_len, N, B, prm.Hq, prm.Hkv, prm.splits);
+                            (const float*)prm.scratch, prm.out, prm.seq_tiles, prm.q_start, prm.base_len, seqs, listed, N, B, prm.Hq, prm.Hkv,
+                            prm.splits);
+}
+
+static bool seq_list(const int* ids, int n, int B, SeqList* out) {
+  if (n <= 0 || n > kMostSeqs) return false;
+  for (int i = 0; i < n; ++i) {
+    if (ids[i] < 0 || ids[i] >= B || ids[i] > 65535) return false;
+    out->b[i] = (unsigned short)ids[i];
+  }
+  for (int i = n; i < kMostSeqs; ++i) out->b[i] = 0;
+  return true;
 }
 
 }  // namespace siar
@@ -671,20 +696,24 @@ extern "C" int siar_attn_quant_tc_parts(int blocks, int longest, float average, 
 
 extern "C" int siar_attn_quant_tc_tile_info_bytes(void) { return (int)sizeof(TileInfo); }
 
-// The batch's keys and values as float16 tiles of 64 positions, sequence after sequence: k_out, v_out
-// [tiles_out, Hkv, 64, D], tiles [tiles_out, Hkv] (siar_attn_quant_tc_tile_info_bytes each), seq_tiles [B, 2].
+extern "C" int siar_attn_quant_tc_most_seqs(void) { return kMostSeqs; }
+
+// The keys and values of `listed` of the batch's B sequences (ids: their places in it, on the host) as float16 tiles of 64
+// positions, sequence after sequence: k_out, v_out [tiles_out, Hkv, 64, D], tiles [tiles_out, Hkv]
+// (siar_attn_quant_tc_tile_info_bytes each), seq_tiles [listed, 2].
 static int siar_widen_tiles_of(int bits, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                                 const int* block_table, const int* slot_ids, const int* q_start, const int* base_len, void* k_out,
-                                void* v_out, void* tiles, int* seq_tiles, int B, int Hkv, int D, int page_tokens, int max_pages,
-                                int n_pages, int tiles_out, int max_kv_len, int* status, void* stream) {
+                                void* v_out, void* tiles, int* seq_tiles, const int* ids, int listed, int B, int Hkv, int D,
+                                int page_tokens, int max_pages, int n_pages, int tiles_out, int max_kv_len, int* status, void* stream) {
   if (B == 0) return 0;
-  if ((bits != 8 && bits != 4) || (D != 64 && D != 128) || B > 65535 || Hkv > 65535 || page_tokens <= 0 || page_tokens % kKeys != 0 ||
+  SeqList seqs;
+  if (!seq_list(ids, listed, B, &seqs) || (bits != 8 && bits != 4) || (D != 64 && D != 128) || Hkv > 65535 || page_tokens <= 0 || page_tokens % kKeys != 0 ||
       max_kv_len <= 0 || n_pages <= 0 || (long long)max_pages * page_tokens >= (1ll << 31))
     return (int)cudaErrorInvalidValue;
   auto go = [&](auto kernel) {
-    return (int)launch_kernel(kernel, dim3((max_kv_len + kKeys - 1) / kKeys, Hkv, B), dim3(256), 0, (cudaStream_t)stream,
+    return (int)launch_kernel(kernel, dim3((max_kv_len + kKeys - 1) / kKeys, Hkv, listed), dim3(256), 0, (cudaStream_t)stream,
                               (const uint8_t*)k_pool, (const uint8_t*)v_pool, k_scale, v_scale, block_table, slot_ids, q_start, base_len,
-                              (__half*)k_out, (__half*)v_out, (TileInfo*)tiles, seq_tiles, B, Hkv, page_tokens, max_pages, n_pages,
+                              (__half*)k_out, (__half*)v_out, (TileInfo*)tiles, seq_tiles, seqs, Hkv, page_tokens, max_pages, n_pages,
                               tiles_out, status);
   };
   if (bits == 8) return D == 64 ? go(widen_tiles_kernel<64, 8>) : go(widen_tiles_kernel<128, 8>);
@@ -693,13 +722,15 @@ static int siar_widen_tiles_of(int bits, const void* k_pool, const void* v_pool,
 SIAR_TAKES_WORDS(siar_widen_tiles)
 
 // q [N, Hq, D] float16 with q_factor [N, Hq]; out [N, Hq * D] bfloat16; scratch: with splits > 1 N * Hq * splits * (D + 8)
-// floats.  splits: parts into which the keys of a block of rows are cut.
+// floats.  splits: parts into which the keys of a block of rows are cut.  ids, listed, and what follows from
+// them in seq_tiles, as siar_widen_tiles had them; max_q_len is that of the listed sequences, rows of others stay as they are.
 static int siar_attn_quant_tc_of(const void* q, const float* q_factor, const void* k_tiles, const void* v_tiles, const void* tiles,
-                                  const int* seq_tiles, const int* q_start, const int* base_len, void* out, float* scratch, int N, int B,
-                                  int Hq, int Hkv, int D, int tiles_out, int max_q_len, int splits, float scale, int* status,
+                                  const int* seq_tiles, const int* q_start, const int* base_len, void* out, float* scratch, const int* ids,
+                                  int listed, int N, int B, int Hq, int Hkv, int D, int tiles_out, int max_q_len, int splits, float scale, int* status,
                                   void* stream) {
   if (B == 0 || max_q_len == 0 || N == 0) return 0;
-  if (Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || Hq / Hkv > kRows || Hkv > 65535 || B > 65535 || splits < 1 || !(scale > 0.f) ||
+  SeqList seqs;
+  if (!seq_list(ids, listed, B, &seqs) || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || Hq / Hkv > kRows || splits < 1 || !(scale > 0.f) ||
       (long long)tiles_out * Hkv * kKeys >= (1ll << 31))
     return (int)cudaErrorInvalidValue;
   CUtensorMap tmQ, tmK, tmV;
@@ -709,10 +740,10 @@ static int siar_attn_quant_tc_of(const void* q, const float* q_factor, const voi
   const QuantTcParams prm = {(__nv_bfloat16*)out, scratch, (const TileInfo*)tiles, seq_tiles, q_factor, q_start, base_len, status, Hq,
                              Hkv, splits, scale * 1.4426950408889634f};
   const int G = Hq / Hkv, block_rows = (kRows / G) * G;
-  const long long across = (long long)splits * Hkv * B, down = (max_q_len * (long long)G + block_rows - 1) / block_rows;
+  const long long across = (long long)splits * Hkv * listed, down = (max_q_len * (long long)G + block_rows - 1) / block_rows;
   if (across >= (1ll << 31) || down > 65535) return (int)cudaErrorInvalidValue;
   const dim3 grid((unsigned)across, (unsigned)down);
-  return D == 64 ? launch_tc<64>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream)
-                 : launch_tc<128>(tmQ, tmK, tmV, prm, grid, N, B, (cudaStream_t)stream);
+  return D == 64 ? launch_tc<64>(tmQ, tmK, tmV, prm, grid, seqs, listed, N, B, (cudaStream_t)stream)
+                 : launch_tc<128>(tmQ, tmK, tmV, prm, grid, seqs, listed, N, B, (cudaStream_t)stream);
 }
 SIAR_TAKES_WORDS(siar_attn_quant_tc)

@@ -8,6 +8,7 @@ what a call needs besides its result is one allocation.
 
 from __future__ import annotations
 
+import array
 import copy
 from typing import Optional, Tuple
 
@@ -135,12 +136,12 @@ def rope_kv_write(qkv: torch.Tensor, rotary, kv, meta, n_heads: int, n_kv_heads:
                     ops.status_word(qkv.device).data_ptr(), ops._stream(), rotary_dim, int(interleaved))
 
 
-def _pages(kv, meta, page: int) -> Tuple[int, int]:
-    """(pages of ``page`` positions that the batch's sequences hold together, the most of one)."""
+def _pages(kv, meta, page: int) -> int:
+    """Pages of ``page`` positions that the batch's sequences hold together."""
     most = -(-min(meta.max_kv_len, kv.block_table.shape[1] * kv.page_tokens) // page)
     if meta.base_lens is None or meta.q_lens is None:        # lengths live on the device only: room for the longest everywhere
-        return meta.n_seqs * most, most
-    return sum([min(-(-(n + m) // page), most) for n, m in zip(meta.base_lens, meta.q_lens)]), most
+        return meta.n_seqs * most
+    return sum([min(-(-(n + m) // page), most) for n, m in zip(meta.base_lens, meta.q_lens)])
 
 
 def _read(kv, meta, dtype: torch.dtype, window: Optional[int], pools, batch, with_slots: bool = False):
@@ -149,7 +150,7 @@ def _read(kv, meta, dtype: torch.dtype, window: Optional[int], pools, batch, wit
     n_kv_heads, head_dim, page = kv.k.shape[1], kv.head_dim, int(kv.page_tokens)
     if meta.max_kv_len <= 0:
         raise ValueError(f"max_kv_len must be positive, got {meta.max_kv_len}")
-    pages, _ = _pages(kv, meta, page)
+    pages = _pages(kv, meta, page)
     k, v = torch.empty((2, pages, n_kv_heads, page, head_dim), dtype=dtype, device=device).unbind(0)
     table = torch.empty((meta.n_seqs, kv.block_table.shape[1]), dtype=torch.int32, device=device)
     slots = torch.empty(meta.n_seqs, dtype=torch.int32, device=device) if with_slots else None
@@ -187,10 +188,34 @@ def works_on_codes(kv, meta, dtype: torch.dtype, n_heads: int, n_kv_heads: int, 
     a multiple of 64, no window): single tokens, short runs, and whatever ``works_on_tiles`` does not take."""
     if dtype != torch.bfloat16 or window is not None or head_dim not in (64, 128) or not options.use_mma_attention:
         return False
-    if kv.page_tokens % 64 or kv.k.shape[0] * n_kv_heads * kv.page_tokens >= 1 << 31:
+    if not _codes_can_be_addressed(kv, n_kv_heads):
         return False
     return meta.is_decode or meta.max_q_len * (n_heads // n_kv_heads) <= MOST_ROWS or not works_on_tiles(
         kv, dtype, n_heads, n_kv_heads, head_dim, scale, window, options)
+
+
+def _codes_can_be_addressed(kv, n_kv_heads: int) -> bool:
+    return kv.page_tokens % 64 == 0 and kv.k.shape[0] * n_kv_heads * kv.page_tokens < 1 << 31
+
+
+def new_on_codes(kv, meta, n_heads: int, n_kv_heads: int) -> int:
+    """In a batch that brings long runs: sequences of up to so many new tokens (0: none) are attended to on the codes all the
+    same, each by its own length.  On tiles they would have their whole cache widened, several times the bytes of the codes,
+    and take a block of 128 rows for a few.  A launch of its own costs 7 us (runs of several tokens: up to 20, at 16 rows a kv
+    head), so it takes keys enough: a long sequence, whose tiles follow one another, or many, each of which costs the tiles about
+    256 keys more.  Measured on B200 beside a chunk of 512, all on tiles against two launches (8 bits, 32 heads on 8, 128
+    dims; us): one token on 100 keys 25 and 30, on 1,000 34 and 32, on 16,000 100 and 40; eight of them on 100 29 and 30, on 500
+    37 and 35, on 4,000 110 and 45; 32 on 100 51 and 33; four new tokens on 2,000 46 and 43, eight times four on 500 37 and 43,
+    on 1,000 46 and 46, 32 times four on 100 51 and 41.  64 dims and 4 bits cross at about the same lengths.  Where the batch's lengths are on the device only, nothing is known of them."""
+    if meta.q_lens is None or meta.base_lens is None or not _codes_can_be_addressed(kv, n_kv_heads):
+        return 0
+    most = max(1, MOST_ROWS * n_kv_heads // n_heads)
+    short = [(m, c + m) for c, m in zip(meta.base_lens, meta.q_lens) if 0 < m <= most]
+    if not short:
+        return 0
+    worth = 1024 if max(short)[0] == 1 else 2048
+    keys = [n for _, n in short]
+    return most if max(keys) >= worth or sum(keys) + 256 * len(keys) >= 4 * worth else 0
 
 
 _workspaces, _captured_workspaces = {}, {}
@@ -235,6 +260,16 @@ def _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_
                 kv.k.shape[0], int(write_kv), ops.status_word(qkv.device).data_ptr(), ops._stream())
 
 
+def _launch_codes(out, qkv, q16: int, factor: int, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, fused,
+                  write_kv, most_new: int, max_q_len: int, max_kv_len: int) -> None:
+    index, stream = qkv.get_device(), ops._stream()
+    counters, scratch = _workspace(index, stream)
+    ops._launch_words("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), q16, factor, *pools, *batch,
+                _at(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads, head_dim,
+                kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], max_q_len, max_kv_len, ops._sm_count(index), int(fused),
+                int(bool(write_kv)), most_new, float(scale), ops.status_word(qkv.device).data_ptr(), stream)
+
+
 def _on_codes(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, fused, write_kv) -> torch.Tensor:
     """``fused``: one token a sequence, rotated (``inv_freq``) and stored (``write_kv``) by the attention kernel itself;
     else, where ``write_kv`` is not None, by a kernel in front."""
@@ -245,13 +280,8 @@ def _on_codes(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_d
             held, q16, factor = _carve(device, n * n_heads * head_dim * 2, n * n_heads * 4)
             _queries16(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, write_kv, q16, factor)
         out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=device)
-        stream = ops._stream()
-        counters, scratch = _workspace(index, stream)
-        ops._launch_words("attention_quant", "siar_attn_quant", kv.bits, qkv.data_ptr(), q16, factor, *pools, *batch,
-                    _at(inv_freq), out.data_ptr(), counters, scratch, meta.n_seqs, n_heads, n_kv_heads, head_dim,
-                    kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], meta.max_q_len, meta.max_kv_len,
-                    ops._sm_count(index), int(fused), int(bool(write_kv)), float(scale), ops.status_word(device).data_ptr(),
-                    stream)
+        _launch_codes(out, qkv, q16, factor, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, fused, write_kv,
+                      0x7fffffff, meta.max_q_len, meta.max_kv_len)
     return out
 
 
@@ -268,31 +298,59 @@ def key_parts(blocks: int, longest: int, average: float, row_floats: int, sms: i
     return ops._fn("attention_quant_tc", "siar_attn_quant_tc_parts")(blocks, longest, average, row_floats, sms)
 
 
+def tiles_of(kv, meta, passed_new: int):
+    """(new tokens, key tiles of 64) of every sequence that is attended to on tiles, (0, 0) of the others: those of no more than
+    ``passed_new`` new tokens."""
+    most = -(-min(meta.max_kv_len, kv.block_table.shape[1] * kv.page_tokens) // 64)
+    if meta.base_lens is None or meta.q_lens is None:        # lengths live on the device only: room for the longest everywhere
+        return [(meta.max_q_len, most)] * meta.n_seqs
+    return [(m, min(-(-(n + m) // 64), most)) if m > passed_new else (0, 0) for n, m in zip(meta.base_lens, meta.q_lens)]
+
+
+def runs_of_tiles(lengths, most_seqs: int):
+    """The places of the sequences that have tiles, in launches of at most ``most_seqs``."""
+    places = [i for i, (_, t) in enumerate(lengths) if t > 0]
+    return [places[i:i + most_seqs] for i in range(0, len(places), most_seqs)]
+
+
 def _on_tiles(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, write_kv) -> torch.Tensor:
-    """Rotates (``inv_freq``) and stores (``write_kv``) the new tokens, widens the batch's cache to float16 tiles and
-    attends on those."""
+    """Rotates (``inv_freq``) and stores (``write_kv``) the new tokens, widens the cache of the sequences that bring long runs to
+    float16 tiles and attends on those; the others (``new_on_codes``) work on the codes."""
     device, index, n, heads = qkv.device, qkv.get_device(), qkv.shape[0], (n_heads, n_kv_heads, head_dim)
-    tiles, most = _pages(kv, meta, 64)
-    q_lens = meta.q_lens if meta.q_lens is not None else [meta.max_q_len] * meta.n_seqs
     group = n_heads // n_kv_heads
     block_rows = 128 // group * group
-    blocks = n_kv_heads * sum([-(-m * group // block_rows) for m in q_lens])
-    splits = key_parts(blocks, most, most - meta.max_q_len / 128, n * n_heads * (head_dim + 8), ops._sm_count(index))
+    passed = new_on_codes(kv, meta, n_heads, n_kv_heads)
+    lengths = tiles_of(kv, meta, passed)
+    fn = ops._fn("attention_quant_tc", "siar_attn_quant_tc_most_seqs")
+    launches, info_bytes = [], ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")()
+    for ids in runs_of_tiles(lengths, fn()):
+        tiles, blocks = [lengths[i][1] for i in ids], [-(-lengths[i][0] * group // block_rows) for i in ids]
+        average = sum([w * (t - lengths[i][0] / 128) for i, w, t in zip(ids, blocks, tiles)]) / sum(blocks)     # key tiles a block
+        splits = key_parts(n_kv_heads * sum(blocks), max(tiles), average, n * n_heads * (head_dim + 8), ops._sm_count(index))
+        launches.append((array.array("i", ids), sum(tiles), max(tiles), max([lengths[i][0] for i in ids]), splits))
+    if not launches:
+        raise ValueError("q_lens, max_q_len and max_kv_len of the batch do not agree")
+    tiles, splits = max([t for _, t, _, _, _ in launches]), max([s for *_, s in launches])
     row_bytes, tile_bytes = n * n_heads * 4, tiles * n_kv_heads * 64 * head_dim * 2
     with ops._on_device(index):
         stream, status = ops._stream(), ops.status_word(device).data_ptr()
         out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=device)
         held, q16, factor, k16, v16, info, seq, scratch = _carve(
-            device, row_bytes // 2 * head_dim, row_bytes, tile_bytes, tile_bytes,
-            tiles * n_kv_heads * ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")(), meta.n_seqs * 8,
-            row_bytes * splits * (head_dim + 8) if splits > 1 else 0)
+            device, row_bytes // 2 * head_dim, row_bytes, tile_bytes, tile_bytes, tiles * n_kv_heads * info_bytes,
+            max([len(ids) for ids, *_ in launches]) * 8, row_bytes * splits * (head_dim + 8) if splits > 1 else 0)
         _queries16(qkv, inv_freq, kv, meta, pools, batch, *heads, write_kv, q16, factor)
-        ops._launch_words("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, *batch, k16, v16, info, seq, meta.n_seqs,
-                    n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], tiles, meta.max_kv_len,
-                    status, stream)
-        ops._launch_words("attention_quant_tc", "siar_attn_quant_tc", q16, factor, k16, v16, info, seq, batch[1], batch[2],
-                    out.data_ptr(), scratch, n, meta.n_seqs, *heads, tiles, meta.max_q_len, splits, float(scale), status, stream,
-                    kernels=2 if splits > 1 else 1)
+        if passed:
+            short = [(m, c + m) for c, m in zip(meta.base_lens, meta.q_lens) if 0 < m <= passed]
+            _launch_codes(out, qkv, q16, factor, None, kv, meta, pools, batch, *heads, scale, False, False, passed,
+                          max([m for m, _ in short]), max([c for _, c in short]))
+        for ids, tiles, most, most_new, splits in launches:
+            which = (ids.buffer_info()[0], len(ids))
+            ops._launch_words("attention_quant_tc", "siar_widen_tiles", kv.bits, *pools, *batch, k16, v16, info, seq, *which,
+                        meta.n_seqs, n_kv_heads, head_dim, kv.page_tokens, kv.block_table.shape[1], kv.k.shape[0], tiles, most * 64,
+                        status, stream)
+            ops._launch_words("attention_quant_tc", "siar_attn_quant_tc", q16, factor, k16, v16, info, seq, batch[1], batch[2],
+                        out.data_ptr(), scratch, *which, n, meta.n_seqs, *heads, tiles, most_new, splits, float(scale), status,
+                        stream, kernels=2 if splits > 1 else 1)
     return out
 
 

@@ -92,25 +92,23 @@ _signatures = {
     },
     "attention_quant": {
         # (taken as words) bits, qkv, q16, q_factor, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, inv_freq, out, counters, scratch,
-        # B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, max_kv_len, sm_count, fused, write_kv, scale, status,
-        # stream
+        # B, Hq, Hkv, D, page_tokens, max_pages, n_pages, max_q_len, max_kv_len, sm_count, fused, write_kv, most_new, scale,
+        # status, stream
         "siar_attn_quant": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
-                            c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+                            c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
         "siar_attn_quant_counters": [c_int],
         "siar_attn_quant_scratch_floats": [c_int],
         "siar_capture_id": [c_void_p],
     },
     "attention_quant_tc": {
-        # bits, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, k_out, v_out, tiles, seq_tiles, B, Hkv, D,
-        # page_tokens, max_pages, n_pages, tiles_out, max_kv_len, status, stream
-        "siar_widen_tiles": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                             c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
-                             c_void_p],
-        # q, q_factor, k_tiles, v_tiles, tiles, seq_tiles, q_start, base_len, out, scratch, N, B, Hq, Hkv, D, tiles_out,
-        # max_q_len, splits, scale, status, stream
-        "siar_attn_quant_tc": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                               c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+        # (these two taken as words) bits, k, v, k_scale, v_scale, block_table, slot_ids, q_start, base_len, k_out, v_out, tiles,
+        # seq_tiles, ids, listed, B, Hkv, D, page_tokens, max_pages, n_pages, tiles_out, max_kv_len, status, stream
+        "siar_widen_tiles": [c_int] + [c_void_p] * 13 + [c_int] * 9 + [c_void_p] * 2,
+        # q, q_factor, k_tiles, v_tiles, tiles, seq_tiles, q_start, base_len, out, scratch, ids, listed, N, B, Hq, Hkv, D,
+        # tiles_out, max_q_len, splits, scale, status, stream
+        "siar_attn_quant_tc": [c_void_p] * 11 + [c_int] * 9 + [c_float] + [c_void_p] * 2,
+        "siar_attn_quant_tc_most_seqs": [],
         "siar_attn_quant_tc_tile_info_bytes": [],
         "siar_attn_quant_tc_parts": [c_int, c_int, c_float, c_longlong, c_int],
     },

@@ -168,3 +168,27 @@ def test_queries_that_would_go_over_other_rows():
     room = torch.zeros(3, 512, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="apart"):
         ops.rope_kv_write(room[:2], None, b.kv, b.meta(), 4, 2, 64, q_out=room[1:])
+
+
+def test_which_sequences_of_a_batch_go_on_the_codes():
+    """Short runs beside a long one: by their own length where their keys are many, or the lengths are known at all."""
+    def new_on_codes(held, new, heads=8, **kw):
+        b = eq.Batch(8, heads, 2, 64, [0] * len(held), [1] * len(held))
+        meta = b.meta()
+        meta.base_lens, meta.q_lens, meta.max_q_len = held, new, max(new)
+        meta.max_kv_len = max(c + n for c, n in zip(held, new))
+        for name, value in kw.items():
+            setattr(meta, name, value)
+        b.kv.block_table = torch.zeros(len(held) + 2, 200, dtype=torch.int32)
+        passed = kv_quant.new_on_codes(b.kv, meta, heads, 2)
+        return passed, kv_quant.tiles_of(b.kv, meta, passed)
+
+    assert new_on_codes([0, 2000], [512, 1]) == (16, [(512, 8), (0, 0)])
+    assert new_on_codes([0, 100], [512, 1]) == (0, [(512, 8), (1, 2)])
+    assert new_on_codes([0] + [600] * 8, [512] + [1] * 8) == (16, [(512, 8)] + [(0, 0)] * 8)
+    assert new_on_codes([0] + [100] * 8, [512] + [1] * 8) == (0, [(512, 8)] + [(1, 2)] * 8)
+    assert new_on_codes([0] + [100] * 16, [512] + [1] * 16) == (16, [(512, 8)] + [(0, 0)] * 16)
+    assert new_on_codes([0, 1500, 0], [512, 4, 0]) == (0, [(512, 8), (4, 24), (0, 0)])
+    assert new_on_codes([0, 2100, 700], [512, 16, 17]) == (16, [(512, 8), (0, 0), (17, 12)])
+    assert new_on_codes([0, 2000], [512, 1], heads=256) == (1, [(512, 8), (0, 0)])
+    assert new_on_codes([0, 2000], [512, 1], base_lens=None) == (0, [(512, 32), (512, 32)])

@@ -739,3 +739,56 @@ def test_queries_with_one_large_channel(bits, new, dim, channel, ratio):
                 square.append((out[int(b.q_start[i]) + t, h] - o).square())
     rms, most = (float(torch.cat(s).mean().sqrt()) for s in (square, expected))
     assert rms <= 1.5 * most, (rms, most)
+
+
+MIXED = {
+    "a chunk and tokens": ([0, 700, 64, 1, 130], [90, 1, 1, 1, 1]),
+    "a chunk and long tokens": ([63, 1200, 0, 300], [90, 1, 1, 1]),
+    "two long runs": ([500, 10, 0, 64, 2100, 2100], [40, 16, 130, 0, 3, 1]),
+}
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (32, 8, 128), (16, 1, 128), (80, 1, 64)])
+@pytest.mark.parametrize("batch", list(MIXED))
+def test_long_and_short_runs_in_one_batch(bits, heads, kv_heads, dim, batch):
+    """Every sequence is attended to by its own length: what a batch of its own kind gives, NaN behind every sequence."""
+    held, new = MIXED[batch]
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=heads + dim)
+    inv, scale = freqs(dim), dim ** -0.5
+    kv = b.entry(DEV)
+    out = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV), *b.sizes(), scale)
+    ops.check_status(DEV)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), inv, want, b.meta(), *b.sizes())
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    pos = [c + i for c, n in zip(held, new) for i in range(n)]
+    check_attention(b, out, eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv), want, scale)
+    check_attention(b, ops.attention(b.qkv.to(DEV), kv, b.meta(DEV), *b.sizes(), scale),
+                    b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), want, scale)
+    again = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV, host_lengths=False), *b.sizes(), scale)
+    ops.check_status(DEV)
+    check_attention(b, again, eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv), want, scale)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_single_tokens_beside_a_chunk_are_not_widened(bits):
+    """24 sequences of 3,000 keys bring one token, one of 100 keys brings 40: besides the result a call takes the float16
+    queries and their factors, the tiles of the one sequence (3 of 64 positions, keys and values, 32 bytes beside each), 8 bytes
+    a sequence and at most 16 parts of every row;
+    256-byte steps of nine pieces and the allocator's 2 MB."""
+    heads, kv_heads, dim = 8, 2, 128
+    held, new = [100] + [3000] * 24, [40] + [1] * 24
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=1, stale="random")
+    kv, qkv, meta = b.entry(DEV), b.qkv.to(DEV), b.meta(DEV)
+    ops.rope_and_attention(qkv, None, kv, meta, *b.sizes(), 0.09)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.rope_and_attention(qkv, None, kv, meta, *b.sizes(), 0.09)
+    taken = torch.cuda.max_memory_allocated() - before
+    rows = b.tokens * heads
+    allowed = 2 * rows * dim * 2 + rows * 4 + 2 * 3 * kv_heads * 64 * dim * 2 + 3 * kv_heads * 32 + 25 * 8 + 16 * rows * (dim + 8) * 4
+    assert taken <= allowed + 9 * 256 + (2 << 20), (taken, allowed)
