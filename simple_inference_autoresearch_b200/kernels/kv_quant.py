@@ -307,10 +307,25 @@ def tiles_of(kv, meta, passed_new: int):
     return [(m, min(-(-(n + m) // 64), most)) if m > passed_new else (0, 0) for n, m in zip(meta.base_lens, meta.q_lens)]
 
 
-def runs_of_tiles(lengths, most_seqs: int):
-    """The places of the sequences that have tiles, in launches of at most ``most_seqs``."""
-    places = [i for i, (_, t) in enumerate(lengths) if t > 0]
-    return [places[i:i + most_seqs] for i in range(0, len(places), most_seqs)]
+#: bytes of float16 tiles that one launch may take, where it has more than one sequence: a batch's tiles are several times its
+#: codes, and only those of a launch are held at a time.  One sequence of 131,072 keys of 8 heads of 128 dims takes half of it.
+MOST_TILE_BYTES = 1 << 30
+
+
+def runs_of_tiles(lengths, most_seqs: int, tile_bytes: int):
+    """The places of the sequences that have tiles (of ``tile_bytes`` each, keys and values), launch by launch: at most
+    ``most_seqs`` of them and MOST_TILE_BYTES, but one at least; about as much in each launch."""
+    bytes_of = [(i, t * tile_bytes) for i, (_, t) in enumerate(lengths) if t > 0]
+    total = sum([n for _, n in bytes_of])
+    share = total / max(1, -(-total // MOST_TILE_BYTES), -(-len(bytes_of) // most_seqs))
+    runs, held = [], 0
+    for i, n in bytes_of:
+        if not runs or len(runs[-1]) == most_seqs or held >= share or held + n > MOST_TILE_BYTES:
+            runs.append([])
+            held = 0
+        runs[-1].append(i)
+        held += n
+    return runs
 
 
 def _on_tiles(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_dim, scale, write_kv) -> torch.Tensor:
@@ -323,7 +338,7 @@ def _on_tiles(qkv, inv_freq, kv, meta, pools, batch, n_heads, n_kv_heads, head_d
     lengths = tiles_of(kv, meta, passed)
     fn = ops._fn("attention_quant_tc", "siar_attn_quant_tc_most_seqs")
     launches, info_bytes = [], ops._fn("attention_quant_tc", "siar_attn_quant_tc_tile_info_bytes")()
-    for ids in runs_of_tiles(lengths, fn()):
+    for ids in runs_of_tiles(lengths, fn(), 2 * n_kv_heads * 64 * head_dim * 2):
         tiles, blocks = [lengths[i][1] for i in ids], [-(-lengths[i][0] * group // block_rows) for i in ids]
         average = sum([w * (t - lengths[i][0] / 128) for i, w, t in zip(ids, blocks, tiles)]) / sum(blocks)     # key tiles a block
         splits = key_parts(n_kv_heads * sum(blocks), max(tiles), average, n * n_heads * (head_dim + 8), ops._sm_count(index))

@@ -192,3 +192,21 @@ def test_which_sequences_of_a_batch_go_on_the_codes():
     assert new_on_codes([0, 2100, 700], [512, 16, 17]) == (16, [(512, 8), (0, 0), (17, 12)])
     assert new_on_codes([0, 2000], [512, 1], heads=256) == (1, [(512, 8), (0, 0)])
     assert new_on_codes([0, 2000], [512, 1], base_lens=None) == (0, [(512, 32), (512, 32)])
+
+
+def test_tiles_of_a_launch_are_bounded():
+    """Sequences in launches of up to 64 and MOST_TILE_BYTES, one at least, in order, none without tiles, about even."""
+    runs, most = kv_quant.runs_of_tiles, kv_quant.MOST_TILE_BYTES
+    assert runs([(70, 3)] * 5, 64, 1000) == [[0, 1, 2, 3, 4]]
+    assert runs([(70, 3), (0, 0), (90, 3)] * 50, 64, 8) == [[i for i in range(75) if i % 3 != 1], [i for i in range(75, 150) if i % 3 != 1]]
+    assert runs([(70, 10)] * 7, 64, most // 30) == [[0, 1, 2], [3, 4, 5], [6]]
+    assert runs([(70, 10)] * 8, 64, most // 70) == [[0, 1, 2, 3], [4, 5, 6, 7]]
+    assert runs([(70, 1), (70, 40), (70, 1), (70, 28), (0, 0), (70, 1)], 64, most // 30) == [[0], [1], [2, 3], [5]]
+    assert runs([(0, 0)], 64, 1) == []
+    g = torch.Generator().manual_seed(0)
+    for _ in range(200):
+        n = int(torch.randint(1, 150, (1,), generator=g))
+        lengths = [(1, t) for t in torch.randint(0, 60, (n,), generator=g).tolist()]
+        got = runs(lengths, 64, most // 100)
+        assert [i for r in got for i in r] == [i for i in range(n) if lengths[i][1]]
+        assert all(len(r) <= 64 and (len(r) == 1 or sum(lengths[i][1] for i in r) <= 100) for r in got)

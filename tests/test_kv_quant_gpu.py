@@ -792,3 +792,30 @@ def test_single_tokens_beside_a_chunk_are_not_widened(bits):
     rows = b.tokens * heads
     allowed = 2 * rows * dim * 2 + rows * 4 + 2 * 3 * kv_heads * 64 * dim * 2 + 3 * kv_heads * 32 + 25 * 8 + 16 * rows * (dim + 8) * 4
     assert taken <= allowed + 9 * 256 + (2 << 20), (taken, allowed)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("host_lengths", [True, False])
+def test_chunks_whose_tiles_are_bounded(bits, host_lengths, monkeypatch):
+    """The tiles of at most two sequences at a time: the same results, with the workspace of two."""
+    from simple_inference_autoresearch_b200.kernels import kv_quant
+    heads, kv_heads, dim = 8, 2, 128
+    b = eq.Batch(bits, heads, kv_heads, dim, [1300, 700, 0, 1500, 1200], [70, 40, 90, 40, 70], seed=4)
+    kv, qkv, meta = b.entry(DEV), b.qkv.to(DEV), b.meta(DEV, host_lengths=host_lengths)
+    whole = attend(b, kv, scale=0.09, meta=meta)
+    per_tile = 2 * kv_heads * 64 * dim * 2
+    tiles = 25                                                # of the longest sequence
+    monkeypatch.setattr(kv_quant, "MOST_TILE_BYTES", 2 * tiles * per_tile)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = ops.rope_and_attention(qkv, None, kv, meta, *b.sizes(), 0.09)
+    taken = torch.cuda.max_memory_allocated() - before
+    ops.check_status(DEV)
+    rows = b.tokens * heads
+    allowed = 2 * rows * dim * 2 + rows * 4 + 2 * tiles * (per_tile + kv_heads * 32) + 5 * 8 + 16 * rows * (dim + 8) * 4
+    assert taken <= allowed + 9 * 256 + (2 << 20), (taken, allowed)
+    want, q = plain_of(b)
+    check_attention(b, out, q, want, 0.09)
+    check_attention(b, whole, q, want, 0.09)
