@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from ..cache.sequence_cache import DEFAULT_PAGE_TOKENS, SequenceCache, round_up
-from ..kernels import ops
+from ..kernels import build, kv_quant, ops
 from ..kernels.options import DEFAULT, KernelOptions
 from ..sampling.params import SamplingParams, request_seed
 from . import generation
@@ -60,12 +60,20 @@ class Engine:
             max_tokens = self.max_batch * round_up(max_seq_len, page_tokens)
         self.cache = SequenceCache(model.cache_needs, int(max_tokens), int(max_slots or self.max_batch),
                                    max_seq_len, model.dtype, self.device, page_tokens, kv_cache)
+        if self._cuda:            # compiled here, not inside the first step
+            build.ensure_built(self.extension_units())
         self.max_seq_len = self.cache.max_seq_len
         self.use_cuda_graph = bool(use_cuda_graph)
         self._graphs: Dict[Tuple[int, int], "_DecodeGraph"] = {}      # in order of last use
         self._graph_state: Optional[_GraphBuffers] = None
         self._graph_pool = None      # one memory pool for all captured steps: they never run at the same time
         self._last_logits: Optional[torch.Tensor] = None
+
+    def extension_units(self) -> List[str]:
+        """The CUDA units that this engine's cache adds to those of its model (``DecoderModel.extension_units``)."""
+        if self.cache.kv_format is None:
+            return []
+        return list(kv_quant.extension_units(self.model.cache_needs, self.model.dtype, self.cache.page_tokens))
 
     # ------------------------------------------------------------------ slots
     def open(self) -> int:

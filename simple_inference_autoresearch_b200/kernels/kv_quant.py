@@ -22,6 +22,16 @@ def is_quantized(kv) -> bool:
     return getattr(kv, "k_scale", None) is not None
 
 
+def extension_units(needs, dtype: torch.dtype, page_tokens: int) -> Tuple[str, ...]:
+    """The CUDA units that steps over a quantised cache of these needs (``parts.base.KVNeed``; others are passed over) launch
+    from, besides those of the same model over a cache in the compute type."""
+    needs = [n for n in needs if getattr(n, "n_kv_heads", None)]
+    units = ("kv_quant",) if needs else ()
+    if dtype == torch.bfloat16 and page_tokens % 64 == 0 and any(n.head_dim in (64, 128) and n.window is None for n in needs):
+        units += ("attention_quant", "attention_quant_tc")
+    return units
+
+
 # ------------------------------------------------------------------ arguments
 def check_entry(kv, n_kv_heads: int, head_dim: int, index: int) -> Tuple[int, ...]:
     """Raises ``ValueError`` unless the entry's tensors are what the kernels index: shapes, types, contiguity, all

@@ -210,3 +210,15 @@ def test_tiles_of_a_launch_are_bounded():
         got = runs(lengths, 64, most // 100)
         assert [i for r in got for i in r] == [i for i in range(n) if lengths[i][1]]
         assert all(len(r) <= 64 and (len(r) == 1 or sum(lengths[i][1] for i in r) <= 100) for r in got)
+
+
+@pytest.mark.parametrize("config,dtype,units", [("A", torch.float32, ["kv_quant"]), ("A", torch.bfloat16, ["kv_quant"]),
+                                                ("D", torch.bfloat16, ["kv_quant", "attention_quant", "attention_quant_tc"])])
+def test_an_engine_names_the_units_of_its_cache(tmp_path, config, dtype, units):
+    loaded = siar.load_model(tiny_configs.make_folder(tmp_path, config, seed=3), device="cpu", dtype=dtype)
+    engine = lambda fmt: siar.build_engine(loaded, max_seq_len=64, kv_cache=fmt)  # noqa: E731
+    assert engine(None).extension_units() == []
+    assert engine("int8").extension_units() == engine("int4").extension_units() == units
+    assert kv_quant.extension_units([None, StateNeed((3,))], torch.bfloat16, 64) == ()
+    assert kv_quant.extension_units([KVNeed(2, 128, window=9)], torch.bfloat16, 64) == ("kv_quant",)
+    assert kv_quant.extension_units([KVNeed(2, 128)], torch.bfloat16, 16) == ("kv_quant",)

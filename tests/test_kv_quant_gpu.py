@@ -819,3 +819,23 @@ def test_chunks_whose_tiles_are_bounded(bits, host_lengths, monkeypatch):
     want, q = plain_of(b)
     check_attention(b, out, q, want, 0.09)
     check_attention(b, whole, q, want, 0.09)
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+@pytest.mark.parametrize("config,dtype", [("A", torch.float32), ("A", torch.bfloat16), ("D", torch.bfloat16)])
+def test_every_unit_of_a_step_is_built_with_the_engine(tmp_path, monkeypatch, kv_format, config, dtype):
+    """Whatever a prompt and decode steps load has been asked for by the time the engine stands: nothing is compiled, and no
+    missing compiler found, inside a step."""
+    import simple_inference_autoresearch_b200 as siar
+    from simple_inference_autoresearch_b200.kernels import build
+    from tests import tiny_configs
+    folder = tiny_configs.make_folder(tmp_path, config, seed=6)
+    built, loaded_units = [], []
+    real_build, real_load = build.ensure_built, build.load_unit
+    monkeypatch.setattr(build, "ensure_built", lambda units: built.extend(units) or real_build(units))
+    engine = siar.build_engine(siar.load_model(folder, device=DEV, dtype=dtype), max_batch=2, max_seq_len=128, kv_cache=kv_format)
+    asked = set(built)
+    monkeypatch.setattr(build, "load_unit", lambda unit: loaded_units.append(unit) or real_load(unit))
+    monkeypatch.setattr(ops, "_bound", {})
+    engine.generate([list(range(1, 90)), [3, 4]], siar.SamplingParams(temperature=0.0), max_new_tokens=4, ignore_eos=True)
+    assert "kv_quant" in loaded_units and set(loaded_units) <= asked, set(loaded_units) - asked
