@@ -137,14 +137,23 @@ attn_prefill_kernel(const T* __restrict__ qkv, const T* __restrict__ k_pool, con
 #pragma unroll
       for (int n = 0; n < NDIM; ++n) acc[i][n] *= alpha;
       // only the keys that the row sees: 0 x a value that is no number would reach it from the others
-      const int j_end = min(kTile, kv_end[i] - j0);
-      for (int j = max(0, kv_begin[i] - j0); j < j_end; ++j) {
+      const int j_begin = max(0, kv_begin[i] - j0), j_end = min(kTile, kv_end[i] - j0);
+      auto add_key = [&](int j) {
         const float pj = __shfl_sync(0xffffffffu, p, j);
 #pragma unroll
         for (int n = 0; n < NDIM; ++n) {
           const int d = lane + 32 * n;
           if (d < D) acc[i][n] = fmaf(pj, v_s[j * D + d], acc[i][n]);
         }
+      };
+      // Up to 64 dims a tile that is seen whole takes a loop of constant length: unrolled it has its loads under way
+      // together, where a key is only a few instructions (1,000 tokens, 6 heads on 2, float32: 16 dims 129 us against
+      // 247, 32 dims 177 against 271, 64 dims 290 against 312).  With more dims the short loop is the faster or as fast (128
+      // dims, 2,048 tokens, 32 heads on 8: 5.5 ms against 7.2; 80 to 256 dims within 2 %).
+      if (NDIM <= 2 && j_begin == 0 && j_end == kTile) {
+        for (int j = 0; j < kTile; ++j) add_key(j);
+      } else {
+        for (int j = j_begin; j < j_end; ++j) add_key(j);
       }
     }
   }
