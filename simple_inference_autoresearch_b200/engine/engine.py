@@ -320,6 +320,7 @@ class _DecodeGraph:
         try:
             with torch.cuda.graph(self.graph, pool=engine._graph_pool):
                 self._body(advance=True)
+                kv_quant.end_of_capture()
         finally:
             if collector_on:
                 gc.enable()

@@ -235,9 +235,12 @@ def _workspace(index: int, stream: int):
     """Pointers to the counters (zeros, which a launch uses and leaves zero) and the scratch of launches on
     one stream of GPU ``index``.  Launches of one stream follow one another and share them; a captured graph may be
     replayed beside anything, so every capture has its own, zeroed by the graph itself, for the launches that
-    it holds on one stream."""
+    it holds on one stream.  It is the graph's memory, held here only as long as the capture may ask for it again: up to
+    ``end_of_capture``, or the next capture or launch on the stream."""
     key = (index, stream)
     if not torch._C._cuda_isCurrentStreamCapturing():
+        if _captured_workspaces:
+            _captured_workspaces.pop(key, None)
         held = _workspaces.get(key)
         if held is None:
             held = _workspaces.setdefault(key, _new_workspace(index))      # (one of two threads' is kept)
@@ -249,6 +252,12 @@ def _workspace(index: int, stream: int):
     if held is None or held[-1] != capture:
         held = _captured_workspaces[key] = _new_workspace(index) + (capture,)
     return held[:2]
+
+
+def end_of_capture() -> None:
+    """As the last thing in a capture: its workspace on the current stream is not asked for again."""
+    index = torch._C._cuda_getDevice()
+    _captured_workspaces.pop((index, torch._C._cuda_getCurrentRawStream(index)), None)
 
 
 def _new_workspace(index: int):

@@ -839,3 +839,59 @@ def test_every_unit_of_a_step_is_built_with_the_engine(tmp_path, monkeypatch, kv
     monkeypatch.setattr(ops, "_bound", {})
     engine.generate([list(range(1, 90)), [3, 4]], siar.SamplingParams(temperature=0.0), max_new_tokens=4, ignore_eos=True)
     assert "kv_quant" in loaded_units and set(loaded_units) <= asked, set(loaded_units) - asked
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+def test_a_dropped_engine_leaves_no_workspace_of_its_captures(tmp_path, kv_format):
+    """The memory of captured steps' workspaces is the graphs': with the engine it goes back to the device."""
+    import gc
+
+    import simple_inference_autoresearch_b200 as siar
+    from simple_inference_autoresearch_b200.kernels import kv_quant
+    from tests import tiny_configs
+    loaded = siar.load_model(tiny_configs.make_folder(tmp_path, "D", seed=6), device=DEV, dtype=torch.bfloat16)
+    kv_quant._captured_workspaces.clear()                     # what captures of other tests left
+
+    def held(graph):
+        engine = siar.build_engine(loaded, max_batch=2, max_seq_len=96, use_cuda_graph=graph, kv_cache=kv_format)
+        out = engine.generate([[5, 6, 7], [8]], siar.SamplingParams(temperature=0.0), max_new_tokens=6, ignore_eos=True)
+        out += engine.generate([[5, 6, 7]], siar.SamplingParams(temperature=0.0), max_new_tokens=6, ignore_eos=True)
+        del engine
+        gc.collect()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return out, torch.cuda.memory_allocated(), torch.cuda.memory_reserved()
+
+    held(False)
+    eager = held(False)
+    assert held(True) == eager and held(True) == eager
+
+
+def test_captures_on_one_stream_let_go_of_each_others_workspaces():
+    """One's own captures, without an engine: an eager call or another capture on the stream lets the last one's go, and every
+    graph still gives its result."""
+    from simple_inference_autoresearch_b200.kernels import kv_quant
+    b = eq.Batch(8, 8, 2, 128, [2000, 70], [1, 1], seed=2)
+    kv, qkv, meta = b.entry(DEV), b.qkv.to(DEV), b.meta(DEV)
+    call = lambda: ops.rope_and_attention(qkv, None, kv, meta, *b.sizes(), 0.09)  # noqa: E731
+    want = call()
+    side, graphs = torch.cuda.Stream(), []
+    for _ in range(3):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs = [call() for _ in range(2)]
+        graphs.append((g, outs))
+        assert len([k for k in kv_quant._captured_workspaces if k[1] == side.cuda_stream]) == 1
+    with torch.cuda.stream(side):
+        assert torch.equal(call(), want)
+    assert not [k for k in kv_quant._captured_workspaces if k[1] == side.cuda_stream]
+    torch.cuda.synchronize()
+    filler = [torch.full((1 << 22,), 7.0, device=DEV) for _ in range(4)]        # what was let go is not the eager pool's to hand out
+    for _ in range(3):
+        for g, outs in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, want) for o in outs)
+    assert all(bool((f == 7.0).all()) for f in filler)
+    ops.check_status(DEV)
