@@ -11,7 +11,7 @@ from simple_inference_autoresearch_b200.cache import CacheError, QuantizedKVEntr
 from simple_inference_autoresearch_b200.kernels import kv_quant, ops
 from simple_inference_autoresearch_b200.parts.base import KVNeed, StateNeed
 from tests import emulated_kv_quant as eq
-from tests import plain_llama, tiny_configs
+from tests import kv_quant_engine, plain_llama, tiny_configs
 
 
 def cache(kv_format, need=KVNeed(2, 80), **kw):
@@ -222,3 +222,24 @@ def test_an_engine_names_the_units_of_its_cache(tmp_path, config, dtype, units):
     assert kv_quant.extension_units([None, StateNeed((3,))], torch.bfloat16, 64) == ()
     assert kv_quant.extension_units([KVNeed(2, 128, window=9)], torch.bfloat16, 64) == ("kv_quant",)
     assert kv_quant.extension_units([KVNeed(2, 128)], torch.bfloat16, 16) == ("kv_quant",)
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+@pytest.mark.parametrize("config", ["C", "D", "E"])
+def test_faults_exceed_the_bounds_of_the_engines_comparison(tmp_path, monkeypatch, kv_format, config):
+    """What the comparison on the GPU allows would not hide a fault: planted in the restated functions, each is three times
+    beyond it, and a cache that is not quantised (its logits) twice where 4 bits make that much of a difference."""
+    folder = kv_quant_engine.folder_of(tmp_path, config)
+
+    def run(fault=None, fmt=kv_format):
+        with monkeypatch.context() as m:
+            kv_quant_engine.restated(m, fault)
+            return kv_quant_engine.run(folder, "cpu", fmt)
+
+    right = run()
+    assert kv_quant_engine.distances(run(), right) == ([0.0] * 4, 0.0)
+    for fault in kv_quant_engine.FAULTS:
+        assert not kv_quant_engine.within(kv_format, run(fault), right, times=3), fault
+    if kv_format == "int4":
+        plain = run(fmt=None)[1]
+        assert float((plain - right[1]).norm() / right[1].norm()) > 2 * kv_quant_engine.LOGIT_BOUND

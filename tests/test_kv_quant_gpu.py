@@ -895,3 +895,43 @@ def test_captures_on_one_stream_let_go_of_each_others_workspaces():
             assert all(torch.equal(o, want) for o in outs)
     assert all(bool((f == 7.0).all()) for f in filler)
     ops.check_status(DEV)
+
+
+WAYS = {"as by default": {}, "rotation and store in front": {"fuse_decode_rope": False},
+        "no tcgen05": {"use_tc_attention": False}, "no tensor cores": {"use_mma_attention": False}}
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("step", [*STEPS, "a chunk and long tokens"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (6, 2, 128), (16, 1, 128)])
+@pytest.mark.parametrize("way", list(WAYS)[1:])
+def test_attention_with_kernels_switched_off(bits, heads, kv_heads, dim, step, way):
+    """Every choice that KernelOptions offers over a quantised cache, with the cache it leaves."""
+    held, new = {**STEPS, **MIXED}[step]
+    b = eq.Batch(bits, heads, kv_heads, dim, held, new, seed=heads + dim)
+    inv, scale, options = freqs(dim), dim ** -0.5, OPTS.but(**WAYS[way])
+    kv = b.entry(DEV)
+    out = ops.rope_and_attention(b.qkv.to(DEV), inv.to(DEV), kv, b.meta(DEV), *b.sizes(), scale, options=options)
+    ops.check_status(DEV)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), inv, want, b.meta(), *b.sizes())
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+    pos = [c + i for c, n in zip(held, new) for i in range(n)]
+    check_attention(b, out, eq.rotate(b.qkv.view(b.tokens, -1, dim)[:, :heads].float(), pos, inv), want, scale)
+
+
+@pytest.mark.parametrize("kv_format", ["int8", "int4"])
+@pytest.mark.parametrize("config", ["C", "D", "E"])
+@pytest.mark.parametrize("way", list(WAYS))
+def test_engine_codes_and_logits_against_the_restated_kernels(tmp_path, monkeypatch, kv_format, config, way):
+    """A model whose results depend on its attention: the codes that both layers leave in the cache and every step's logits,
+    within bounds that planted faults exceed (test_kv_quant.py plants them)."""
+    from tests import kv_quant_engine
+    folder = kv_quant_engine.folder_of(tmp_path, config)
+    got = kv_quant_engine.run(folder, DEV, kv_format, options=OPTS.but(**WAYS[way]))
+    ops.check_status(DEV)
+    with monkeypatch.context() as m:
+        kv_quant_engine.restated(m)
+        want = kv_quant_engine.run(folder, "cpu", kv_format)
+    assert kv_quant_engine.within(kv_format, got, want), kv_quant_engine.distances(got, want)
