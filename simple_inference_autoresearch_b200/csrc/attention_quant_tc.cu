@@ -218,11 +218,11 @@ attn_quant_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           tma_load_2d(v_s + s * kTileBytes + h * (kTileBytes / kHalves), &tmV, &v_full[s], 64 * h, row);
         issued_v = i + 1;
       }
-      if (SIAR_ABORTED()) {    // let copies in flight land before the block leaves
-        mbar_wait(&q_full, 0);
-        for (int i = max(0, issued_k - kStages); i < issued_k; ++i) mbar_wait(&k_full[i % kStages], (i / kStages) & 1);
-        for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
-      }
+      // Copies in flight land before the block leaves, whoever gives up and when: the last ones may be under way when every
+      // load has been issued.
+      mbar_wait(&q_full, 0);
+      for (int i = max(0, issued_k - kStages); i < issued_k; ++i) mbar_wait(&k_full[i % kStages], (i / kStages) & 1);
+      for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
     }
   } else if (warp == 1 || warp == 3) {
     // ---------------- MMA issue: warp 1 the scores, warp 3 P.V.  One thread issues; the whole warp walks along, so that all it

@@ -187,11 +187,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         issued_v = i + 1;
       }
       if (bad_page) atomicOr(prm.status, kStatusBadPage);
-      if (SIAR_ABORTED()) {    // let copies in flight land before the block leaves
-        mbar_wait(&q_full, 0);
-        for (int i = max(0, issued_k - kStages); i < issued_k; ++i) mbar_wait(&k_full[i % kStages], (i / kStages) & 1);
-        for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
-      }
+      // Copies in flight land before the block leaves, whoever gives up and when: the last ones may be under way when every
+      // load has been issued.
+      mbar_wait(&q_full, 0);
+      for (int i = max(0, issued_k - kStages); i < issued_k; ++i) mbar_wait(&k_full[i % kStages], (i / kStages) & 1);
+      for (int i = max(0, issued_v - kStages); i < issued_v; ++i) mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
     }
   } else if (warp == 1 || warp == 2) {
     // ---------------- MMA issue: one thread per query tile (the two tiles depend on nothing of

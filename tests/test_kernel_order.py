@@ -33,3 +33,13 @@ def test_tensor_memory_is_taken_between_the_wait_and_the_next_kernels_start():
     body = body_of("attention_quant_tc", "attn_quant_tc_kernel")
     assert body.index("pdl_wait();") < body.index("tmem_alloc(") < body.index("__syncthreads();") < body.index("pdl_launch_dependents();")
     assert body.count("pdl_launch_dependents();") == 1 and body.count("tmem_alloc(") == 1
+
+
+@pytest.mark.parametrize("unit,kernel", [("attention_tc", "attn_prefill_tc_kernel"), ("attention_quant_tc", "attn_quant_tc_kernel")])
+def test_the_loading_thread_waits_for_its_last_copies_on_every_way_out(unit, kernel):
+    """Another warp may give up after the last load was issued: the copies have to land before the block leaves all the same."""
+    body = body_of(unit, kernel)
+    at = body.index("for (int i = max(0, issued_k - kStages); i < issued_k; ++i) mbar_wait(&k_full")
+    loop_end = body.rindex("issued_v = i + 1;", 0, at)
+    between = body[loop_end:at]
+    assert "if (" not in between.replace("if (bad_page)", "") and "mbar_wait(&q_full, 0);" in between
