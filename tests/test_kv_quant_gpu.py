@@ -935,3 +935,47 @@ def test_engine_codes_and_logits_against_the_restated_kernels(tmp_path, monkeypa
         kv_quant_engine.restated(m)
         want = kv_quant_engine.run(folder, "cpu", kv_format)
     assert kv_quant_engine.within(kv_format, got, want), kv_quant_engine.distances(got, want)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_a_batch_of_both_kinds_captured_padded_and_repeated(bits):
+    """Long and short runs in one call: the same from a graph, on another stream and with rows behind the last sequence, which
+    the store leaves out."""
+    heads, kv_heads, dim = 8, 2, 128
+    b = eq.Batch(bits, heads, kv_heads, dim, [2100, 0, 50, 1400], [1, 90, 3, 40], seed=6)
+    pad = torch.randn(21, b.qkv.shape[1], generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    kv, inv, meta = b.entry(DEV), freqs(dim).to(DEV), b.meta(DEV)
+    padded_meta = b.meta(DEV)
+    padded_meta.n_tokens += len(pad)
+    qkv, padded = b.qkv.to(DEV), torch.cat([b.qkv, pad]).to(DEV)
+    call = lambda x, m: ops.rope_and_attention(x, inv, kv, m, *b.sizes(), 0.09)  # noqa: E731
+    first = call(qkv, meta)
+    want = b.entry()
+    eq.rope_kv_write(b.qkv.clone(), freqs(dim), want, b.meta(), *b.sizes())
+    assert torch.equal(call(padded, padded_meta)[:b.tokens], first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [call(qkv, meta), call(padded, padded_meta)]
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o[:b.tokens], first) for o in outs)
+        with torch.cuda.stream(side):
+            assert torch.equal(call(qkv, meta), first)
+        torch.cuda.synchronize()
+    ops.check_status(DEV)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert same(getattr(kv, name).cpu().float(), getattr(want, name).float()), name
+
+
+def test_host_lengths_that_do_not_agree_are_refused():
+    b = eq.Batch(8, 8, 2, 64, [70, 2100], [90, 1], seed=1)
+    meta = b.meta(DEV)
+    meta.q_lens = [1, 1]
+    with pytest.raises(ValueError, match="do not agree"):
+        attend(b, b.entry(DEV), scale=0.1, meta=meta)
