@@ -29,10 +29,16 @@
 // at most two steps more a block, it gets them: a border costs about that much.  A unit that was cut is joined
 // in block order by the block that finishes it last.
 //
-// Measured (keys and values at the measured copy rate in brackets): 64 sequences of up to 4,500 keys, 8 bits, 32 heads on
-// 8, 80 us (71); 64 of up to 9,000 in 4 bits 96 (77); one of 130,018 in 8 bits 50 (42); one of 34 keys 6.2, the
-// latency of the chain batch -> block table -> keys -> softmax -> values.  Three blocks an SM for 8 bits 82 us, rings of
-// four stages there 83.
+// Measured from a graph (keys and values at the measured copy rate in brackets; calls one by one take 2 to 8 % more): 64
+// sequences of up to 4,500 keys, 8 bits, 32 heads on 8, 80 us (71); 64 of up to 9,000 in 4 bits 96 (77); one of 130,018
+// in 8 bits 50 (42); one of 34 keys 6.2, the latency of the chain batch -> block table -> keys -> softmax -> values.  Three
+// blocks an SM for 8 bits 82 us, rings of four stages there 83.  4 bits are bound by issue: 0.47 instructions a cycle and
+// scheduler with two warps on it, 47 million of them for the 64 sequences (8 bits: 0.29).
+// More rows a kv head repeat products and softmax for every tile of four: 64 sequences of up to 4,500 with groups of 8 take
+// 87 us (8 bits; 71) and 82 (4 bits; 39), 32 of them with groups of 16 71 (36) and 89 (20); 4 new tokens on 6 of up to 16,000 47
+// (18.6) and 55 (10.2).  The instances of 8 and 16 rows at 128 dims use all 255 registers and spill (bytes stored / loaded:
+// 8 bits, 16 rows 48 / 36; 4 bits, 8 rows 56 / 52, 16 rows 280 / 224), outside the steps: 0.1 and 0.2 % of the instructions.  64 dims take a step's fixed work for half the bytes: two of
+// 60,001 in 4 bits 23 (10), in 8 bits 29 (19).
 #include "attention_mma.cuh"
 #include "kv_quant.cuh"
 #include "load_ring.h"

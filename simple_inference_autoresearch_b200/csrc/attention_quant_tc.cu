@@ -13,6 +13,10 @@
 //                   the GPU the keys of a block of rows are cut into parts;
 //   attn_quant_join adds the parts up.
 //
+// Roundings to fewer bits: queries, keys, values and P to float16 (11 bits of each; the sum of P takes the unrounded ones).
+// They are small beside the result's own to bfloat16: relative error against 64 bits 0.00177 for the chunk below, 0.00169
+// with 32 bits throughout.
+//
 // All of it, with the kernel that stores the tokens, takes 64 us for a prompt of 2,048 tokens (4 bits, 32 heads on 8, 128
 // dims; its products at the measured matrix rate 21 us) and 99 us for a chunk of 515 on 8,191 held (8 bits, 24 on 8; 32
 // us).  The chunk's kernels one by one: 9 us storing, 16 widening, 75 the products, 10 joining (they overlap at their
@@ -666,7 +670,10 @@ SIAR_DEFINE_PDL_SWITCH()
 // every SM 0.66 us a tile and SM, the last round a third of a block more; parts (`row_floats` floats each) are written and
 // read again at 3.6 TB/s by a kernel of its own.  A chunk of 128 tokens on 8,000 held (32 heads on 8): one part 139 us, 8
 // parts 54; a chunk of 515 on 8,191 (24 on 8): parts 1, 2, 3, 4, 5, 6, 8 take 134, 101, 114, 99, 97, 109, 109 us (the rule
-// takes 4); a prompt of 2,048: one part 64 us, two over 100.
+// takes 4); a prompt of 2,048: one part 64 us, two over 100.  Where its estimate is furthest off: 1,000 tokens of 8 heads on 1 on
+// 20,000 held take 127 us with the rule's 7 parts, 103 with 4; 256 on 60,000 343 with 13, 318 with 4.  The constants are those
+// of 128 dims; at 64 dims (us, the rule's choice and the best of 1 to 16): 128 on 8,000 44 (10 parts) and 37 (8), 515 on
+// 8,191 89 (6) and 80 (5), 300 on 2,000 30 (3) and 30, four times 64 on 16,000 93 (11) and 91 (6), prompts one part and best.
 extern "C" int siar_attn_quant_tc_parts(int blocks, int longest, float average, long long row_floats, int sms) {
   int best = 1;
   float best_cost = 1e30f;

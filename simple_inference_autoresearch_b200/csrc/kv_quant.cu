@@ -9,8 +9,10 @@
 //           high half), scales bfloat16 [pages][Hkv][page_tokens][ceil(D/64)][2]: for every run of 64
 //           dims s = bf16(max(x) (1/15) - min(x) (1/15)), m = bf16(min(x) + 8 s), c_d = rint((x_d - m) / s) + 8
 //           within 0..15, value (c_d - 8) * s + m.  s and m are rounded to 16 bits because they are a
-//           ninth of the format's bytes; the codes are taken against the rounded ones, so that costs
-//           at most 15 * 2^-9 steps at the ends of the range.
+//           ninth of the format's bytes; the codes are taken against the rounded ones.  The scale is off by at most
+//           2^-8 of itself, 15 * 2^-9 steps at the ends of the range.  The mid is off by at most 2^-8 of itself,
+//           which for a run that lies far from zero beside its own range is many steps: of 100 and 100.5 (s = 0.0334,
+//           m = 100.5 for 100.27) the lower one reads back as 100.23, seven steps off, its code at the end.
 // A row (8 bits) or run (4 bits) that holds an infinity or a NaN gets the scale NaN and reads back as
 // NaN: it is not turned into ordinary numbers.  A constant run has s = 0 and reads back as m.
 //

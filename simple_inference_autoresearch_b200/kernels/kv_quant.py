@@ -187,8 +187,10 @@ def read_kv(kv, meta, dtype: torch.dtype, window: Optional[int] = None, options:
 # ------------------------------------------------------------------ attention
 #: query rows (new tokens x heads of a group) a sequence may bring to the kernel that works on the codes; a longer run
 #: widens the cache once for the tensor-core kernel instead of walking the codes for every 16 rows.  Measured on B200,
-#: four sequences of 4,000 held positions (8 bits, 32 heads on 8, 128 dims): 64 rows 33 us against 40, 256 rows 83
-#: against 54; one sequence of 500: 64 rows 19 us against 18
+#: codes against tiles in us, 32 heads on 8.  Four sequences of 4,000 held positions, 128 dims: 64 rows 33 and 41 (4 bits 41
+#: and 43), 96 rows 50 and 43 (64 and 44), 256 rows 86 and 51; 64 dims: 64 rows 25 and 33 (4 bits 27 and 34), 128 rows 32 and 31
+#: (35 and 32).  One sequence of 500: 64 rows 20 and 17 (4 bits 24 and 17; 64 dims 19 and 15), of 16,000 44 and 52 (52 and 52; 30
+#: and 37)
 MOST_ROWS = 64
 
 

@@ -591,7 +591,8 @@ def attention(qkv: torch.Tensor, kv, meta, n_heads: int, n_kv_heads: int, head_d
     with head_dim 64 or 128 runs on the tensor cores, everything else on the CUDA cores.
     ``window`` = w: a query at position p sees keys p - w + 1 .. p only (CUDA-core kernels).
     Over a ``QuantizedKVEntry`` single tokens and short runs in bfloat16 (head_dim 64 or 128) work on the
-    codes, longer runs and prompts on the cache widened to float16 tiles, everything else on the cache read back as
+    codes, longer runs and prompts on the cache widened to float16 tiles, each sequence of a batch by its own length where the
+    short ones' keys are worth a launch, everything else on the cache read back as
     pages of qkv's dtype (``read_kv``)."""
     if kv_quant.is_quantized(kv):
         return kv_quant.attention(qkv, kv, meta, n_heads, n_kv_heads, head_dim, scale, window, options)
