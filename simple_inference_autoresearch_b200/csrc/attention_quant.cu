@@ -10,7 +10,7 @@
 // for the small elements of a row in which one stands out, where bfloat16 would keep 8 bits of each), split into two
 // bytes that take two columns of the product; the integer scores are exact.  For the value product the p_j sv_j of one step of keys become
 // whole numbers of 16 bits too, against the largest of the step, again two bytes in two columns: within a
-// step 2^-17 of the largest is lost, and a step's integer sum goes into the 32-bit accumulators with the
+// step 2^-17 of the largest is lost (the sum of p, and in 4 bits the mids' share, take p unrounded), and a step's integer sum goes into the 32-bit accumulators with the
 // step's own factor, so nothing is lost between steps.  Statistics and sums are 32 bits.
 //
 // Shape.  The products are taken transposed, keys (then value dims) on the MMA's 16 rows and the query
