@@ -8,10 +8,11 @@
 //           out_g = (sum_j (p_j sv_jg) cv_jg + sum_j p_j (mv_jg - 8 sv_jg)) / sum_j p_j
 // A query row becomes whole numbers of 16 bits in both formats (largest element 32512: a step is 1 / 32512 of it, also
 // for the small elements of a row in which one stands out, where bfloat16 would keep 8 bits of each), split into two
-// bytes that take two columns of the product; the integer scores are exact.  For the value product the p_j sv_j of one step of keys become
-// whole numbers of 16 bits too, against the largest of the step, again two bytes in two columns: within a
-// step 2^-17 of the largest is lost (the sum of p, and in 4 bits the mids' share, take p unrounded), and a step's integer sum goes into the 32-bit accumulators with the
-// step's own factor, so nothing is lost between steps.  Statistics and sums are 32 bits.
+// bytes that take two columns of the product; the integer scores are exact.  For the value product the p_j sv_j of one
+// step of keys become whole numbers of 16 bits too, against the largest of the step, again two bytes in two columns:
+// within a step 2^-17 of the largest is lost (the sum of p, and in 4 bits the mids' share, take p unrounded), and a
+// step's integer sum goes into the 32-bit accumulators with the step's own factor, so nothing is lost between steps.
+// Statistics and sums are 32 bits.
 //
 // Shape.  The products are taken transposed, keys (then value dims) on the MMA's 16 rows and the query
 // rows on its columns, four of them (times two bytes) a tile of eight: with four query heads to a
