@@ -60,8 +60,9 @@ class Engine:
             max_tokens = self.max_batch * round_up(max_seq_len, page_tokens)
         self.cache = SequenceCache(model.cache_needs, int(max_tokens), int(max_slots or self.max_batch),
                                    max_seq_len, model.dtype, self.device, page_tokens, kv_cache)
-        if self._cuda:            # compiled here, not inside the first step
-            build.ensure_built(self.extension_units())
+        units = self.extension_units()
+        if units and self._cuda:  # compiled here, not inside the first step
+            build.ensure_built(units)
         self.max_seq_len = self.cache.max_seq_len
         self.use_cuda_graph = bool(use_cuda_graph)
         self._graphs: Dict[Tuple[int, int], "_DecodeGraph"] = {}      # in order of last use
